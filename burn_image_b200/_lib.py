@@ -24,6 +24,7 @@ ACT_NONE, ACT_GELU_TANH, ACT_SILU = 0, 1, 2
 NOALLOC_SCRATCH_BYTES = 32 << 20  # BQ4_NOALLOC_SCRATCH_BYTES
 NUMERICS_AUTO, NUMERICS_EXACT, NUMERICS_FOLDED = 0, 1, 2
 DTYPE_F32, DTYPE_F16 = 0, 1
+CACHE_F16, CACHE_Q8, CACHE_Q4 = 0, 1, 2
 MAX_PEERS = 8            # BQ4_MAX_PEERS
 IPC_HANDLE_BYTES = 64    # BQ4_IPC_HANDLE_BYTES
 
@@ -90,6 +91,13 @@ SIGNATURES = {
     "bq4_packed_f16_conv2d": (_st, [_p, _i64, _i64, _i64, _i64, _p, _i64, _i32, _i32, _p, _p, _p, _p, _sz, _p]),
     "bq4_attention_workspace_size": (_st, [_i64, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_sz)]),
     "bq4_attention": (_st, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _p, _p, _sz, _p]),
+    "bq4_cache_sizes": (_st, [_p, ctypes.POINTER(_sz), ctypes.POINTER(_sz)]),
+    "bq4_cache_append": (_st, [_p, _p, _p, _p, _p, _p, _i32, _i64, _p]),
+    "bq4_cache_read": (_st, [_p, _p, _p, _i64, _p, _p, _p, _i32, _p]),
+    "bq4_cache_attention_workspace_size": (_st, [_p, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_sz)]),
+    "bq4_cache_attention": (_st, [_p, _p, _i64, _p, _p, _i64, _i64, _i32, ctypes.c_float, _p, _p, _sz, _p]),
+    "bq4_cache_prefix_attention": (_st, [_p, _p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _i32, ctypes.c_float, _p, _p,
+                                         _sz, _p]),
     "bq4_launch_count": (_u64, []),
     "bq4_launch_count_reset": (None, []),
 }
@@ -104,6 +112,17 @@ class QuantScheme(ctypes.Structure):
 class Conv2dOptions(ctypes.Structure):
     """bq4_conv2d_options: Burn ConvOptions<2> ([height, width] pairs, groups)."""
     _fields_ = [("stride", _i32 * 2), ("padding", _i32 * 2), ("dilation", _i32 * 2), ("groups", _i32)]
+
+
+class Cache(ctypes.Structure):
+    """bq4_cache: the buffers and geometry of a paged key/value cache."""
+    _fields_ = [("values", _p), ("scales", _p), ("pages", _i64), ("page_size", _i32), ("kv_heads", _i32),
+                ("head_dim", _i32), ("format", _i32), ("device", _i32)]
+
+
+class CacheSequences(ctypes.Structure):
+    """bq4_cache_sequences: page table and lengths of a call's sequences."""
+    _fields_ = [("page_table", _p), ("table_stride", _i64), ("table_width", _i64), ("lengths", _p), ("batch", _i64)]
 
 
 class Bq4Error(RuntimeError):

@@ -1,0 +1,69 @@
+// bq4_cache.h -- layout of the paged key/value cache, shared by its kernels.
+//
+// One page holds page_size consecutive tokens of one sequence, for every kv
+// head.  Rows are padded to HP = 64 or 128 values (head_dim rounded up):
+//   values u8  [pages][kv_heads][2 (k, v)][page_size][row_bytes]
+//   scales u16 [pages][kv_heads][page_size][2 (k, v)][nb]        (bf16 bits)
+// so that the k rows (and the v rows) of one page and head are contiguous.
+//   f16: 2 HP bytes, no scales.
+//   q8:  byte d holds q_d + 128; one scale for the row (nb = 1).
+//   q4:  a nibble holds q + 8; one scale for each 32 values (nb = HP / 32).
+//        The nibbles are placed for the lanes that feed the tensor core:
+//        k: the 8 values 32 b + 8 t .. + 7 form word t nb + b; within it
+//           value 2 p sits in nibble p and value 2 p + 1 in nibble p + 4, so
+//           (w >> 4 p) & 0x000F000F is the pair (2 p, 2 p + 1).
+//        v: the 4 values 32 b + 4 g .. + 3 form u16 g nb + b, in order.
+// Padding values are q = 0 with scale 0 (f16: 0).
+#pragma once
+#include "bq4_internal.h"
+
+namespace bq4 {
+
+constexpr int kCacheBlock = 32;       // values under one q4 scale
+constexpr int kCachePageUnit = 16;    // page sizes are multiples of this
+constexpr int kCacheMaxHeadDim = 128;
+
+struct CacheView {
+  uint8_t* values;
+  uint16_t* scales;
+  int32_t pages, page_size, kv_heads, head_dim;
+  int32_t hp, nb, row_bytes;  // padded head, scales of a row, bytes of a row
+  int32_t format;
+  int64_t kv_bytes;           // k (or v) rows of one page and head
+};
+
+struct SeqView {
+  const int32_t* table;
+  const int32_t* lengths;
+  int64_t table_stride;
+  int32_t table_width, batch;
+};
+
+inline int cache_hp(int head_dim) { return head_dim <= 64 ? 64 : 128; }
+inline int cache_nb(int format, int hp) {
+  return format == BQ4_CACHE_Q8 ? 1 : format == BQ4_CACHE_Q4 ? hp / kCacheBlock : 0;
+}
+inline int cache_row_bytes(int format, int hp) {
+  return format == BQ4_CACHE_F16 ? 2 * hp : format == BQ4_CACHE_Q8 ? hp : hp / 2;
+}
+
+// Arguments of one attention call (bq4_cache_attn.cu).
+struct CacheAttnCall {
+  CacheView c;
+  SeqView s;
+  const int32_t* prefix_table;   // null: no prefix
+  const int32_t* prefix_length;  // one value on the device
+  int32_t prefix_width;
+  const uint16_t* q;             // f16
+  int64_t q_stride[3];           // batch, token, head
+  uint16_t* out;                 // f16 [batch][tokens][q_heads][head_dim]
+  int32_t tokens, q_heads, causal;
+  int32_t max_length;            // lengths are at most this
+  float scale;                   // of the scores
+  int* err;
+};
+
+size_t cache_attn_workspace(const CacheAttnCall& c, int sms);
+bq4_status run_cache_attn(const CacheAttnCall& c, int sms, void* workspace, cudaStream_t s);
+
+}  // namespace bq4

@@ -1,0 +1,189 @@
+"""A paged, optionally quantised key/value cache and the attention that reads
+it, over libbq4 (the ``bq4_cache_*`` calls of include/bq4.h).
+
+The q/k/v projections leave k and v rows; ``KVCache.append`` quantises the
+newest of them into the cache, ``KVCache.attention`` attends the newest query
+tokens with what is cached, ``KVCache.prefix_attention`` does so for a batch
+whose sequences share their first rows, and ``KVCache.read`` widens rows for a
+consumer of contiguous k and v such as ``f16.attention``.
+
+Sequences are given by two int32 tensors on the cache's device: a page table
+[B, W] (position p of sequence b is row p % page_size of page
+``page_table[b, p // page_size]``) and lengths [B], the rows that each
+sequence holds, the newest included.  Nothing is copied to the host, so calls
+can be captured into a CUDA graph and replayed with new tables and lengths in
+the same tensors.  All arithmetic runs in the CUDA kernels; there is no CPU
+fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib as L
+from ._lib import Bq4Error, check
+
+FORMATS = {"f16": L.CACHE_F16, "q8": L.CACHE_Q8, "q4": L.CACHE_Q4}
+_DTYPES = {torch.float32: L.DTYPE_F32, torch.float16: L.DTYPE_F16}
+_Strides = ctypes.c_int64 * 3
+
+
+class KVCache:
+    """``pages`` pages of ``page_size`` tokens (a multiple of 16) for
+    ``kv_heads`` heads of ``head_dim`` values (a multiple of 8, at most 128).
+    format "f16": rows rounded to binary16; "q8": 8 bits a value and one scale
+    a row; "q4": 4 bits a value and one scale for each 32 values (symmetric,
+    q * scale, bf16 scales).  Which page holds what is the caller's business:
+    the cache keeps no page table of its own."""
+
+    def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, format: str = "q8",
+                 device: Optional[torch.device] = None):
+        if format not in FORMATS:
+            raise Bq4Error(L.EINVAL_ARG, f"format {format!r} is not one of {', '.join(FORMATS)}")
+        c = L.Cache(None, None, pages, page_size, kv_heads, head_dim, FORMATS[format], 0)
+        nv, ns = ctypes.c_size_t(), ctypes.c_size_t()
+        check(L.lib().bq4_cache_sizes(ctypes.byref(c), ctypes.byref(nv), ctypes.byref(ns)))
+        dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        if dev.type != "cuda":
+            raise Bq4Error(L.EINVAL_ARG, "a key/value cache lives on a CUDA device")
+        if dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        self.pages, self.page_size, self.format = pages, page_size, format
+        self.kv_heads, self.head_dim = kv_heads, head_dim
+        self.device = dev
+        self.values = torch.zeros(nv.value, dtype=torch.uint8, device=dev)
+        self.scales = torch.zeros(ns.value, dtype=torch.uint8, device=dev)
+        c.values, c.scales, c.device = self.values.data_ptr(), self.scales.data_ptr() or None, dev.index
+        self._c = c
+        self._ref = ctypes.byref(c)
+
+    @property
+    def device_bytes(self) -> int:
+        return self.values.numel() + self.scales.numel()
+
+    def _stream(self):
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _ints(self, t: torch.Tensor, what: str, dim: int) -> torch.Tensor:
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self.device or t.dim() != dim \
+                or (t.numel() > 1 and t.stride(-1) != 1):
+            raise Bq4Error(L.EINVAL_ARG,
+                           f"{what} must be int32 with {dim} dimension(s) and unit stride on {self.device}")
+        return t
+
+    def _sequences(self, page_table: torch.Tensor, lengths: torch.Tensor, batch: Optional[int] = None):
+        self._ints(page_table, "page_table", 2)
+        self._ints(lengths, "lengths", 1)
+        b, w = page_table.shape
+        if lengths.shape[0] != b or (batch is not None and batch != b):
+            raise Bq4Error(L.EINVAL_SHAPE, f"page_table holds {b} sequences, lengths {lengths.shape[0]}"
+                           + (f", the rows {batch}" if batch is not None else ""))
+        return L.CacheSequences(page_table.data_ptr() or None, page_table.stride(0), w, lengths.data_ptr() or None, b)
+
+    def _rows(self, t: torch.Tensor, what: str, heads: Optional[int]) -> torch.Tensor:
+        if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype not in _DTYPES:
+            raise Bq4Error(L.EINVAL_ARG, f"{what} must be float32 or float16 on {self.device}")
+        if t.dim() != 4 or t.shape[3] != self.head_dim or (heads is not None and t.shape[2] != heads):
+            raise Bq4Error(L.EINVAL_SHAPE,
+                           f"{what} must be [B, S, {heads or 'heads'}, {self.head_dim}], got {tuple(t.shape)}")
+        return t if t.stride(3) == 1 or t.numel() == 0 else t.contiguous()
+
+    def append(self, key: torch.Tensor, value: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor) -> None:
+        """Quantise the newest rows of every sequence into the cache: key and
+        value [B, S, kv_heads, head_dim] (float32 or float16, any strides; a
+        view of the projection's output will do), row i of sequence b to
+        position lengths[b] - S + i.  Positions below 0 are skipped, so a padded batch
+        aligns its rows at their ends.  Sequences that share a page must not
+        write the same row."""
+        k = self._rows(key, "key", self.kv_heads)
+        v = self._rows(value, "value", self.kv_heads)
+        if v.shape != k.shape or v.dtype != k.dtype:
+            raise Bq4Error(L.EINVAL_SHAPE, "key and value must have one shape and type")
+        seqs = self._sequences(page_table, lengths, k.shape[0])
+        ks, vs = k.stride(), v.stride()
+        check(L.lib().bq4_cache_append(self._ref, ctypes.byref(seqs), k.data_ptr() or None,
+                                       _Strides(ks[0], ks[1], ks[2]), v.data_ptr() or None,
+                                       _Strides(vs[0], vs[1], vs[2]), _DTYPES[k.dtype], k.shape[1], self._stream()))
+
+    def read(self, page_table: torch.Tensor, lengths: torch.Tensor, count: int,
+             starts: Optional[torch.Tensor] = None,
+             dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
+        """k and v [B, kv_heads, count, head_dim] of positions starts[b] + i
+        (starts: int32 [B]; None reads from 0), q * scale rounded once to
+        ``dtype`` (float16 or float32).  A position below 0 or behind the
+        sequence's length reads as 0."""
+        seqs = self._sequences(page_table, lengths)
+        if dtype not in _DTYPES:
+            raise Bq4Error(L.EINVAL_ARG, f"rows are read as float16 or float32, not {dtype}")
+        if count < 0:
+            raise Bq4Error(L.EINVAL_SHAPE, f"count={count}")
+        if starts is not None and self._ints(starts, "starts", 1).shape[0] != seqs.batch:
+            raise Bq4Error(L.EINVAL_SHAPE, f"starts holds {starts.shape[0]} sequences, page_table {seqs.batch}")
+        shape = (seqs.batch, self.kv_heads, count, self.head_dim)
+        k = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty(shape, dtype=dtype, device=self.device)
+        st = k.stride()
+        check(L.lib().bq4_cache_read(self._ref, ctypes.byref(seqs), starts.data_ptr() if starts is not None else None,
+                                     count, k.data_ptr() or None, v.data_ptr() or None, _Strides(st[0], st[1], st[2]),
+                                     _DTYPES[dtype], self._stream()))
+        return k, v
+
+    def attention(self, query: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, causal: bool = True,
+                  scale: Optional[float] = None, max_length: Optional[int] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """softmax(scale * q k^T) v of the newest query tokens over the cached
+        rows: query float16 [B, S, q_heads, head_dim], query head h on kv head
+        h // (q_heads // kv_heads).  causal: query i of sequence b sees
+        positions below lengths[b] - S + i + 1, else every row.  A query that
+        sees nothing gives 0.  Returns float16 [B, S, q_heads, head_dim].
+        scale None: 1 / sqrt(head_dim).  max_length: a bound of the lengths
+        known to the host, by which the keys are split (None: the page
+        table's width)."""
+        return self._attention(query, None, None, page_table, lengths, causal, scale, max_length, out)
+
+    def prefix_attention(self, query: torch.Tensor, prefix_pages: torch.Tensor, prefix_length: torch.Tensor,
+                         page_table: torch.Tensor, lengths: torch.Tensor, causal: bool = True,
+                         scale: Optional[float] = None, max_length: Optional[int] = None,
+                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``attention`` for a batch whose sequences begin with the same rows:
+        every query sees the first prefix_length (int32 [1]) rows of the page
+        list prefix_pages (int32 [W]), read once for the whole batch, and then
+        its own sequence; page_table, lengths, causal and max_length are about
+        the sequences' own rows."""
+        self._ints(prefix_pages, "prefix_pages", 1)
+        if self._ints(prefix_length, "prefix_length", 1).shape[0] != 1:
+            raise Bq4Error(L.EINVAL_SHAPE, "prefix_length must hold one value")
+        return self._attention(query, prefix_pages, prefix_length, page_table, lengths, causal, scale, max_length, out)
+
+    def _attention(self, query, prefix_pages, prefix_length, page_table, lengths, causal, scale, max_length, out):
+        q = self._rows(query, "query", None)
+        if q.dtype != torch.float16:
+            raise Bq4Error(L.EINVAL_ARG, "query must be float16")
+        B, S, Hq, D = q.shape
+        seqs = self._sequences(page_table, lengths, B)
+        if out is None:
+            out = torch.empty((B, S, Hq, D), dtype=torch.float16, device=self.device)
+        elif out.shape != q.shape or out.dtype != torch.float16 or out.device != self.device or not out.is_contiguous():
+            raise Bq4Error(L.EINVAL_ARG, f"out must be contiguous float16 {tuple(q.shape)} on {self.device}")
+        held = seqs.table_width * self.page_size
+        longest = held if max_length is None else max_length
+        if longest < 0:
+            raise Bq4Error(L.EINVAL_SHAPE, f"max_length={max_length}")
+        lib = L.lib()
+        n = ctypes.c_size_t()
+        width = prefix_pages.shape[0] if prefix_pages is not None else 0
+        check(lib.bq4_cache_attention_workspace_size(self._ref, B, S, Hq, min(longest, held) or held,
+                                                     width * self.page_size, ctypes.byref(n)))
+        # a workspace of the call's own: calls on several streams, and graphs captured side by side, never share one
+        ws = torch.empty(n.value, dtype=torch.uint8, device=self.device) if n.value else None
+        qs = _Strides(*q.stride()[:3])
+        tail = (q.data_ptr() or None, qs, S, Hq, 1 if causal else 0, float(scale or 0.0), out.data_ptr() or None,
+                ws.data_ptr() if ws is not None else None, n.value, self._stream())
+        if prefix_pages is None:
+            check(lib.bq4_cache_attention(self._ref, ctypes.byref(seqs), longest, *tail))
+        else:
+            check(lib.bq4_cache_prefix_attention(self._ref, prefix_pages.data_ptr() or None, width,
+                                                 prefix_length.data_ptr(), ctypes.byref(seqs), longest, *tail))
+        return out

@@ -572,6 +572,99 @@ BQ4_API bq4_status bq4_attention(const uint32_t* q, const uint32_t* k, const uin
                                  int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D, float scale, float* out,
                                  void* workspace, size_t workspace_bytes, bq4_stream_t stream);
 
+/* ---------------------------------------------------------------- key/value cache
+ * A paged cache of the k and v rows that the q/k/v projections leave, for
+ * callers that decode token by token (the few-token linears) or that prompt
+ * many sequences behind one instruction.  The reference keeps no cache; the
+ * formats follow its symmetric quantisation (one scale per block, q * scale).
+ *
+ *   BQ4_CACHE_F16  rows rounded to binary16
+ *   BQ4_CACHE_Q8   8 bits a value, one scale for each row of head_dim values
+ *   BQ4_CACHE_Q4   4 bits a value, one scale for each 32 values of a row
+ * For a block of largest magnitude a: scale = bf16(a / qmax) (f32 quotient,
+ * rounded to nearest even), q = rint(x / scale) clamped to [-qmax, qmax] (f32
+ * quotient), qmax = 127 or 7; scale 0 gives q = 0.  A block with a non-finite
+ * value gets the scale NaN and reads back as NaN.
+ *
+ * `values` and `scales` are device buffers of bq4_cache_sizes bytes on
+ * `device`, 256-byte aligned (scales may be NULL for F16); what they hold is
+ * read through the calls below.  A page holds page_size (a multiple of 16,
+ * at most 65536) consecutive tokens of one sequence for every kv head;
+ * head_dim is a multiple of 8 of at most 128 (rows are stored padded to 64 or
+ * 128 values).
+ */
+typedef enum { BQ4_CACHE_F16 = 0, BQ4_CACHE_Q8 = 1, BQ4_CACHE_Q4 = 2 } bq4_cache_format;
+typedef struct {
+  void* values;
+  void* scales;
+  int64_t pages;
+  int32_t page_size, kv_heads, head_dim;
+  int32_t format; /* bq4_cache_format */
+  int32_t device;
+} bq4_cache;
+/* The sequences of a call, on the device.  Position p of sequence b is row
+ * p % page_size of page page_table[b * table_stride + p / page_size]; lengths[b]
+ * counts the rows that it holds.  A length below 0 counts as 0, one that its
+ * pages (or the call's max_length) cannot hold as what they can, and a page
+ * outside [0, pages) as holding nothing; each of these records
+ * BQ4_EINVAL_ARG, reported by bq4_poll_device_error. */
+typedef struct {
+  const int32_t* page_table;
+  int64_t table_stride, table_width;
+  const int32_t* lengths;
+  int64_t batch;
+} bq4_cache_sequences;
+
+/* Bytes of a cache's two buffers (its pointers and device are not read). */
+BQ4_API bq4_status bq4_cache_sizes(const bq4_cache* cache, size_t* values_bytes, size_t* scales_bytes);
+
+/* Quantises the newest `tokens` rows of every sequence into the cache: row i
+ * of sequence b goes to position lengths[b] - tokens + i (lengths count the
+ * new rows; a position below 0 is skipped, so that short sequences of a padded
+ * batch keep their last rows).  k and v are f32 or f16, element (b, i, h, d) at
+ * b * strides[0] + i * strides[1] + h * strides[2] + d.  Two sequences of a call may
+ * share pages, but not write the same row: which values such a row then holds is
+ * not defined. */
+BQ4_API bq4_status bq4_cache_append(const bq4_cache* cache, const bq4_cache_sequences* seqs, const void* k,
+                                    const int64_t k_strides[3], const void* v, const int64_t v_strides[3],
+                                    bq4_dtype dtype, int64_t tokens, bq4_stream_t stream);
+
+/* Reads rows back: position starts[b] + i (starts NULL: i) of every sequence,
+ * i < count, q * scale rounded once to `dtype`, to element (b, h, i, d) of k_out
+ * and v_out at b * strides[0] + h * strides[1] + i * strides[2] + d.  A position below 0
+ * or not below lengths[b] gives zeros. */
+BQ4_API bq4_status bq4_cache_read(const bq4_cache* cache, const bq4_cache_sequences* seqs, const int32_t* starts,
+                                  int64_t count, void* k_out, void* v_out, const int64_t strides[3],
+                                  bq4_dtype dtype, bq4_stream_t stream);
+
+/* Attention of the newest `tokens` queries of every sequence over its cached
+ * rows: out = softmax(scale q k^T) v in f32 sums, as bq4_attention, with query
+ * head h on kv head h / (q_heads / kv_heads).  causal: query i sees positions
+ * below lengths[b] - tokens + i + 1; else all lengths[b].  A query that sees
+ * nothing gives 0.  q is f16, strided (batch, token, head) like k above; out f16
+ * [batch][tokens][q_heads][head_dim], contiguous.  scale <= 0 means
+ * 1/sqrt(head_dim).  max_length bounds the lengths on the host (the split of
+ * the keys is planned by it; 0 means table_width * page_size). */
+BQ4_API bq4_status bq4_cache_attention_workspace_size(const bq4_cache* cache, int64_t batch, int64_t tokens,
+                                                      int64_t q_heads, int64_t max_length, int64_t max_prefix,
+                                                      size_t* bytes);
+BQ4_API bq4_status bq4_cache_attention(const bq4_cache* cache, const bq4_cache_sequences* seqs, int64_t max_length,
+                                       const void* q, const int64_t q_strides[3], int64_t tokens, int64_t q_heads,
+                                       int32_t causal, float scale, void* out, void* workspace,
+                                       size_t workspace_bytes, bq4_stream_t stream);
+
+/* bq4_cache_attention for a batch whose sequences all begin with the same
+ * rows: every query sees the prefix_length[0] (on the device) rows of the page
+ * list prefix_pages[prefix_width], which are read once for the whole batch, and
+ * then its own sequence (lengths and the causal rule count its own rows only).
+ * Workspace: max_prefix = prefix_width * page_size. */
+BQ4_API bq4_status bq4_cache_prefix_attention(const bq4_cache* cache, const int32_t* prefix_pages,
+                                              int64_t prefix_width, const int32_t* prefix_length,
+                                              const bq4_cache_sequences* seqs, int64_t max_length, const void* q,
+                                              const int64_t q_strides[3], int64_t tokens, int64_t q_heads,
+                                              int32_t causal, float scale, void* out, void* workspace,
+                                              size_t workspace_bytes, bq4_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,507 @@
+"""GPU: the paged key/value cache (KVCache) against plain 64-bit
+implementations of its definitions.
+
+- written rows read back exactly as q * scale rounded once, for every format,
+  head size and source type, strided sources, pages of 16 to 128 rows;
+- attention over the cache and with a shared prefix: formats, head layouts,
+  one to many query tokens, ragged and zero lengths, causal or not, pages that
+  end inside a tile, NaN behind a length;
+- rows that no call names stay as they were; out-of-range pages and lengths
+  are reported; caches past 4 GiB; streams and graphs; the calls in sequence.
+
+Tolerance of an attention output (f16).  The kernels sum f16-rounded
+probabilities (off by at most half a step, 2^-11 of each) in f32 and round the
+result once (2^-11 of it), so with a = sum_j p_j |v_j|
+    |out - exact| <= 2^-11 |exact| + 2^-11 a + a d + 2^-25,
+where d covers the f32 score: an error of e in the exponent moves p by a
+factor 1 + e.  A score is at most SCORE in size (asserted) with sums of |q k|
+at most 8 SCORE, over at most 32 roundings of 2^-24: e <= 2^-16 SCORE for the
+numerator, the same for the sum; plus 2^-14 for the exponential, the online
+rescalings and f32 sums of up to 2^10 steps of 2^-24.
+"""
+import math
+
+import pytest
+import torch
+
+from burn_image_b200 import KVCache, q4
+from burn_image_b200 import f16 as F
+from burn_image_b200.q4 import Bq4Error
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+QMAX = {"q8": 127.0, "q4": 7.0}
+
+
+# --------------------------------------------------------------------- 64-bit definitions
+
+def held(x, fmt):
+    """What the cache stands for, of rows [..., D], in 64 bits."""
+    if fmt == "f16":
+        return x.float().half().double()
+    parts = []
+    for p in x.double().split(x.shape[-1] if fmt == "q8" else 32, -1):
+        top = p.abs().amax(-1, keepdim=True)
+        s = (top / QMAX[fmt]).float().bfloat16().double()
+        q = (p / s).float().double().round().clamp(-QMAX[fmt], QMAX[fmt])
+        w = torch.where(s > 0, q * s, torch.zeros_like(q))
+        parts.append(torch.where(p.isfinite().all(-1, keepdim=True), w, torch.full_like(w, math.nan)))
+    return torch.cat(parts, -1)
+
+
+def attend(q, ks, vs, causal, pk=None, pv=None, scale=None):
+    """q [B,S,Hq,D] (64-bit); ks, vs: per sequence [n,Hkv,D]; pk, pv: prefix rows or None.
+    Returns out and sum p |v| (both [B,S,Hq,D]), and the largest |score|."""
+    B, S, Hq, D = q.shape
+    c = 1 / math.sqrt(D) if scale is None else scale
+    out, mag, top = torch.zeros_like(q), torch.zeros_like(q), 0.0
+    for b in range(B):
+        k, v = ks[b], vs[b]
+        n0 = 0
+        if pk is not None:
+            k, v, n0 = torch.cat([pk, k]), torch.cat([pv, v]), pk.shape[0]
+        n = k.shape[0]
+        if n == 0:
+            continue
+        g = Hq // k.shape[1]
+        k, v = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
+        s = torch.einsum("shd,nhd->hsn", q[b], k) * c
+        top = max(top, s.abs().nan_to_num().max().item())
+        if causal:
+            see = n0 + (n - n0 - S + 1 + torch.arange(S, device=q.device)).clamp(min=0)  # the whole prefix, always
+            s = s.masked_fill(torch.arange(n, device=q.device)[None, None] >= see[None, :, None], -math.inf)
+        p = torch.softmax(s, -1).masked_fill((s == -math.inf).all(-1, keepdim=True), 0.0)
+        out[b] = torch.einsum("hsn,nhd->shd", p, v)
+        mag[b] = torch.einsum("hsn,nhd->shd", p, v.abs())
+    return out, mag, top
+
+
+def check(got, exact, mag, top):
+    q4.poll_device_error()
+    tol = 2.0 ** -11 * exact.abs() + (2.0 ** -11 + 2.0 ** -15 * top + 2.0 ** -14) * mag + 2.0 ** -25
+    err = (got.double() - exact).abs()
+    assert not got.isnan().any()
+    worst = (err / tol).max().item() if err.numel() else 0.0
+    assert worst <= 1.0, f"{worst} times the tolerance (max error {err.max().item()})"
+
+
+class Book:
+    """A cache whose pages are handed out in no order, beside the rows that went in."""
+
+    def __init__(self, fmt, lengths, Hkv, D, page, prefix=0, seed=0, spare=3, poison=False):
+        g = torch.Generator().manual_seed(seed + 77)
+        self.g = torch.Generator(device=DEV).manual_seed(seed)
+        B = len(lengths)
+        W = max(1, -(-max(lengths + [1]) // page))
+        PW = -(-prefix // page)
+        pages = B * W + PW + spare
+        order = torch.randperm(pages, generator=g).int().to(DEV)
+        self.table, self.ptable = order[:B * W].reshape(B, W), order[B * W:B * W + PW]
+        self.lengths = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+        self.plen = torch.tensor([prefix], dtype=torch.int32, device=DEV)
+        self.cache = KVCache(pages, page, Hkv, D, fmt, DEV)
+        if poison:  # NaN in every place that a length leaves out
+            self.cache.values.view(torch.uint8).fill_(0xFF)
+            self.cache.scales.fill_(0xFF)
+        self.k, self.v = [], []
+        for b, n in enumerate(lengths):
+            k, v = self.rows(n, Hkv, D), self.rows(n, Hkv, D)
+            if n:
+                self.cache.append(k[None], v[None], self.table[b:b + 1], self.lengths[b:b + 1])
+            self.k.append(held(k, fmt)), self.v.append(held(v, fmt))
+        self.pk = self.pv = None
+        if prefix:
+            k, v = self.rows(prefix, Hkv, D), self.rows(prefix, Hkv, D)
+            self.cache.append(k[None], v[None], self.ptable[None], self.plen)
+            self.pk, self.pv = held(k, fmt), held(v, fmt)
+
+    def rows(self, n, H, D):
+        off = torch.randn((1, H, D), generator=self.g, device=DEV) * 0.5
+        return (torch.randn((n, H, D), generator=self.g, device=DEV) + off).half()
+
+    def query(self, S, Hq):
+        return torch.randn((len(self.k), S, Hq, self.cache.head_dim), generator=self.g, device=DEV).half()
+
+
+# --------------------------------------------------------------------- write and read
+
+@pytest.mark.parametrize("fmt", ["f16", "q8", "q4"])
+@pytest.mark.parametrize("D", [128, 120, 72, 64, 8])
+@pytest.mark.parametrize("src", [torch.float32, torch.float16])
+def test_write_and_read_back(fmt, D, src):
+    B, S, H, page = 3, 19, 3, 16
+    g = torch.Generator(device=DEV).manual_seed(D)
+    lengths = torch.tensor([40, 19, 7], dtype=torch.int32, device=DEV)  # the third: 12 rows fall below 0
+    table = torch.randperm(12, generator=torch.Generator().manual_seed(1)).int().to(DEV)[:9].reshape(3, 3)
+    c = KVCache(12, page, H, D, fmt, DEV)
+    size = torch.rand((B, S, H, 1), generator=g, device=DEV) * 3
+    k = (torch.randn((B, S, H, D), generator=g, device=DEV) * size).to(src)
+    v = torch.randn((B, S, H, D), generator=g, device=DEV).to(src)
+    k[0, 3] = 0.0  # an all-zero row
+    k[1, 2, 1, :8] *= 1e-4 if src == torch.float16 else 1e-30
+    c.append(k, v, table, lengths)
+    for dtype in (torch.float32, torch.float16):
+        got = c.read(table, lengths, S + 5, starts=lengths - S, dtype=dtype)
+        for x, y in zip((k, v), got):
+            want = torch.zeros((B, H, S + 5, D), dtype=torch.float64, device=DEV)
+            want[:, :, :S] = held(x, fmt).transpose(1, 2)
+            want[2, :, :12] = 0.0  # positions below 0
+            assert torch.equal(y, want.float().to(dtype))
+    q4.poll_device_error()
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8", "q4"])
+def test_extreme_values(fmt):
+    c = KVCache(2, 16, 1, 64, fmt, DEV)
+    x = torch.zeros((1, 8, 1, 64), device=DEV)
+    x[0, 0] = 1e-42            # under the smallest scale
+    x[0, 1] = 3e38             # near the largest float32
+    x[0, 2, 0, 5] = math.inf
+    x[0, 3, 0, 40] = math.nan
+    x[0, 4] = torch.linspace(-6e4, 6e4, 64, device=DEV)
+    x[0, 5] = torch.linspace(-1.0, 1.0, 64, device=DEV) * 2.0 ** -120
+    x[0, 6, 0, 0] = -7.0       # whole numbers are exact
+    x[0, 7, 0, 33] = -math.inf
+    table = torch.tensor([[1]], dtype=torch.int32, device=DEV)
+    n = torch.tensor([8], dtype=torch.int32, device=DEV)
+    c.append(x, -x, table, n)
+    k, v = c.read(table, n, 8, dtype=torch.float32)
+    q4.poll_device_error()
+    for y, z in ((k, x), (v, -x)):
+        want = held(z[0], fmt).float()[:, 0]
+        assert torch.equal(y[0, 0].nan_to_num(123.0), want.nan_to_num(123.0))
+        assert torch.equal(y[0, 0].isnan(), want.isnan())
+
+
+@pytest.mark.parametrize("fmt", ["q8", "q4", "f16"])
+def test_strided_sources_and_untouched_rows(fmt):
+    # k and v as sections of one projection output, head-major views, an odd offset (scalar loads)
+    B, S, H, D = 2, 5, 2, 128
+    g = torch.Generator(device=DEV).manual_seed(4)
+    proj = torch.randn((B, S, 4 * H * D), generator=g, device=DEV).half()
+    k = proj[:, :, 2 * H * D:3 * H * D].unflatten(-1, (H, D))
+    v = proj[:, :, 3 * H * D:].unflatten(-1, (H, D))
+    table = torch.tensor([[5, 0], [3, 1]], dtype=torch.int32, device=DEV)
+    n = torch.tensor([18, 5], dtype=torch.int32, device=DEV)
+    plain = KVCache(6, 16, H, D, fmt, DEV)
+    plain.values.fill_(0x5A), plain.scales.fill_(0x3C)
+    before = plain.read(torch.arange(6, dtype=torch.int32, device=DEV)[:, None], torch.full((6,), 16, dtype=torch.int32,
+                                                                                           device=DEV), 16)
+    plain.append(k.contiguous(), v.contiguous(), table, n)
+    odd = torch.empty(B * S * H * D + 1, dtype=torch.float16, device=DEV)[1:].view(B, S, H, D).copy_(k)
+    turned = v.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+    for kk, vv in ((k, v), (odd, turned), (k.transpose(-1, -2).contiguous().transpose(-1, -2), v)):
+        c = KVCache(6, 16, H, D, fmt, DEV)
+        c.values.fill_(0x5A), c.scales.fill_(0x3C)
+        c.append(kk, vv, table, n)
+        assert torch.equal(c.values, plain.values) and torch.equal(c.scales, plain.scales)
+    after = plain.read(torch.arange(6, dtype=torch.int32, device=DEV)[:, None], torch.full((6,), 16, dtype=torch.int32,
+                                                                                          device=DEV), 16)
+    touched = torch.zeros((6, 16), dtype=torch.bool, device=DEV)
+    for b, length in ((0, 18), (1, 5)):
+        for p in range(length - S, length):
+            touched[table[b, p // 16].long(), p % 16] = True
+    for x, y in zip(before, after):
+        keep = ~touched[:, None, :, None].expand_as(x)
+        assert torch.equal(x[keep].nan_to_num(9.0), y[keep].nan_to_num(9.0))
+    # an output dtype and starts past the length read zeros
+    k0, v0 = plain.read(table, n, 4, starts=torch.tensor([17, -2], dtype=torch.int32, device=DEV))
+    assert k0[0, :, 1:].abs().sum() == 0 and k0[1, :, :2].abs().sum() == 0 and v0[1, :, 2:].abs().sum() > 0
+    q4.poll_device_error()
+
+
+# --------------------------------------------------------------------- attention
+
+def run_attention(book, S, Hq, causal=True, scale=None, **kw):
+    q = book.query(S, Hq)
+    got = book.cache.attention(q, book.table, book.lengths, causal=causal, scale=scale, **kw)
+    check(got, *attend(q.double(), book.k, book.v, causal, scale=scale))
+    return q, got
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8", "q4"])
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (28, 7, 120), (3, 3, 64), (6, 1, 72), (16, 1, 128), (40, 2, 96),
+                                      (2, 1, 8)])
+def test_decode(fmt, Hq, Hkv, D):
+    book = Book(fmt, [0, 1, 15, 16, 17, 63, 64, 129, 500], Hkv, D, 16, seed=Hq + D, poison=True)
+    run_attention(book, 1, Hq)
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8", "q4"])
+@pytest.mark.parametrize("S,causal", [(2, True), (3, False), (5, True), (8, True), (17, True), (33, False), (70, True)])
+def test_several_query_tokens(fmt, S, causal):
+    # lengths below S leave the first rows without a key
+    book = Book(fmt, [S + 200, S, max(0, S - 2), 1, S + 31], 2, 128, 48, seed=S, poison=True)
+    run_attention(book, S, 8, causal)
+
+
+@pytest.mark.parametrize("fmt", ["q8", "q4", "f16"])
+def test_one_long_context(fmt):
+    book = Book(fmt, [9001], 2, 128, 64, seed=3)
+    run_attention(book, 1, 8)
+    run_attention(book, 4, 16)
+
+
+def test_many_query_tokens():
+    for fmt, S, n, D, causal in (("q8", 300, 1111, 128, True), ("q4", 129, 129, 64, True),
+                                 ("f16", 256, 700, 120, False), ("q8", 513, 2000, 120, True)):
+        run_attention(Book(fmt, [n, max(0, n - 130), 40], 2, D, 32, seed=S, poison=True), S, 8, causal)
+
+
+def test_scale_and_running_maximum():
+    # scores that grow along the keys: the running maximum moves all the way
+    for fmt in ("f16", "q8", "q4"):
+        book = Book(fmt, [700], 1, 128, 16, seed=8)
+        ramp = torch.linspace(0.05, 4.0, 700, device=DEV)[:, None, None]
+        k = (book.rows(700, 1, 128).abs() * ramp).half()
+        book.cache.append(k[None], k[None].flip(1), book.table, book.lengths)
+        book.k, book.v = [held(k, fmt)], [held(k.flip(0), fmt)]
+        q = book.query(2, 4).abs()
+        for scale in (0.02, 0.2):
+            got = book.cache.attention(q, book.table, book.lengths, scale=scale)
+            check(got, *attend(q.double(), book.k, book.v, True, scale=scale))
+
+
+@pytest.mark.parametrize("fmt", ["q8", "q4"])
+def test_values_of_very_different_size(fmt):
+    # v rows from 2^-12 to 2^12: their scales must not leave a probability's range.  Small rows
+    # beside large ones: the tolerance's a is the large ones' share.
+    book = Book(fmt, [300, 77], 2, 128, 16, seed=5)
+    for b, n in enumerate((300, 77)):
+        size = 2.0 ** torch.randint(-12, 13, (n, 1, 1), generator=book.g, device=DEV).float()
+        v = (book.rows(n, 2, 128).float() * size)
+        k = book.rows(n, 2, 128).float()
+        book.cache.append(k[None], v[None], book.table[b:b + 1], book.lengths[b:b + 1])
+        book.k[b], book.v[b] = held(k, fmt), held(v, fmt)
+    run_attention(book, 3, 8)
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8", "q4"])
+@pytest.mark.parametrize("S,Hq,Hkv,D,prefix", [(1, 8, 2, 128, 700), (1, 28, 7, 120, 17), (4, 8, 8, 64, 333),
+                                               (3, 8, 1, 128, 1), (40, 8, 2, 128, 260)])
+def test_shared_prefix(fmt, S, Hq, Hkv, D, prefix):
+    book = Book(fmt, [0, 1, 100, 37, 64, S], Hkv, D, 16, prefix=prefix, seed=S + D, poison=True)
+    q = book.query(S, Hq)
+    for causal in (True, False):
+        got = book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths, causal=causal)
+        exact = attend(q.double(), book.k, book.v, causal, book.pk, book.pv)
+        check(got, *exact)
+    # an empty prefix is plain attention; an empty table is the prefix alone
+    none = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = book.cache.prefix_attention(q, book.ptable, none, book.table, book.lengths)
+    check(got, *attend(q.double(), book.k, book.v, True))
+    got = book.cache.prefix_attention(q, book.ptable, book.plen, book.table[:, :0], torch.zeros_like(book.lengths))
+    empty = [x[:0] for x in book.k]
+    check(got, *attend(q.double(), empty, empty, False, book.pk, book.pv))
+
+
+def test_shared_prefix_of_a_large_batch():
+    B, prefix = 70, 1500
+    book = Book("q8", [i % 90 for i in range(B)], 2, 128, 64, prefix=prefix, seed=2)
+    q = book.query(2, 16)
+    got = book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths, max_length=100)
+    check(got, *attend(q.double(), book.k, book.v, True, book.pk, book.pv))
+
+
+def test_strided_queries_and_out():
+    book = Book("q8", [100, 33], 2, 128, 16, seed=6)
+    q = book.query(3, 8)
+    want = book.cache.attention(q, book.table, book.lengths)
+    turned = q.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+    wide = torch.zeros((2, 3, 9, 130), dtype=torch.float16, device=DEV)
+    wide[:, :, 1:, 1:129] = q
+    out = torch.empty_like(q)
+    for x in (turned, wide[:, :, 1:, 1:129]):
+        assert torch.equal(book.cache.attention(x, book.table, book.lengths, out=out), want)
+        assert torch.equal(out, want)
+    # the bound of the lengths changes the split, not the result's meaning
+    check(book.cache.attention(q, book.table, book.lengths, max_length=100),
+          *attend(q.double(), book.k, book.v, True))
+    q4.poll_device_error()
+
+
+def test_masked_nan_and_held_nan():
+    book = Book("f16", [20, 20], 1, 64, 16, seed=9, poison=True)
+    k = torch.ones((1, 1, 1, 64), device=DEV).half()
+    v = torch.full((1, 1, 1, 64), math.nan, device=DEV).half()
+    book.cache.append(k, v, book.table[:1], book.lengths[:1])  # the last row of sequence 0
+    q = book.query(2, 2)
+    out = book.cache.attention(q, book.table, book.lengths)
+    q4.poll_device_error()
+    assert out[0, 1].isnan().all()      # sees it
+    assert not out[1].isnan().any()
+    exact = attend(q.double()[:, :1], [x[:19] for x in book.k], [x[:19] for x in book.v], True)
+    check(out[:, :1], *exact)           # query 0 sees 19 rows
+
+
+# --------------------------------------------------------------------- bad pages, long caches
+
+def reported():
+    with pytest.raises(Bq4Error, match="EINVAL_ARG|device error"):
+        q4.poll_device_error()
+
+
+def test_bad_pages_and_lengths_are_reported():
+    c = KVCache(4, 16, 2, 128, "q8", DEV)
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device=DEV)  # noqa: E731
+    x = torch.ones((2, 2, 2, 128), device=DEV).half()
+    q = torch.ones((2, 1, 4, 128), device=DEV).half()
+    good = i32([0, 1], [2, 3])
+    ones = torch.ones((2, 32, 2, 128), device=DEV).half()
+    c.append(ones, ones, good, i32(32, 32))
+    q4.poll_device_error()
+    before = c.values.clone()
+    for bad in (i32([4, 4], [-1, -1]), i32([2 ** 31 - 1, -2 ** 31], [4, 5])):
+        c.append(x, x, bad, i32(20, 20))
+        reported()
+        k, v = c.read(bad, i32(32, 32), 32)
+        reported()
+        assert k.abs().sum() == 0 and v.abs().sum() == 0
+        out = c.attention(q, bad, i32(32, 32))
+        reported()
+        assert out.abs().sum() == 0
+        out = c.prefix_attention(q, bad[0], i32(32), good, i32(0, 32))
+        reported()
+        assert out[0].abs().sum() == 0 and torch.equal(out[1], torch.ones_like(out[1]))
+    assert torch.equal(c.values, before)
+    for n in (i32(33, 2), i32(-1, 2), i32(2 ** 31 - 1, 2)):
+        c.read(good, n, 8)
+        reported()
+        c.attention(q, good, n)
+        reported()
+        c.prefix_attention(q, good[0], n[:1], good, i32(1, 1))
+        reported()
+    c.attention(q, good, i32(20, 32), max_length=16)  # above the caller's own bound
+    reported()
+    q4.poll_device_error()
+
+
+def test_cache_past_four_gib():
+    # 5 GiB of pages: offsets of the last ones pass 32 bits
+    pages, page, H, D = 20480, 64, 16, 128
+    c = KVCache(pages, page, H, D, "q8", DEV)
+    assert c.values.numel() >= 2 ** 32 + 2 ** 30
+    table = torch.tensor([[pages - 1, 3, pages - 2]], dtype=torch.int32, device=DEV)
+    n = torch.tensor([150], dtype=torch.int32, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    k = torch.randn((1, 150, H, D), generator=g, device=DEV).half()
+    v = torch.randn((1, 150, H, D), generator=g, device=DEV).half()
+    c.append(k, v, table, n)
+    got = c.read(table, n, 150, dtype=torch.float32)
+    assert torch.equal(got[0][0], held(k[0], "q8").float().transpose(0, 1))
+    q = torch.randn((1, 2, H, D), generator=g, device=DEV).half()
+    out = c.attention(q, table, n)
+    check(out, *attend(q.double(), [held(k[0], "q8")], [held(v[0], "q8")], True))
+    out = c.prefix_attention(q, table[0], n, table[:, :0], n * 0)
+    check(out, *attend(q.double(), [held(k[0], "q8")[:0]], [held(v[0], "q8")[:0]], False, held(k[0], "q8"),
+                       held(v[0], "q8")))
+    assert int(c.values.view(pages, -1).any(1).sum()) == 3  # nothing went to another page
+
+
+# --------------------------------------------------------------------- in use
+
+def test_refusals():
+    c = KVCache(4, 16, 2, 128, "q8", DEV)
+    t = torch.zeros((1, 2), dtype=torch.int32, device=DEV)
+    n = torch.ones(1, dtype=torch.int32, device=DEV)
+    x = torch.zeros((1, 1, 2, 128), device=DEV).half()
+    q = torch.zeros((1, 1, 4, 128), device=DEV).half()
+    for bad in (lambda: c.append(x.cpu(), x, t, n), lambda: c.append(x.double(), x.double(), t, n),
+                lambda: c.append(x[..., :64], x[..., :64], t, n), lambda: c.append(x, x.float(), t, n),
+                lambda: c.append(x, x, t.long(), n), lambda: c.append(x, x, t, n.cpu()),
+                lambda: c.append(x, x, t[0], n),
+                lambda: c.append(x, x, t, torch.cat([n, n])), lambda: c.append(x[:, :, :1], x[:, :, :1], t, n),
+                lambda: c.read(t, n, -1), lambda: c.read(t, n, 1, dtype=torch.bfloat16),
+                lambda: c.read(t, n, 1, starts=t[0]), lambda: c.attention(q.float(), t, n),
+                lambda: c.attention(q[:, :, :3], t, n), lambda: c.attention(q, t, n, max_length=-1),
+                lambda: c.attention(q, t, n, scale=math.nan), lambda: c.attention(q, t, n, out=q.float()),
+                lambda: c.prefix_attention(q, t, n, t, n), lambda: c.prefix_attention(q, t[0], t[0], t, n)):
+        with pytest.raises(Bq4Error):
+            bad()
+    e = torch.zeros((0, 2), dtype=torch.int32, device=DEV)  # empty batches and no tokens do nothing
+    c.append(x[:0], x[:0], e, n[:0])
+    assert c.read(e, n[:0], 3)[0].shape == (0, 2, 3, 128)
+    assert c.read(t, n, 0)[0].numel() == 0
+    assert c.attention(q[:0], e, n[:0]).shape == (0, 1, 4, 128)
+    assert c.attention(q[:, :0], t, n).shape == (1, 0, 4, 128)
+    q4.poll_device_error()
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8", "q4"])
+def test_prompt_then_decode_matches_contiguous_attention(fmt):
+    # a prompt enters in two chunks, tokens follow one by one: each step's output is that of
+    # f16.attention on rows read back (f32 output, so f16's half step and both kernels' errors)
+    B, Hq, Hkv, D, page = 2, 8, 2, 128, 16
+    g = torch.Generator(device=DEV).manual_seed(1)
+    c = KVCache(2 * 6, page, Hkv, D, fmt, DEV)
+    table = torch.randperm(12, generator=torch.Generator().manual_seed(2)).int().to(DEV).reshape(2, 6)
+    lengths = torch.zeros(B, dtype=torch.int32, device=DEV)
+    for S in (30, 21, 1, 1, 1, 3):
+        lengths = lengths + S
+        new = torch.randn((B, S, Hq + 2 * Hkv, D), generator=g, device=DEV).half()
+        q, k, v = new.split([Hq, Hkv, Hkv], 2)
+        c.append(k, v, table, lengths)
+        out = c.attention(q, table, lengths)
+        total = int(lengths[0])
+        kk, vv = c.read(table, lengths, total, dtype=torch.float16)
+        want = F.attention(q[:, -1:].transpose(1, 2), kk, vv).transpose(1, 2)
+        # both round probabilities to f16 (2^-11 of a <= max |v|), K and V to f16 once more when
+        # read (2^-11 of a score of at most 8, 2^-11 of v), the result here to f16
+        bound = (2 ** -11 * (3 + 2 * 8) + 2 ** -9) * vv.abs().max().item()
+        assert (out[:, -1:].float() - want).abs().max().item() <= bound
+    q4.poll_device_error()
+
+
+def test_streams_and_graphs():
+    book = Book("q8", [300, 150, 40, 9], 2, 128, 16, prefix=200, seed=11)
+    c = book.cache
+    q = book.query(1, 8)
+    new_k, new_v = book.rows(4, 2, 128)[:, None], book.rows(4, 2, 128)[:, None]
+    lengths = book.lengths.clone()
+    want0 = c.attention(q, book.table, lengths)
+    # another stream than the current one's tensors, and two calls in flight on two streams
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s1):
+        a = c.attention(q, book.table, lengths)
+    with torch.cuda.stream(s2):
+        b = c.prefix_attention(q, book.ptable, book.plen, book.table, lengths)
+    torch.cuda.synchronize()
+    assert torch.equal(a, want0)
+    assert torch.equal(b, c.prefix_attention(q, book.ptable, book.plen, book.table, lengths))
+    # captured: write the new row, then attend; replayed with lengths changed in place
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.append(new_k, new_v, book.table, lengths)
+        out = c.attention(q, book.table, lengths, max_length=19 * 16)
+    with torch.cuda.graph(other):
+        out2 = c.prefix_attention(q, book.ptable, book.plen, book.table, lengths, max_length=19 * 16)
+    for step in (1, 2):
+        lengths.copy_(book.lengths + step)
+        graph.replay()
+        torch.cuda.synchronize()
+        ks = [torch.cat([x] + [held(new_k[i], "q8")] * step) for i, x in enumerate(book.k)]
+        vs = [torch.cat([x] + [held(new_v[i], "q8")] * step) for i, x in enumerate(book.v)]
+        check(out, *attend(q.double(), ks, vs, True))
+        want = out.clone()
+        # both graphs in flight at once: neither uses the other's workspace
+        out.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s1):
+            graph.replay()
+        with torch.cuda.stream(s2):
+            other.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        check(out2, *attend(q.double(), ks, vs, True, book.pk, book.pv))
+    q4.poll_device_error()
+
+
+def test_same_bits_every_time():
+    book = Book("q4", [1000, 5000, 20], 4, 128, 64, prefix=900, seed=12)
+    q = book.query(1, 16)
+    one = book.cache.attention(q, book.table, book.lengths)
+    two = book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths)
+    for _ in range(5):
+        assert torch.equal(one, book.cache.attention(q, book.table, book.lengths))
+        assert torch.equal(two, book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths))
