@@ -421,7 +421,9 @@ bq4_status attention(const bq4_cache* cache, const int32_t* prefix_pages, int64_
   if (st) return st;
   Guard guard(cache->device);
   const int sms = device_sm_count(cache->device);
-  const size_t need = cache_attn_workspace(call, sms);
+  size_t need = 0;
+  st = cache_attn_workspace(call, sms, &need);
+  if (st) return st;
   if (need > workspace_bytes || (need && !workspace))
     return set_error(BQ4_EWORKSPACE, "workspace of %zu bytes; cache attention needs %zu", workspace_bytes, need);
   if (need && !al(workspace, 256)) return set_error(BQ4_EALIGN, "workspace not 256-byte aligned");
@@ -559,8 +561,7 @@ bq4_status bq4_cache_attention_workspace_size(const bq4_cache* cache, int64_t ba
   if (batch == 0 || tokens == 0) return BQ4_OK;
   st = device_ready(cache->device);
   if (st) return st;
-  *bytes = cache_attn_workspace(call, device_sm_count(cache->device));
-  return BQ4_OK;
+  return cache_attn_workspace(call, device_sm_count(cache->device), bytes);
 }
 
 bq4_status bq4_cache_attention(const bq4_cache* cache, const bq4_cache_sequences* seqs, int64_t max_length,

@@ -63,7 +63,7 @@ struct CacheAttnCall {
   int* err;
 };
 
-size_t cache_attn_workspace(const CacheAttnCall& c, int sms);
+bq4_status cache_attn_workspace(const CacheAttnCall& c, int sms, size_t* bytes);
 bq4_status run_cache_attn(const CacheAttnCall& c, int sms, void* workspace, cudaStream_t s);
 
 }  // namespace bq4
