@@ -22,16 +22,16 @@ namespace {
 constexpr int kCThreads = 256;
 
 struct CacheRow {
-  int64_t k;      // byte offset of the k row in values
-  int64_t scale;  // index of the k scales
+  uint8_t* rows;   // k or v rows of the page and head
+  uint16_t* scales;
 };
 
-// Row of (page, head, place); v rows lie kv_bytes (values) and nb (scales) behind.
-__device__ __forceinline__ CacheRow cache_row(const CacheView& c, int page, int head, int place) {
+// Rows of (page, head) and the scales of the row at `place`; kv: 0 k, 1 v.
+__device__ __forceinline__ CacheRow cache_row(const CacheView& c, int page, int head, int place, int kv) {
   const int64_t ph = (int64_t)page * c.kv_heads + head;
   CacheRow r;
-  r.k = ph * 2 * c.kv_bytes + (int64_t)place * c.row_bytes;
-  r.scale = (ph * c.page_size + place) * 2 * c.nb;
+  r.rows = c.values + (ph * 2 + kv) * c.kv_bytes;
+  r.scales = c.scales + ((ph * c.page_size + place) * 2 + kv) * c.nb;
   return r;
 }
 
@@ -108,14 +108,14 @@ __global__ void __launch_bounds__(kCThreads) cache_append_kernel(const AppendArg
     if (page >= 0 && d0 < a.c.head_dim)
       load4<kF16>(a.x[kv], b * a.stride[kv][0] + i * a.stride[kv][1] + h * a.stride[kv][2] + d0, a.vec, x);
   }
-  const CacheRow r = cache_row(a.c, page < 0 ? 0 : page, h, place);
-  uint8_t* dst = a.c.values + r.k + kv * a.c.kv_bytes;
+  const CacheRow r = cache_row(a.c, page < 0 ? 0 : page, h, place, kv);
+  auto dst = [&](int at) { return r.rows + cache_swizzle(kv, a.c.row_bytes, place, at); };
   if constexpr (kFmt == BQ4_CACHE_F16) {
     const __half2 lo = __floats2half2_rn(x[0], x[1]), hi = __floats2half2_rn(x[2], x[3]);
     uint2 u;
     u.x = *reinterpret_cast<const uint32_t*>(&lo);
     u.y = *reinterpret_cast<const uint32_t*>(&hi);
-    if (page >= 0) reinterpret_cast<uint2*>(dst)[L] = u;
+    if (page >= 0) *reinterpret_cast<uint2*>(dst(8 * L)) = u;
     return;
   }
   constexpr float kTop = kFmt == BQ4_CACHE_Q8 ? 127.0f : 7.0f;
@@ -137,13 +137,12 @@ __global__ void __launch_bounds__(kCThreads) cache_append_kernel(const AppendArg
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     q[j] = s > 0.0f ? (int)fminf(fmaxf(rintf(__fdiv_rn(x[j], s)), -kTop), kTop) : 0;
-  uint16_t* sc = a.c.scales + r.scale + kv * a.c.nb;
   if constexpr (kFmt == BQ4_CACHE_Q8) {
     const uint32_t w = (uint32_t)(q[0] + 128) | (uint32_t)(q[1] + 128) << 8 | (uint32_t)(q[2] + 128) << 16 |
                        (uint32_t)(q[3] + 128) << 24;
     if (page >= 0) {
-      reinterpret_cast<uint32_t*>(dst)[L] = w;
-      if (L == 0) *sc = __bfloat16_as_ushort(sb);
+      *reinterpret_cast<uint32_t*>(dst(4 * L)) = w;
+      if (L == 0) r.scales[0] = __bfloat16_as_ushort(sb);
     }
   } else {
     const int blk = L >> 3, g = L & 7;
@@ -153,12 +152,12 @@ __global__ void __launch_bounds__(kCThreads) cache_append_kernel(const AppendArg
                    (uint32_t)(q[3] + 8) << 20;
       w <<= 8 * (L & 1);
       w |= __shfl_xor_sync(0xffffffffu, w, 1);
-      if (page >= 0 && !(L & 1)) reinterpret_cast<uint32_t*>(dst)[(g >> 1) * a.c.nb + blk] = w;
+      if (page >= 0 && !(L & 1)) *reinterpret_cast<uint32_t*>(dst(4 * ((g >> 1) * a.c.nb + blk))) = w;
     } else {
       const uint16_t w = (uint16_t)((q[0] + 8) | (q[1] + 8) << 4 | (q[2] + 8) << 8 | (q[3] + 8) << 12);
-      if (page >= 0) reinterpret_cast<uint16_t*>(dst)[g * a.c.nb + blk] = w;
+      if (page >= 0) *reinterpret_cast<uint16_t*>(dst(2 * (g * a.c.nb + blk))) = w;
     }
-    if (page >= 0 && g == 0) sc[blk] = __bfloat16_as_ushort(sb);
+    if (page >= 0 && g == 0) r.scales[blk] = __bfloat16_as_ushort(sb);
   }
 }
 
@@ -193,27 +192,27 @@ __global__ void __launch_bounds__(kCThreads) cache_read_kernel(const ReadArgs a)
     if (page < 0 || page >= a.c.pages) {
       atomicCAS(a.err, 0, (int)BQ4_EINVAL_ARG);
     } else {
-      const CacheRow r = cache_row(a.c, page, h, (int)pos - pi * a.c.page_size);
-      const uint8_t* src = a.c.values + r.k + kv * a.c.kv_bytes;
-      const uint16_t* sc = a.c.scales + r.scale + kv * a.c.nb;
+      const int place = (int)pos - pi * a.c.page_size;
+      const CacheRow r = cache_row(a.c, page, h, place, kv);
+      auto src = [&](int at) { return r.rows + cache_swizzle(kv, a.c.row_bytes, place, at); };
       if constexpr (kFmt == BQ4_CACHE_F16) {
-        load4<true>(src, d0, true, x);
+        load4<true>(src(2 * d0), 0, true, x);
       } else if constexpr (kFmt == BQ4_CACHE_Q8) {
-        const uint32_t w = reinterpret_cast<const uint32_t*>(src)[L];
-        const float s = __uint_as_float((uint32_t)sc[0] << 16);
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(src(4 * L));
+        const float s = __uint_as_float((uint32_t)r.scales[0] << 16);
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = (float)((int)(w >> 8 * j & 255) - 128) * s;
       } else {
         const int blk = L >> 3, g = L & 7;
-        const float s = __uint_as_float((uint32_t)sc[blk] << 16);
+        const float s = __uint_as_float((uint32_t)r.scales[blk] << 16);
         if (kv == 0) {
-          const uint32_t w = reinterpret_cast<const uint32_t*>(src)[(g >> 1) * a.c.nb + blk] >> 8 * (L & 1);
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(src(4 * ((g >> 1) * a.c.nb + blk))) >> 8 * (L & 1);
           x[0] = (float)((int)(w & 15) - 8) * s;
           x[1] = (float)((int)(w >> 16 & 15) - 8) * s;
           x[2] = (float)((int)(w >> 4 & 15) - 8) * s;
           x[3] = (float)((int)(w >> 20 & 15) - 8) * s;
         } else {
-          const uint32_t w = reinterpret_cast<const uint16_t*>(src)[g * a.c.nb + blk];
+          const uint32_t w = *reinterpret_cast<const uint16_t*>(src(2 * (g * a.c.nb + blk)));
 #pragma unroll
           for (int j = 0; j < 4; ++j) x[j] = (float)((int)(w >> 4 * j & 15) - 8) * s;
         }

@@ -14,6 +14,11 @@
 //           (w >> 4 p) & 0x000F000F is the pair (2 p, 2 p + 1).
 //        v: the 4 values 32 b + 4 g .. + 3 form u16 g nb + b, in order.
 // Padding values are q = 0 with scale 0 (f16: 0).
+//
+// The 16-byte pieces of a 128-byte line are permuted by the row (cache_swizzle),
+// so that 16 rows copied to shared memory as they lie are read by fragments
+// without bank conflicts: 8 lanes take a 16-byte piece each of either two
+// adjacent k rows (4 pieces of each) or four even v rows (2 of each).
 #pragma once
 #include "bq4_internal.h"
 
@@ -45,6 +50,13 @@ inline int cache_nb(int format, int hp) {
 }
 inline int cache_row_bytes(int format, int hp) {
   return format == BQ4_CACHE_F16 ? 2 * hp : format == BQ4_CACHE_Q8 ? hp : hp / 2;
+}
+
+// Byte of the k (v) rows of a page and head where byte `at` of row r lies.
+__host__ __device__ __forceinline__ constexpr int cache_swizzle(int kv, int row_bytes, int r, int at) {
+  const int f = kv == 0 ? (row_bytes >= 128 ? 4 * (r & 1) : 0)
+                        : row_bytes >= 64 ? 2 * (r >> 1 & 3) : 2 * (r >> 2 & 1);
+  return (r * row_bytes + at) ^ f << 4;
 }
 
 // Arguments of one attention call (bq4_cache_attn.cu).

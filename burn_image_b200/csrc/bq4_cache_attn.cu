@@ -3,31 +3,38 @@
 // keys being a prefix that the whole batch shares (if any) and the
 // sequence's own rows.
 //
-// The keys of a sequence (or of the prefix) are cut into chunks; one CTA takes
-// one chunk, one kv head and a tile of 8 kNT query rows (the tokens and
-// grouped heads that read this kv head; for the prefix those of the whole
-// batch, so that it is read once).  It keeps a running maximum m, sum l and
-// product O in f32 (O = sum_j 2^(x_j - m) v_j, x in log2 units), and a second
-// kernel joins the chunks: O = sum_c 2^(m_c - M) O_c, l likewise.
+// The work is a line of units of 64 keys: for every kv head and tile of 8 kNT
+// query rows (the tokens and grouped heads that read this kv head; for the
+// prefix those of the whole batch, so that it is read once) the units of the
+// prefix, then those of each sequence.  The lengths are on the device, so
+// every CTA adds them up itself and takes one share of the line, as many
+// units as every other: one wave, whatever the lengths.  A share is cut where
+// one (head, tile)'s keys end; each such piece keeps a running maximum m, sum l
+// and product O in f32 (O = sum_j 2^(x_j - m) v_j, x in log2 units).  Rows that
+// one piece covers are finished at once; a second kernel joins the others:
+// O = sum_c 2^(m_c - M) O_c, l likewise, pieces in their order.
 //
 // cache_split_kernel: four warps, each its own 16-key steps.
 //   * Keys are the M side of the tensor core's m16n8k16 (f16 in, f32 out) and
 //     the query rows its N side: S^T = K Q^T, then O^T = V^T P^T.  A group of 4
 //     query heads fills half of N = 8, not a quarter of M = 16, and the widened
 //     cache values (A) are made once for all rows.
-//   * A lane (g = lane / 4, t = lane % 4) copies exactly the bytes that its
-//     fragments need, 16 at a time (cp.async), into its own slots of a ring in
-//     shared memory: k rows g and g + 8 at quarter t, v rows 2t, 2t + 1,
-//     2t + 8, 2t + 9 at eighth g.  No lane reads what another copied, so the
-//     loop has no barrier, and any order of the head's values inside a
-//     fragment is as good as another as long as q follows it.
+//   * The 16 rows of a step lie together in their page (k, v and scales): one
+//     lane brings them to a ring of the warp's own with three bulk copies,
+//     some steps ahead; an mbarrier says when they are there.  No warp waits
+//     for another in the loop.
+//   * Lane (g = lane / 4, t = lane % 4) reads quarter t of k rows g and g + 8
+//     and eighth g of v rows 2t, 2t + 1, 2t + 8, 2t + 9, 16 bytes at a time.  Any
+//     order of the head's values inside a fragment is as good as another as
+//     long as q follows it.
 //   * Stored values are whole numbers u = q + 128 (q + 8).  Zero-extended to
 //     16 bits they are the subnormal halves u 2^-24, exact in the tensor core:
 //     widening a pair of k values is one byte permute (q8) or mask (q4).  The
 //     offset leaves the scores through the accumulator's start value -128
-//     2^-24 sum(q) (f32; q4: for each scale's 32 values); v, whose products
-//     are summed over many keys, is made signed (one add a pair), since there
-//     an offset would cost the sum its low bits.
+//     2^-24 sum(q) (f32; q4: for each scale's 32 values).  v is made signed, one
+//     add a pair: in O = sum p v, over many keys, an offset would cost the sum
+//     its low bits (taking it out in every step, by a product with A = -128
+//     2^-24, left values of q = 0 up to 2^-17 of the offset away from 0).
 //   * k scales multiply the f32 scores.  v scales multiply the probabilities,
 //     over a running power of two that is at least the largest of them, so
 //     that the f16 rounding of p s_v is a relative one (2^-11; the only
@@ -54,26 +61,11 @@ namespace {
 constexpr int kSWarps = 4;
 constexpr int kSThreads = 32 * kSWarps;
 constexpr int kStep = 16;                     // keys of a warp's step
-constexpr int kMinChunk = kStep * kSWarps;    // one step a warp
-constexpr int kMaxChunk = 32 * kMinChunk;     // a lane holds one page id of its warp's 32 steps
+constexpr int kUnit = kStep * kSWarps;        // one step a warp
 constexpr float kNone = -1e30f;               // the maximum of no score (finite: differences stay defined)
 constexpr float kHead = 6.0f, kJump = 14.0f;  // log2 units; see above
 
-template <int kN>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? kN : 0;  // 0: the bytes are filled with zeros
-  if constexpr (kN == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kN), "r"(n) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kLeft>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
-}
-
-// kWords 32-bit words from this lane's slot in shared memory.
+// kWords 32-bit words from shared memory.
 template <int kWords>
 __device__ __forceinline__ void lds(uint32_t at, uint32_t (&w)[kWords]) {
   if constexpr (kWords == 4)
@@ -134,11 +126,14 @@ struct Layout {
   static constexpr int kVPiece = kVLane < 16 ? kVLane : 16;
   static constexpr int kVPieces = kVLane / kVPiece;  // piece c of lane g lies at (8 c + g) kVPiece
   static constexpr int kScale = 4 * kNb;             // bytes of a token's scales, k then v
-  // a stage: [k row g, g + 8][piece], [v row][piece], [row g, g + 8] scales; 32 lanes' slots each
-  static constexpr int kOffV = 2 * kKPieces * kKPiece * 32;
-  static constexpr int kOffS = kOffV + 4 * kVPieces * kVPiece * 32;
-  static constexpr int kStage = kOffS + (kQ ? 2 * kScale * 32 : 0);
-  static constexpr int kStages = kFmt == BQ4_CACHE_F16 ? (kHP == 128 ? 2 : 3) : kFmt == BQ4_CACHE_Q8 ? 3 : 4;
+  // a stage: 16 k rows, 16 v rows, 16 tokens' scales
+  static constexpr int kOffV = kStep * kRow;
+  static constexpr int kOffS = 2 * kStep * kRow;
+  static constexpr int kStage = kOffS + kStep * kScale;
+  // CTAs of an SM with 8 rows a warp, by registers and by the ring (two with 16 rows, by registers)
+  static constexpr int kPerSm = kFmt == BQ4_CACHE_F16 && kHP == 128 ? 3 : 4;
+  static constexpr int kStages = (kPerSm == 3 ? 72 : 54) * 1024 / (kSWarps * kStage) < 8
+                                     ? (kPerSm == 3 ? 72 : 54) * 1024 / (kSWarps * kStage) : 8;
   // value d of the head that element e (0..3) of k step ks holds in lane t: at + e
   __device__ static int qd(int ks, int t) {
     return kFmt == BQ4_CACHE_Q8 ? 64 * (ks >> 2) + 16 * t + 4 * (ks & 3) : 32 * (ks >> 1) + 8 * t + 4 * (ks & 1);
@@ -158,13 +153,15 @@ struct SplitArgs {
   float c;               // scale * log2(e)
   int group;             // query heads of a kv head
   int p_tiles, s_tiles;  // row tiles of the prefix and of one sequence
-  int p_chunk, s_chunk, p_chunks, s_chunks;
-  unsigned p_items;      // CTAs of the prefix, first in the grid
   int q_vec;             // q rows lie on 8-byte boundaries
-  int direct;            // one chunk in all: rows are finished here
-  float* part;           // [row][p_chunks + s_chunks][hp]
-  float2* ml;            // [row][p_chunks + s_chunks]: m, l
+  float* part;           // [grid + ranges][8 kNT][hp]: O of piece (CTA + range)
+  float2* ml;            // [grid + ranges][8 kNT]: m, l
+  int2* pieces;          // [ranges]: first and last CTA with keys of the range
 };
+
+// A range is the line's units of one (kv head, row tile): prefix ranges
+// [kv_heads][p_tiles] first, then [batch][kv_heads][s_tiles].  Piece CTA +
+// range is unique: from one piece to the next one of them grows.
 
 // Query row r of a tile's space: its sequence, token and head.
 struct Row {
@@ -196,85 +193,148 @@ __device__ __forceinline__ int prefix_rows(const CacheAttnCall& a) {
 }
 
 template <int kFmt, int kHP, int kNT>
-__global__ void __launch_bounds__(kSThreads, kNT == 1 ? 4 : 2) cache_split_kernel(const __grid_constant__ SplitArgs s) {
+__global__ void __launch_bounds__(kSThreads, kNT == 1 ? Layout<kFmt, kHP>::kPerSm : 2)
+    cache_split_kernel(const __grid_constant__ SplitArgs s) {
   using Y = Layout<kFmt, kHP>;
   extern __shared__ __align__(16) uint8_t smem[];
   const CacheAttnCall& a = s.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   ptx::griddep_launch_dependents();
 
-  // ---- which chunk, kv head and rows
-  const bool prefix = blockIdx.x < s.p_items;
-  unsigned item = prefix ? blockIdx.x : blockIdx.x - s.p_items;
-  const int tiles = prefix ? s.p_tiles : s.s_tiles;
-  const int tile = (int)(item % (unsigned)tiles);
-  item /= (unsigned)tiles;
-  const int kvh = (int)(item % (unsigned)a.c.kv_heads);
-  item /= (unsigned)a.c.kv_heads;
-  const int b = prefix ? 0 : (int)(item % (unsigned)a.s.batch);
-  const int chunk = prefix ? (int)item : (int)(item / (unsigned)a.s.batch);
-  const int len = prefix ? s.p_chunk : s.s_chunk, key0 = chunk * len;
+  // ---- the line: units before each sequence (a thread adds up `per` of them)
+  __shared__ int64_t before[kSThreads + 1];
+  __shared__ int64_t warp_sum[kSWarps];
+  __shared__ __align__(8) uint64_t bars[kSWarps * Y::kStages];
+  __shared__ int abort_flag;
+  if (threadIdx.x < kSWarps * Y::kStages) ptx::mbar_init(&bars[threadIdx.x], 1);
+  if (threadIdx.x == 0) abort_flag = 0;
+  ptx::fence_mbar_init();
+  const int n_prefix = prefix_rows(a);
+  const int per_p = (n_prefix + kUnit - 1) / kUnit;
+  const int64_t line_p = (int64_t)per_p * a.c.kv_heads * s.p_tiles;
+  const int heads_tiles = a.c.kv_heads * s.s_tiles;
+  const int per = (a.s.batch + kSThreads - 1) / kSThreads;
+  {
+    int64_t mine = 0;
+    for (int i = 0; i < per; ++i) {
+      const int sb = (int)threadIdx.x * per + i;
+      if (sb < a.s.batch) mine += (own_length(a, sb) + kUnit - 1) / kUnit;
+    }
+    mine *= heads_tiles;
+    int64_t sum = mine;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, sum, w);
+      if (lane >= w) sum += y;
+    }
+    if (lane == 31) warp_sum[warp] = sum;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) sum += warp_sum[w];
+    before[threadIdx.x + 1] = line_p + sum;
+    if (threadIdx.x == 0) before[0] = line_p;
+    __syncthreads();
+  }
+  const int64_t line = before[kSThreads], share = (line + gridDim.x - 1) / gridDim.x;
+  int64_t at_unit = blockIdx.x * share;
+  const int64_t to_unit = min(line, at_unit + share);
+  if (at_unit >= to_unit) return;
+
+  // ---- the range that holds at_unit
+  bool prefix = at_unit < line_p;
+  int b = 0, tile, kvh, n, units;
+  int64_t first;  // of the range, along the line
+  if (prefix) {
+    const int r = (int)(at_unit / per_p);
+    tile = r % s.p_tiles;
+    kvh = r / s.p_tiles;
+    first = (int64_t)r * per_p;
+    n = n_prefix;
+    units = per_p;
+  } else {
+    int lo = 0, hi = kSThreads;  // before[lo] <= at_unit < before[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (before[mid] <= at_unit) lo = mid; else hi = mid;
+    }
+    first = before[lo];
+    b = lo * per;
+    for (;; ++b) {
+      n = own_length(a, b);
+      units = (n + kUnit - 1) / kUnit;
+      if (at_unit < first + (int64_t)units * heads_tiles) break;
+      first += (int64_t)units * heads_tiles;
+    }
+    const int r = (int)((at_unit - first) / units);
+    tile = r % s.s_tiles;
+    kvh = r / s.s_tiles;
+    first += (int64_t)r * units;
+  }
+
+  // this warp's ring: stages filled and taken so far, as slot and parity
+  const uint32_t ring = ptx::smem_u32(smem) + warp * Y::kStages * Y::kStage;
+  uint64_t* full = bars + warp * Y::kStages;
+  int put = 0, get = 0;
+  uint32_t parity = 0;
+  // lane offsets of its pieces in a stage; k rows g, g + 8 and v rows 2t (+ 8), 2t + 1 (+ 8) lie alike
+  const uint32_t k_at = cache_swizzle(0, Y::kRow, g, t * Y::kKPiece);
+  const uint32_t v_at0 = Y::kOffV + cache_swizzle(1, Y::kRow, 2 * t, g * Y::kVPiece);
+  const uint32_t v_at1 = Y::kOffV + cache_swizzle(1, Y::kRow, 2 * t + 1, g * Y::kVPiece);
+
+  for (;;) {  // a piece a turn
+  const int range = prefix ? kvh * s.p_tiles + tile
+                           : a.c.kv_heads * s.p_tiles + (b * a.c.kv_heads + kvh) * s.s_tiles + tile;
+  const int64_t piece_to = min(to_unit, first + units);
+  const int key0 = (int)(at_unit - first) * kUnit;
   const int rows = (prefix ? a.s.batch : 1) * a.tokens * s.group;
   const int row0 = tile * 8 * kNT;
   const bool causal = !prefix && a.causal;
-  const int n = prefix ? prefix_rows(a) : own_length(a, b);
   // the keys that the tile's last row sees
   const int last_i = (min(row0 + 8 * kNT, rows) - 1) / s.group;
-  const int end = min(key0 + len, causal ? n - a.tokens + last_i + 1 : n);
-  if (end <= key0 && !s.direct) return;
+  const int end = min(min(n, (int)(piece_to - first) * kUnit), causal ? n - a.tokens + last_i + 1 : n);
+  const bool whole = at_unit == first && piece_to == first + units;
+  if (at_unit == first && threadIdx.x == 0)
+    s.pieces[range] = make_int2((int)blockIdx.x, (int)((first + units - 1) / share));
   const int32_t* table = prefix ? a.prefix_table : a.s.table + b * a.s.table_stride;
 
-  // ---- page of this warp's step `lane` (-1: none)
+  // ---- pages of this warp's steps: lane j % 32 holds step j's, of the 32 steps fetched last
   const int steps = end <= key0 ? 0 : (end - key0 + kStep - 1) / kStep;
   const int mine = steps > warp ? (steps - warp + kSWarps - 1) / kSWarps : 0;
-  int page = -1, place = 0;
-  if (lane < mine) {
-    const unsigned u = (unsigned)(key0 / kStep) + (unsigned)(warp + kSWarps * lane);
-    const int pi = (int)((u * s.page_magic) >> 38);
-    page = table[pi];
-    place = (int)u * kStep - pi * a.c.page_size;
-    if (page < 0 || page >= a.c.pages) {
-      atomicCAS(a.err, 0, (int)BQ4_EINVAL_ARG);
-      page = -1;
-    }
-  }
+  int page = 0, place = 0;
+  unsigned held = 0, held_before = 0;  // bit j % 32: step j's page exists; of the 32 steps before them
 
-  // ---- copies of one step into stage st of this warp's ring
-  const uint32_t ring = ptx::smem_u32(smem) + warp * Y::kStages * Y::kStage;
+  // ---- bulk copies of step j into the ring
   const int64_t head_at = (int64_t)kvh * 2 * a.c.kv_bytes;
   auto fetch = [&](int j) {
-    if (j < mine) {
-      const int pg = __shfl_sync(0xffffffffu, page, j), pl = __shfl_sync(0xffffffffu, place, j);
-      const int left = pg < 0 ? 0 : end - (key0 + (warp + kSWarps * j) * kStep);  // valid keys of the step
-      const uint8_t* k = a.c.values + (int64_t)max(pg, 0) * s.page_stride + head_at + pl * Y::kRow;
-      const uint8_t* v = k + a.c.kv_bytes;
-      const uint32_t st = ring + (j % Y::kStages) * Y::kStage;
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int c = 0; c < Y::kKPieces; ++c)
-          copy_async<Y::kKPiece>(st + ((r * Y::kKPieces + c) * 32 + lane) * Y::kKPiece,
-                                 k + (g + 8 * r) * Y::kRow + (4 * c + t) * Y::kKPiece, g + 8 * r < left);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = 2 * t + (r & 1) + 8 * (r >> 1);
-#pragma unroll
-        for (int c = 0; c < Y::kVPieces; ++c)
-          copy_async<Y::kVPiece>(st + Y::kOffV + ((r * Y::kVPieces + c) * 32 + lane) * Y::kVPiece,
-                                 v + key * Y::kRow + (8 * c + g) * Y::kVPiece, key < left);
+    if (j >= mine) return;
+    if ((j & 31) == 0) {
+      bool ok = false;
+      if (j + lane < mine) {
+        const unsigned u = (unsigned)(key0 / kStep) + (unsigned)(warp + kSWarps * (j + lane));
+        const int pi = (int)((u * s.page_magic) >> 38);
+        page = table[pi];
+        place = (int)u * kStep - pi * a.c.page_size;
+        ok = page >= 0 && page < a.c.pages;
+        if (!ok) atomicCAS(a.err, 0, (int)BQ4_EINVAL_ARG);
       }
-      if constexpr (Y::kQ) {
-        const uint8_t* sc = reinterpret_cast<const uint8_t*>(a.c.scales) +
-                            (((int64_t)max(pg, 0) * a.c.kv_heads + kvh) * a.c.page_size + pl) * Y::kScale;
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          copy_async<Y::kScale>(st + Y::kOffS + (r * 32 + lane) * Y::kScale, sc + (g + 8 * r) * Y::kScale,
-                                g + 8 * r < left);
-      }
+      held_before = held;
+      held = __ballot_sync(0xffffffffu, ok);
     }
-    copy_commit();  // an empty group past the end keeps the count
+    if (!(held >> (j & 31) & 1)) return;
+    const int pg = __shfl_sync(0xffffffffu, page, j & 31), pl = __shfl_sync(0xffffffffu, place, j & 31);
+    if (lane == 0) {
+      const uint8_t* k = a.c.values + (int64_t)pg * s.page_stride + head_at + pl * Y::kRow;
+      uint8_t* st = smem + (warp * Y::kStages + put) * Y::kStage;
+      ptx::mbar_arrive_expect_tx(&full[put], Y::kStage);
+      ptx::bulk_load(st, k, kStep * Y::kRow, &full[put]);
+      ptx::bulk_load(st + Y::kOffV, k + a.c.kv_bytes, kStep * Y::kRow, &full[put]);
+      if constexpr (Y::kQ)
+        ptx::bulk_load(st + Y::kOffS,
+                       reinterpret_cast<const uint8_t*>(a.c.scales) +
+                           (((int64_t)pg * a.c.kv_heads + kvh) * a.c.page_size + pl) * Y::kScale,
+                       kStep * Y::kScale, &full[put]);
+    }
+    put = put + 1 == Y::kStages ? 0 : put + 1;
   };
-#pragma unroll
   for (int j = 0; j < Y::kStages - 1; ++j) fetch(j);
 
   // ---- q fragments; the offset's start values; what each row sees
@@ -347,11 +407,23 @@ __global__ void __launch_bounds__(kSThreads, kNT == 1 ? 4 : 2) cache_split_kerne
   const float c = Y::kQ ? s.c * 0x1p24f : s.c;
 
   for (int j = 0; j < mine; ++j) {
+    __syncwarp();  // the slot that is filled next has been read by every lane
     fetch(j + Y::kStages - 1);
-    copy_wait<Y::kStages - 1>();
-    const uint32_t st = ring + (j % Y::kStages) * Y::kStage;
     const int at = key0 + (warp + kSWarps * j) * kStep;
-    if (__shfl_sync(0xffffffffu, page, j) < 0) continue;  // a bad page holds nothing
+    {
+      // the fetches are kStages - 1 steps ahead, perhaps among the next 32 already
+      const bool next = (min(j + Y::kStages - 1, mine - 1) >> 5) != (j >> 5);
+      if (!((next ? held_before : held) >> (j & 31) & 1)) continue;  // a bad page holds nothing
+    }
+    const uint32_t st = ring + get * Y::kStage;
+    if (!__all_sync(0xffffffffu, ptx::mbar_wait(&full[get], parity, &abort_flag))) {
+      if (lane == 0) {
+        abort_flag = 1;
+        atomicCAS(a.err, 0, (int)BQ4_ETIMEOUT);
+      }
+      break;
+    }
+    if (++get == Y::kStages) get = 0, parity ^= 1;
 
     // ---- scales of keys g, g + 8
     float sk[2][Y::kQ ? Y::kNb : 1], sv[2][Y::kQ ? Y::kNb : 1];
@@ -359,7 +431,7 @@ __global__ void __launch_bounds__(kSThreads, kNT == 1 ? 4 : 2) cache_split_kerne
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         uint32_t w[Y::kNb];
-        lds(st + Y::kOffS + (r * 32 + lane) * Y::kScale, w);
+        lds(st + Y::kOffS + (g + 8 * r) * Y::kScale, w);
         if constexpr (kFmt == BQ4_CACHE_Q8) {
           sk[r][0] = __uint_as_float(w[0] << 16);
           sv[r][0] = __uint_as_float(w[0] & 0xffff0000u);
@@ -384,8 +456,9 @@ __global__ void __launch_bounds__(kSThreads, kNT == 1 ? 4 : 2) cache_split_kerne
 #pragma unroll
     for (int p = 0; p < Y::kKPieces; ++p) {
       uint32_t w0[Y::kKPiece / 4], w1[Y::kKPiece / 4];
-      lds(st + (p * 32 + lane) * Y::kKPiece, w0);
-      lds(st + ((Y::kKPieces + p) * 32 + lane) * Y::kKPiece, w1);
+      const uint32_t from = st + (k_at ^ p << 6);  // 4 pieces of 16 bytes on; the swizzle is in bit 6
+      lds(from, w0);
+      lds(from + 8 * Y::kRow, w1);
       if constexpr (kFmt == BQ4_CACHE_F16) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -433,6 +506,7 @@ __global__ void __launch_bounds__(kSThreads, kNT == 1 ? 4 : 2) cache_split_kerne
       for (int u = 0; u < 4; ++u) x[nt][u] *= kFmt == BQ4_CACHE_Q8 ? sk[u >> 1][0] * c : c;
 
     // ---- mask; a step below see_all has none
+    // (rows behind the end hold anything)
     const bool edge = at + kStep > see_all;
     if (edge) {
 #pragma unroll
@@ -450,6 +524,13 @@ __global__ void __launch_bounds__(kSThreads, kNT == 1 ? 4 : 2) cache_split_kerne
       for (int e = 0; e < 2; ++e) move |= fmaxf(x[nt][e], x[nt][e + 2]) > m[nt][e] + kJump;
     float sv_top = 0.0f;
     if constexpr (Y::kQ) {
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          if (at + g + 8 * r >= end)
+#pragma unroll
+            for (int e = 0; e < Y::kNb; ++e) sv[r][e] = 0.0f;
+      }
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -531,7 +612,7 @@ __global__ void __launch_bounds__(kSThreads, kNT == 1 ? 4 : 2) cache_split_kerne
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int p = 0; p < Y::kVPieces; ++p)
-        lds(st + Y::kOffV + ((r * Y::kVPieces + p) * 32 + lane) * Y::kVPiece, v[r][p]);
+        lds(st + (r & 1 ? v_at1 : v_at0) + (r >> 1) * 8 * Y::kRow + p * 128, v[r][p]);
     if constexpr (kFmt == BQ4_CACHE_F16) {
       weigh(0);
 #pragma unroll
@@ -617,8 +698,18 @@ __global__ void __launch_bounds__(kSThreads, kNT == 1 ? 4 : 2) cache_split_kerne
   }
 
   // ---- join the four warps through shared memory, in warp order
-  copy_wait<0>();
   __syncthreads();
+  if (abort_flag) {
+    // a copy did not come: wait once more for those under way, then leave
+    __shared__ int never;
+    if (threadIdx.x == 0) never = 0;
+    __syncthreads();
+    for (; get != put; get = get + 1 == Y::kStages ? 0 : get + 1) {
+      ptx::mbar_wait(&full[get], parity, &never);
+      if (get + 1 == Y::kStages) parity ^= 1;
+    }
+    return;
+  }
   float* om = reinterpret_cast<float*>(smem);                                  // [warp][row][kHP + 4]
   float2* mlw = reinterpret_cast<float2*>(om + kSWarps * 8 * kNT * (kHP + 4));  // [warp][row]
   const float unit = Y::kQ ? vs * 0x1p24f : 1.0f;
@@ -639,7 +730,8 @@ __global__ void __launch_bounds__(kSThreads, kNT == 1 ? 4 : 2) cache_split_kerne
       }
     }
   __syncthreads();
-  const int slots = s.p_chunks + s.s_chunks, slot = prefix ? chunk : s.p_chunks + chunk;
+  const int64_t piece = ((int64_t)blockIdx.x + range) * 8 * kNT;
+  const bool finish = whole && line_p == 0;
   for (int i = threadIdx.x; i < 8 * kNT * (kHP / 4); i += kSThreads) {
     const int r = i / (kHP / 4), d = 4 * (i - r * (kHP / 4));
     if (row0 + r >= rows) break;
@@ -656,36 +748,70 @@ __global__ void __launch_bounds__(kSThreads, kNT == 1 ? 4 : 2) cache_split_kerne
       lsum += f * e.y;
       sum.x += f * y.x, sum.y += f * y.y, sum.z += f * y.z, sum.w += f * y.w;
     }
-    const Row w = row_of(s, prefix, b, kvh, row0 + r);
-    const int64_t row = ((int64_t)w.b * a.tokens + w.i) * a.q_heads + w.h;
-    if (s.direct) {
+    if (finish) {
       if (d < a.c.head_dim) {
+        const Row w = row_of(s, prefix, b, kvh, row0 + r);
+        const int64_t row = ((int64_t)w.b * a.tokens + w.i) * a.q_heads + w.h;
         const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
         const uint2 u = make_uint2(pack_h2(sum.x * inv, sum.y * inv), pack_h2(sum.z * inv, sum.w * inv));
         *reinterpret_cast<uint2*>(a.out + row * a.c.head_dim + d) = u;
       }
     } else {
-      *reinterpret_cast<float4*>(s.part + (row * slots + slot) * kHP + d) = sum;
-      if (d == 0) s.ml[row * slots + slot] = make_float2(top, lsum);
+      *reinterpret_cast<float4*>(s.part + (piece + r) * kHP + d) = sum;
+      if (d == 0) s.ml[piece + r] = make_float2(top, lsum);
     }
+  }
+
+  // ---- the next range of the line
+  at_unit = piece_to;
+  if (at_unit >= to_unit) return;
+  ptx::fence_proxy_async_smem();  // the copies write where the warps were joined
+  __syncthreads();
+  first += units;
+  if (++tile == (prefix ? s.p_tiles : s.s_tiles)) {
+    tile = 0;
+    if (++kvh == a.c.kv_heads) {
+      kvh = 0;
+      b = prefix ? 0 : b + 1;
+      prefix = false;
+      for (;; ++b) {
+        n = own_length(a, b);
+        units = (n + kUnit - 1) / kUnit;
+        if (units) break;
+      }
+    }
+  }
   }
 }
 
-// Joins a row's chunks in their order: one warp a row, four values a lane.
-__global__ void __launch_bounds__(kSThreads) cache_join_kernel(const __grid_constant__ SplitArgs s, unsigned rows) {
+// Joins the pieces of a row, the prefix's and then its own in their order: one
+// warp a row, four values a lane.
+__global__ void __launch_bounds__(kSThreads) cache_join_kernel(const __grid_constant__ SplitArgs s, unsigned rows,
+                                                               int tile_rows) {
   const CacheAttnCall& a = s.a;
   const unsigned row = blockIdx.x * kSWarps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, d = 4 * lane;
   ptx::griddep_wait();
   if (row >= rows) return;
-  const unsigned bi = row / (unsigned)a.q_heads;
-  const unsigned b = bi / (unsigned)a.tokens;
-  int n = own_length(a, (int)b);
-  if (a.causal) n = n - a.tokens + (int)(bi - b * a.tokens) + 1;
-  const int np = (prefix_rows(a) + s.p_chunk - 1) / s.p_chunk;
-  const int nc = np + (max(n, 0) + s.s_chunk - 1) / s.s_chunk;
-  const int64_t at = (int64_t)row * (s.p_chunks + s.s_chunks);
-  auto slot = [&](int i) { return at + (i < np ? i : s.p_chunks + i - np); };
+  const int bi = (int)(row / (unsigned)a.q_heads), h = (int)row - bi * a.q_heads;
+  const int b = bi / a.tokens, kvh = h / s.group;
+  const int own = (bi - b * a.tokens) * s.group + h - kvh * s.group;  // row among the sequence's
+  const int all = b * a.tokens * s.group + own;                       // among the prefix's
+  const bool have_p = prefix_rows(a) > 0, have_s = own_length(a, b) > 0;
+  int range[2], local[2];
+  int2 cta[2] = {make_int2(0, -1), make_int2(0, -1)};
+  range[0] = kvh * s.p_tiles + all / tile_rows;
+  local[0] = all % tile_rows;
+  range[1] = a.c.kv_heads * s.p_tiles + (b * a.c.kv_heads + kvh) * s.s_tiles + own / tile_rows;
+  local[1] = own % tile_rows;
+  if (have_p) cta[0] = s.pieces[range[0]];
+  if (have_s) cta[1] = s.pieces[range[1]];
+  if (!have_p && have_s && cta[1].x == cta[1].y) return;  // finished by the one piece
+  const int np = cta[0].y - cta[0].x + 1, nc = np + cta[1].y - cta[1].x + 1;
+  auto slot = [&](int i) {
+    return i < np ? ((int64_t)cta[0].x + i + range[0]) * tile_rows + local[0]
+                  : ((int64_t)cta[1].x + (i - np) + range[1]) * tile_rows + local[1];
+  };
   float top = kNone;
   for (int i = lane; i < nc; i += 32) top = fmaxf(top, s.ml[slot(i)].x);
 #pragma unroll
@@ -711,21 +837,16 @@ __global__ void __launch_bounds__(kSThreads) cache_join_kernel(const __grid_cons
 
 // ------------------------------------------------------------------ host side
 
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
 struct SplitPlan {
-  int nt, p_tiles, s_tiles, p_chunk, s_chunk, p_chunks, s_chunks;
-  int64_t p_items, s_items, slots, rows;
-  size_t part_bytes, ml_bytes;
+  int nt, p_tiles, s_tiles, grid;
+  int64_t rows;
+  size_t part_bytes, ml_bytes, pieces_bytes;
 };
 
-// Chunks of `keys` keys for `units` (kv head, row tile) pairs: as long as they
-// leave three CTAs for every one that the GPU holds at a time (four an SM),
-// so that sequences of unequal length even out.
-int pick_chunk(int64_t keys, int64_t units, int sms) {
-  const int64_t want = 3LL * 4 * sms;
-  const int64_t per = keys * units / want / kMinChunk * kMinChunk;
-  return (int)std::min<int64_t>(std::max<int64_t>(per, kMinChunk), kMaxChunk);
-}
-
+// CTAs: what the GPU holds at a time, or fewer where the lengths' bounds give
+// fewer units.
 bool plan_split(const CacheAttnCall& a, int sms, SplitPlan* p) {
   const int group = a.q_heads / a.c.kv_heads;
   const int64_t own = (int64_t)a.tokens * group, all = own * a.s.batch;
@@ -734,19 +855,19 @@ bool plan_split(const CacheAttnCall& a, int sms, SplitPlan* p) {
   const int tile = 8 * p->nt;
   p->s_tiles = (int)((own + tile - 1) / tile);
   p->p_tiles = (int)((all + tile - 1) / tile);
-  p->s_chunk = pick_chunk(a.max_length, (int64_t)a.s.batch * a.c.kv_heads * p->s_tiles, sms);
-  p->p_chunk = pick_chunk(prefix, (int64_t)a.c.kv_heads * p->p_tiles, sms);
-  p->s_chunks = (int)(((int64_t)a.max_length + p->s_chunk - 1) / p->s_chunk);
-  p->p_chunks = (int)((prefix + p->p_chunk - 1) / p->p_chunk);
-  if (p->s_chunks + p->p_chunks == 0) p->s_chunks = 1;  // no keys at all: the rows are still written
-  p->s_items = (int64_t)p->s_chunks * a.s.batch * a.c.kv_heads * p->s_tiles;
-  p->p_items = (int64_t)p->p_chunks * a.c.kv_heads * p->p_tiles;
-  p->slots = (int64_t)p->s_chunks + p->p_chunks;
+  const int64_t ranges = ((int64_t)p->p_tiles + (int64_t)a.s.batch * p->s_tiles) * a.c.kv_heads;
+  const int64_t per = ((int64_t)a.max_length + kUnit - 1) / kUnit, per_p = (prefix + kUnit - 1) / kUnit;
+  const int per_sm = p->nt == 2 ? 2 : a.c.format == BQ4_CACHE_F16 && a.c.hp == 128 ? 3 : 4;  // Layout::kPerSm
+  const int64_t most = (int64_t)per_sm * sms;
+  const int64_t units = std::min(most, per_p * p->p_tiles * a.c.kv_heads) +
+                        std::min(most, per * std::min(most, (int64_t)a.s.batch * p->s_tiles * a.c.kv_heads));
+  p->grid = (int)std::max<int64_t>(1, std::min(most, units));
   p->rows = (int64_t)a.s.batch * a.tokens * a.q_heads;
-  if (p->s_items + p->p_items > 0x7fffffff || p->rows * p->slots > ((int64_t)1 << 40)) return false;
-  const bool direct = p->slots == 1;
-  p->part_bytes = direct ? 0 : (size_t)(p->rows * p->slots) * a.c.hp * 4;
-  p->ml_bytes = direct ? 0 : (size_t)(p->rows * p->slots) * 8;
+  const int64_t slots = (ranges + p->grid) * tile;
+  if (ranges > 0x3fffffff || slots > ((int64_t)1 << 40)) return false;
+  p->part_bytes = up256((size_t)slots * a.c.hp * 4);
+  p->ml_bytes = up256((size_t)slots * 8);
+  p->pieces_bytes = up256((size_t)ranges * 8);
   return true;
 }
 
@@ -760,7 +881,7 @@ cudaError_t launch_split(const SplitArgs& s, unsigned grid, cudaStream_t stream)
   static std::atomic<uint64_t> ready{0};  // a bit for each device
   int dev = 0;
   cudaGetDevice(&dev);
-  if (kSmem > 48 * 1024 && (dev < 0 || dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
+  if (kSmem > 46 * 1024 /* the static part comes on top */ && (dev < 0 || dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
@@ -779,22 +900,20 @@ cudaError_t launch_head(const SplitArgs& s, int nt, unsigned grid, cudaStream_t 
   return s.a.c.hp == 64 ? launch_rows<kFmt, 64>(s, nt, grid, stream) : launch_rows<kFmt, 128>(s, nt, grid, stream);
 }
 
-size_t up256(size_t v) { return (v + 255) / 256 * 256; }
-
 }  // namespace
 
 bq4_status cache_attn_workspace(const CacheAttnCall& a, int sms, size_t* bytes) {
   SplitPlan p;
   if (!plan_split(a, sms, &p))
-    return set_error(BQ4_EINVAL_SHAPE, "cache attention: too many rows and chunks for one launch");
-  *bytes = up256(p.part_bytes) + up256(p.ml_bytes);
+    return set_error(BQ4_EINVAL_SHAPE, "cache attention: too many rows for one launch");
+  *bytes = p.part_bytes + p.ml_bytes + p.pieces_bytes;
   return BQ4_OK;
 }
 
 bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, cudaStream_t stream) {
   SplitPlan p;
   if (!plan_split(a, sms, &p))
-    return set_error(BQ4_EINVAL_SHAPE, "cache attention: too many rows and chunks for one launch");
+    return set_error(BQ4_EINVAL_SHAPE, "cache attention: too many rows for one launch");
   SplitArgs s;
   s.a = a;
   const uint64_t unit = (uint64_t)(a.c.page_size / kStep);
@@ -804,24 +923,19 @@ bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, cuda
   s.group = a.q_heads / a.c.kv_heads;
   s.p_tiles = p.p_tiles;
   s.s_tiles = p.s_tiles;
-  s.p_chunk = p.p_chunk;
-  s.s_chunk = p.s_chunk;
-  s.p_chunks = p.p_chunks;
-  s.s_chunks = p.s_chunks;
-  s.p_items = (unsigned)p.p_items;
   s.q_vec = reinterpret_cast<uintptr_t>(a.q) % 8 == 0 && a.q_stride[0] % 4 == 0 && a.q_stride[1] % 4 == 0 &&
             a.q_stride[2] % 4 == 0;
-  s.direct = p.slots == 1;
-  s.part = static_cast<float*>(workspace);
-  s.ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + up256(p.part_bytes));
-  const unsigned grid = (unsigned)(p.p_items + p.s_items);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  s.part = reinterpret_cast<float*>(ws);
+  s.ml = reinterpret_cast<float2*>(ws + p.part_bytes);
+  s.pieces = reinterpret_cast<int2*>(ws + p.part_bytes + p.ml_bytes);
+  const unsigned grid = (unsigned)p.grid;
   cudaError_t e = a.c.format == BQ4_CACHE_F16  ? launch_head<BQ4_CACHE_F16>(s, p.nt, grid, stream)
                   : a.c.format == BQ4_CACHE_Q8 ? launch_head<BQ4_CACHE_Q8>(s, p.nt, grid, stream)
                                                : launch_head<BQ4_CACHE_Q4>(s, p.nt, grid, stream);
   note_launch();
   if (e != cudaSuccess) return check_cuda(e, "cache attention launch");
-  if (s.direct) return BQ4_OK;
-  // the join is launched ahead and waits on the device for the chunks
+  // the join is launched ahead and waits on the device for the pieces
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((p.rows + kSWarps - 1) / kSWarps));
   cfg.blockDim = dim3(kSThreads);
@@ -831,7 +945,7 @@ bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, cuda
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, cache_join_kernel, s, (unsigned)p.rows);
+  e = cudaLaunchKernelEx(&cfg, cache_join_kernel, s, (unsigned)p.rows, 8 * p.nt);
   note_launch();
   return check_cuda(e, "cache attention join launch");
 }
