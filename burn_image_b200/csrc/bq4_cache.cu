@@ -3,11 +3,12 @@
 // attention kernels are in bq4_cache_attn.cu).
 //
 // Both kernels move each byte once and compute next to nothing, so HBM (and,
-// for a decode step's few rows, the launch) bounds them.  A row of HP values
-// is taken by HP / 4 lanes, four consecutive values each: 16- or 8-byte
-// accesses on the wide side, the block maximum by shuffles over the 8 lanes
-// of a q4 block or all lanes of a q8 row, and one store of 4 (q8), 2 (q4) or
-// 8 (f16) bytes a lane on the cache side.
+// for a decode step's few rows, the launch) bounds them.  A warp takes 4 to 16
+// neighbouring positions of one page, for one head's k or v, as many as it
+// loads before it uses the first: page, row and
+// sequence are worked out once for them.  A row of HP values is taken by HP / W
+// lanes, W consecutive values each, W such that the wide side moves 16 bytes a
+// lane (8 f16 or 4 f32); the block maximum comes from shuffles.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -26,7 +27,8 @@ struct CacheRow {
   uint16_t* scales;
 };
 
-// Rows of (page, head) and the scales of the row at `place`; kv: 0 k, 1 v.
+// Rows of (page, head) and the scales of the row at `place`; kv: 0 k, 1 v.  The next
+// row's scales lie 2 nb on.
 __device__ __forceinline__ CacheRow cache_row(const CacheView& c, int page, int head, int place, int kv) {
   const int64_t ph = (int64_t)page * c.kv_heads + head;
   CacheRow r;
@@ -46,118 +48,214 @@ __device__ __forceinline__ int seq_length(const SeqView& s, int page_size, int b
   return n;
 }
 
-template <bool kF16>
-__device__ __forceinline__ void load4(const void* base, int64_t at, bool vec, float (&x)[4]) {
+// kW consecutive values at element `at`, in f32; vec: they lie on 16 bytes.
+template <bool kF16, int kW>
+__device__ __forceinline__ void load_values(const void* base, int64_t at, bool vec, float (&x)[kW]) {
   if constexpr (kF16) {
     const __half* p = static_cast<const __half*>(base) + at;
     if (vec) {
-      const uint2 u = *reinterpret_cast<const uint2*>(p);
-      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-      const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-      x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+      uint32_t u[kW / 2];
+      if constexpr (kW == 8)
+        *reinterpret_cast<uint4*>(u) = __ldg(reinterpret_cast<const uint4*>(p));
+      else
+        *reinterpret_cast<uint2*>(u) = __ldg(reinterpret_cast<const uint2*>(p));
+#pragma unroll
+      for (int j = 0; j < kW / 2; ++j) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
+        x[2 * j] = f.x, x[2 * j + 1] = f.y;
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = __half2float(p[j]);
+      for (int j = 0; j < kW; ++j) x[j] = __half2float(p[j]);
     }
   } else {
     const float* p = static_cast<const float*>(base) + at;
     if (vec) {
-      const float4 u = *reinterpret_cast<const float4*>(p);
-      x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+#pragma unroll
+      for (int j = 0; j < kW; j += 4) {
+        const float4 u = __ldg(reinterpret_cast<const float4*>(p + j));
+        x[j] = u.x, x[j + 1] = u.y, x[j + 2] = u.z, x[j + 3] = u.w;
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = p[j];
+      for (int j = 0; j < kW; ++j) x[j] = p[j];
     }
   }
 }
+
+// n bytes (2, 4, 8 or 16) of packed words.
+template <int kBytes>
+__device__ __forceinline__ void store_words(uint8_t* dst, const uint32_t* w) {
+  if constexpr (kBytes == 2)
+    *reinterpret_cast<uint16_t*>(dst) = (uint16_t)w[0];
+  else if constexpr (kBytes == 4)
+    *reinterpret_cast<uint32_t*>(dst) = w[0];
+  else if constexpr (kBytes == 8)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  else
+    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <int kBytes>
+__device__ __forceinline__ void load_words(const uint8_t* src, uint32_t* w) {
+  if constexpr (kBytes == 2)
+    w[0] = *reinterpret_cast<const uint16_t*>(src);
+  else if constexpr (kBytes == 4)
+    w[0] = *reinterpret_cast<const uint32_t*>(src);
+  else if constexpr (kBytes == 8)
+    *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(src);
+  else
+    *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(src);
+}
+
+// How a warp of the append and of the read kernel (kF16: of f16 rows) takes
+// rows: kW values a lane, kLanes lanes a row, kPer rows at a time, kTake in all.
+template <int kHP>
+struct TakeAppend {
+  static constexpr int kW = 8, kLanes = kHP / kW, kPer = 32 / kLanes, kRounds = kPer < 4 ? 4 : 2;
+  static constexpr int kTake = kPer * kRounds;
+};
+template <bool kF16, int kHP>
+struct TakeRead {
+  static constexpr int kW = kF16 ? 8 : 4, kLanes = kHP / kW, kPer = 32 / kLanes, kRounds = 4;
+  static constexpr int kTake = kPer * kRounds;
+};
 
 struct AppendArgs {
   CacheView c;
   SeqView s;
   const void* x[2];       // k, v
   int64_t stride[2][3];   // batch, token, head
-  int vec;                // every row of x starts on a 4-value boundary
-  int tokens;
-  unsigned rows;          // batch * tokens * kv_heads
+  int vec;                // every row of x lies on 16 bytes
+  int tokens, steps;      // steps: the most warps that a sequence's new rows of a head take
+  unsigned items;         // batch * steps * kv_heads * 2
   int* err;
 };
 
-// One row a group of HP / 4 lanes; blockIdx.y: k or v.
-template <int kFmt, bool kF16>
-__global__ void __launch_bounds__(kCThreads) cache_append_kernel(const AppendArgs a) {
-  const int kv = blockIdx.y;
-  const int lpr = a.c.hp >> 2;                     // lanes of a row: 16 or 32
-  const int L = threadIdx.x & (lpr - 1), d0 = 4 * L;
-  const unsigned row = blockIdx.x * (unsigned)(kCThreads / lpr) + threadIdx.x / lpr;
-  int page = -1, place = 0, h = 0;
-  float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (row < a.rows) {
-    const unsigned bi = row / (unsigned)a.c.kv_heads;
-    h = (int)(row - bi * a.c.kv_heads);
-    const unsigned b = bi / (unsigned)a.tokens, i = bi - b * a.tokens;
-    const int pos = seq_length(a.s, a.c.page_size, (int)b, a.err) - a.tokens + (int)i;
-    if (pos >= 0) {
-      const int pi = pos / a.c.page_size;
-      page = a.s.table[b * a.s.table_stride + pi];
-      place = pos - pi * a.c.page_size;
-      if (page < 0 || page >= a.c.pages) {
-        atomicCAS(a.err, 0, (int)BQ4_EINVAL_ARG);
-        page = -1;
+__device__ __forceinline__ int page_of(const CacheView& c, const SeqView& s, int b, int base, int* place, int* err) {
+  const int pi = base / c.page_size;
+  const int page = s.table[b * s.table_stride + pi];
+  *place = base - pi * c.page_size;
+  if (page >= 0 && page < c.pages) return page;
+  atomicCAS(err, 0, (int)BQ4_EINVAL_ARG);
+  return -1;
+}
+
+template <int kFmt, bool kF16, int kHP>
+__global__ void __launch_bounds__(kCThreads) cache_append_kernel(const __grid_constant__ AppendArgs a) {
+  using T = TakeAppend<kHP>;
+  constexpr int kW = T::kW, kLanes = T::kLanes, kPer = T::kPer, kAhead = T::kRounds, kTake = T::kTake;
+  constexpr int kRow = kFmt == BQ4_CACHE_F16 ? 2 * kHP : kFmt == BQ4_CACHE_Q8 ? kHP : kHP / 2;
+  constexpr int kNb = kFmt == BQ4_CACHE_Q8 ? 1 : kHP / kCacheBlock;
+  const int lane = threadIdx.x & 31, L = lane % kLanes, sub = lane / kLanes, d0 = kW * L;
+  unsigned item = (blockIdx.x * kCThreads + threadIdx.x) >> 5;
+  if (item >= a.items) return;
+  // kv, then head, fastest: neighbouring warps read neighbouring rows
+  const int kv = item & 1;
+  item >>= 1;
+  const int head = (int)(item % (unsigned)a.c.kv_heads);
+  item /= (unsigned)a.c.kv_heads;
+  const int b = (int)(item / (unsigned)a.steps), step = (int)(item - (unsigned)b * a.steps);
+  const int end = seq_length(a.s, a.c.page_size, b, a.err), from = end - a.tokens, first = max(from, 0);
+  const int base = (first & ~(kTake - 1)) + kTake * step;
+  if (base >= end) return;
+  int place0;
+  const int page = page_of(a.c, a.s, b, base, &place0, a.err);
+  if (page < 0) return;
+  const CacheRow r = cache_row(a.c, page, head, place0, kv);
+  const int64_t src = b * a.stride[kv][0] + head * a.stride[kv][2] + d0;
+
+  {
+    float xs[kAhead][kW];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int pos = base + j * kPer + sub;
+#pragma unroll
+      for (int e = 0; e < kW; ++e) xs[j][e] = 0.0f;
+      if (pos >= first && pos < end && d0 < a.c.head_dim)
+        load_values<kF16, kW>(a.x[kv], src + (int64_t)(pos - from) * a.stride[kv][1], a.vec, xs[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int row = j * kPer + sub;
+      const bool live = base + row >= first && base + row < end;
+      if (!__any_sync(0xffffffffu, live)) continue;
+      float(&x)[kW] = xs[j];
+      auto dst = [&](int at) { return r.rows + cache_swizzle(kv, kRow, place0 + row, at); };
+      uint16_t* sc = r.scales + row * 2 * kNb;
+      if constexpr (kFmt == BQ4_CACHE_F16) {
+        uint32_t w[kW / 2];
+#pragma unroll
+        for (int e = 0; e < kW / 2; ++e) {
+          const __half2 h = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+          w[e] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        if (live) store_words<2 * kW>(dst(2 * d0), w);
+      } else {
+        constexpr float kTop = kFmt == BQ4_CACHE_Q8 ? 127.0f : 7.0f;
+        float top = 0.0f;
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < kW; ++e) {
+          top = fmaxf(top, fabsf(x[e]));
+          odd |= !(fabsf(x[e]) <= 3.402823466e38f);
+        }
+        if (odd) top = INFINITY;  // infinities and NaN
+#pragma unroll
+        for (int o = (kFmt == BQ4_CACHE_Q8 ? kLanes : kCacheBlock / kW) >> 1; o; o >>= 1)
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // f32 quotients, rounded to nearest: the scale and every q follow from the
+        // definition bit for bit.
+        const __nv_bfloat16 sb = __float2bfloat16_rn(top == INFINITY ? __int_as_float(0x7fc00000)
+                                                                     : __fdiv_rn(top, kTop));
+        const float s = __bfloat162float(sb);
+        uint32_t q[kW];  // u = q + 128 or q + 8
+        // x (1 / s) is the quotient but for three roundings, 2^-22 of at most 2^7.1: where it lies
+        // 2^-14 or more from a half, both round to the same whole number.  The divisions are
+        // left for a lane that holds another one, and for scales whose inverse is not normal.
+        const float inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
+        bool near = s > 0.0f && !(s >= 0x1p-120f && s <= 0x1p120f);
+        float whole[kW];
+#pragma unroll
+        for (int e = 0; e < kW; ++e) {
+          const float y = x[e] * inv;
+          whole[e] = rintf(y);
+          near |= fabsf(y - whole[e]) > 0.5f - 0x1p-14f;
+        }
+        if (near) {
+#pragma unroll
+          for (int e = 0; e < kW; ++e) whole[e] = rintf(__fdiv_rn(x[e], s));
+        }
+#pragma unroll
+        for (int e = 0; e < kW; ++e)
+          q[e] = (uint32_t)((int)fminf(fmaxf(whole[e], -kTop), kTop) + (kFmt == BQ4_CACHE_Q8 ? 128 : 8));
+        if constexpr (kFmt == BQ4_CACHE_Q8) {
+          uint32_t w[kW / 4];
+#pragma unroll
+          for (int e = 0; e < kW / 4; ++e)
+            w[e] = q[4 * e] | q[4 * e + 1] << 8 | q[4 * e + 2] << 16 | q[4 * e + 3] << 24;
+          if (live) {
+            store_words<kW>(dst(d0), w);
+            if (L == 0) sc[0] = __bfloat16_as_ushort(sb);
+          }
+        } else {
+          const int blk = d0 >> 5;
+          if (kv == 0) {
+            // value o of the 8 of a word: nibble o / 2 + 4 (o & 1)
+            uint32_t w = 0;
+#pragma unroll
+            for (int e = 0; e < kW; ++e) w |= q[e] << (4 * (e >> 1) + 16 * (e & 1));
+            if (live) store_words<4>(dst(4 * (((d0 >> 3) & 3) * kNb + blk)), &w);
+          } else {
+#pragma unroll
+            for (int e = 0; e < kW; e += 4) {
+              const uint32_t w = q[e] | q[e + 1] << 4 | q[e + 2] << 8 | q[e + 3] << 12;
+              if (live) store_words<2>(dst(2 * ((((d0 + e) >> 2) & 7) * kNb + blk)), &w);
+            }
+          }
+          if (live && (d0 & 31) == 0) sc[blk] = __bfloat16_as_ushort(sb);
+        }
       }
     }
-    if (page >= 0 && d0 < a.c.head_dim)
-      load4<kF16>(a.x[kv], b * a.stride[kv][0] + i * a.stride[kv][1] + h * a.stride[kv][2] + d0, a.vec, x);
-  }
-  const CacheRow r = cache_row(a.c, page < 0 ? 0 : page, h, place, kv);
-  auto dst = [&](int at) { return r.rows + cache_swizzle(kv, a.c.row_bytes, place, at); };
-  if constexpr (kFmt == BQ4_CACHE_F16) {
-    const __half2 lo = __floats2half2_rn(x[0], x[1]), hi = __floats2half2_rn(x[2], x[3]);
-    uint2 u;
-    u.x = *reinterpret_cast<const uint32_t*>(&lo);
-    u.y = *reinterpret_cast<const uint32_t*>(&hi);
-    if (page >= 0) *reinterpret_cast<uint2*>(dst(8 * L)) = u;
-    return;
-  }
-  constexpr float kTop = kFmt == BQ4_CACHE_Q8 ? 127.0f : 7.0f;
-  float top = 0.0f;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float m = fabsf(x[j]);
-    top = m <= 3.402823466e38f ? fmaxf(top, m) : INFINITY;  // NaN too; INFINITY stays the maximum
-    if (top == INFINITY) break;
-  }
-  const int span = kFmt == BQ4_CACHE_Q8 ? lpr : kCacheBlock / 4;
-  for (int o = span >> 1; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  // f32 quotients, rounded to nearest: the scale and every q follow from the
-  // definition bit for bit.
-  const __nv_bfloat16 sb =
-      top == INFINITY ? __float2bfloat16_rn(__int_as_float(0x7fc00000)) : __float2bfloat16_rn(__fdiv_rn(top, kTop));
-  const float s = __bfloat162float(sb);
-  int q[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    q[j] = s > 0.0f ? (int)fminf(fmaxf(rintf(__fdiv_rn(x[j], s)), -kTop), kTop) : 0;
-  if constexpr (kFmt == BQ4_CACHE_Q8) {
-    const uint32_t w = (uint32_t)(q[0] + 128) | (uint32_t)(q[1] + 128) << 8 | (uint32_t)(q[2] + 128) << 16 |
-                       (uint32_t)(q[3] + 128) << 24;
-    if (page >= 0) {
-      *reinterpret_cast<uint32_t*>(dst(4 * L)) = w;
-      if (L == 0) r.scales[0] = __bfloat16_as_ushort(sb);
-    }
-  } else {
-    const int blk = L >> 3, g = L & 7;
-    if (kv == 0) {
-      // values o = 4 (L & 1) + j of the word: nibble o / 2 + 4 (o & 1)
-      uint32_t w = (uint32_t)(q[0] + 8) | (uint32_t)(q[1] + 8) << 16 | (uint32_t)(q[2] + 8) << 4 |
-                   (uint32_t)(q[3] + 8) << 20;
-      w <<= 8 * (L & 1);
-      w |= __shfl_xor_sync(0xffffffffu, w, 1);
-      if (page >= 0 && !(L & 1)) *reinterpret_cast<uint32_t*>(dst(4 * ((g >> 1) * a.c.nb + blk))) = w;
-    } else {
-      const uint16_t w = (uint16_t)((q[0] + 8) | (q[1] + 8) << 4 | (q[2] + 8) << 8 | (q[3] + 8) << 12);
-      if (page >= 0) *reinterpret_cast<uint16_t*>(dst(2 * (g * a.c.nb + blk))) = w;
-    }
-    if (page >= 0 && g == 0) r.scales[blk] = __bfloat16_as_ushort(sb);
   }
 }
 
@@ -167,77 +265,118 @@ struct ReadArgs {
   const int32_t* starts;
   void* out[2];
   int64_t stride[3];      // batch, head, position
-  int vec;
-  int count;
-  unsigned rows;          // batch * kv_heads * count
+  int vec;                // every row of out lies on 16 bytes
+  int count, steps;       // steps: the most warps that `count` positions of a head take
+  unsigned items;         // batch * kv_heads * 2 * steps
   int* err;
 };
 
-template <int kFmt, bool kF16>
-__global__ void __launch_bounds__(kCThreads) cache_read_kernel(const ReadArgs a) {
-  const int kv = blockIdx.y;
-  const int lpr = a.c.hp >> 2;
-  const int L = threadIdx.x & (lpr - 1), d0 = 4 * L;
-  const unsigned row = blockIdx.x * (unsigned)(kCThreads / lpr) + threadIdx.x / lpr;
-  if (row >= a.rows || d0 >= a.c.head_dim) return;
-  const unsigned bh = row / (unsigned)a.count;
-  const int i = (int)(row - bh * a.count);
-  const unsigned b = bh / (unsigned)a.c.kv_heads;
-  const int h = (int)(bh - b * a.c.kv_heads);
-  const int64_t pos = (a.starts ? (int64_t)a.starts[b] : 0) + i;
-  float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (pos >= 0 && pos < seq_length(a.s, a.c.page_size, (int)b, a.err)) {
-    const int pi = (int)pos / a.c.page_size;
-    const int page = a.s.table[b * a.s.table_stride + pi];
-    if (page < 0 || page >= a.c.pages) {
-      atomicCAS(a.err, 0, (int)BQ4_EINVAL_ARG);
-    } else {
-      const int place = (int)pos - pi * a.c.page_size;
-      const CacheRow r = cache_row(a.c, page, h, place, kv);
-      auto src = [&](int at) { return r.rows + cache_swizzle(kv, a.c.row_bytes, place, at); };
-      if constexpr (kFmt == BQ4_CACHE_F16) {
-        load4<true>(src(2 * d0), 0, true, x);
-      } else if constexpr (kFmt == BQ4_CACHE_Q8) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(src(4 * L));
-        const float s = __uint_as_float((uint32_t)r.scales[0] << 16);
+template <int kFmt, bool kF16, int kHP>
+__global__ void __launch_bounds__(kCThreads) cache_read_kernel(const __grid_constant__ ReadArgs a) {
+  using T = TakeRead<kF16, kHP>;
+  constexpr int kW = T::kW, kLanes = T::kLanes, kPer = T::kPer, kAhead = T::kRounds, kTake = T::kTake;
+  constexpr int kRow = kFmt == BQ4_CACHE_F16 ? 2 * kHP : kFmt == BQ4_CACHE_Q8 ? kHP : kHP / 2;
+  constexpr int kNb = kFmt == BQ4_CACHE_Q8 ? 1 : kHP / kCacheBlock;
+  constexpr int kHeld = kFmt == BQ4_CACHE_F16 ? 2 * kW : kFmt == BQ4_CACHE_Q8 ? kW : kW / 2;  // bytes of kW values
+  constexpr int kWords = kHeld < 4 ? 1 : kHeld / 4;
+  const int lane = threadIdx.x & 31, L = lane % kLanes, sub = lane / kLanes, d0 = kW * L;
+  unsigned item = (blockIdx.x * kCThreads + threadIdx.x) >> 5;
+  if (item >= a.items) return;
+  const int step = (int)(item % (unsigned)a.steps);
+  item /= (unsigned)a.steps;
+  const int kv = item & 1;
+  item >>= 1;
+  const int b = (int)(item / (unsigned)a.c.kv_heads), head = (int)(item - (unsigned)b * a.c.kv_heads);
+  const int64_t start = a.starts ? (int64_t)a.starts[b] : 0;
+  const int64_t base = (start & ~(int64_t)(kTake - 1)) + kTake * step, to = start + a.count;
+  if (base >= to) return;
+  const int end = seq_length(a.s, a.c.page_size, b, a.err);
+  int place0 = 0, page = -1;
+  if (base >= 0 && base < end) page = page_of(a.c, a.s, b, (int)base, &place0, a.err);
+  const CacheRow r = cache_row(a.c, max(page, 0), head, place0, kv);
+  const int64_t dst = b * a.stride[0] + head * a.stride[1] + (base - start) * a.stride[2] + d0;
+
+  {
+    uint32_t held[kAhead][kWords];
+    uint32_t scale[kAhead];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = (float)((int)(w >> 8 * j & 255) - 128) * s;
-      } else {
-        const int blk = L >> 3, g = L & 7;
-        const float s = __uint_as_float((uint32_t)r.scales[blk] << 16);
-        if (kv == 0) {
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(src(4 * ((g >> 1) * a.c.nb + blk))) >> 8 * (L & 1);
-          x[0] = (float)((int)(w & 15) - 8) * s;
-          x[1] = (float)((int)(w >> 16 & 15) - 8) * s;
-          x[2] = (float)((int)(w >> 4 & 15) - 8) * s;
-          x[3] = (float)((int)(w >> 20 & 15) - 8) * s;
+    for (int j = 0; j < kAhead; ++j) {
+      const int row = j * kPer + sub;
+      const bool live = page >= 0 && base + row < end;
+#pragma unroll
+      for (int e = 0; e < kWords; ++e) held[j][e] = 0;
+      scale[j] = 0;
+      if (live) {
+        auto src = [&](int at) { return r.rows + cache_swizzle(kv, kRow, place0 + row, at); };
+        const uint16_t* sc = r.scales + row * 2 * kNb;
+        if constexpr (kFmt == BQ4_CACHE_F16) {
+          load_words<kHeld>(src(2 * d0), held[j]);
+        } else if constexpr (kFmt == BQ4_CACHE_Q8) {
+          load_words<kHeld>(src(d0), held[j]);
+          scale[j] = sc[0];
         } else {
-          const uint32_t w = *reinterpret_cast<const uint16_t*>(src(2 * (g * a.c.nb + blk)));
+          const int blk = d0 >> 5;
+          scale[j] = sc[blk];
+          if (kv == 0) {
+            load_words<4>(src(4 * (((d0 >> 3) & 3) * kNb + blk)), held[j]);
+          } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = (float)((int)(w >> 4 * j & 15) - 8) * s;
+            for (int e = 0; e < kW; e += 4) {
+              uint32_t w;
+              load_words<2>(src(2 * ((((d0 + e) >> 2) & 7) * kNb + blk)), &w);
+              held[j][0] |= w << 4 * e;
+            }
+          }
         }
       }
     }
-  }
-  const int64_t at = b * a.stride[0] + h * a.stride[1] + i * a.stride[2] + d0;
-  if constexpr (kF16) {
-    __half* o = static_cast<__half*>(a.out[kv]) + at;
-    const __half2 lo = __floats2half2_rn(x[0], x[1]), hi = __floats2half2_rn(x[2], x[3]);
-    if (a.vec) {
-      uint2 u;
-      u.x = *reinterpret_cast<const uint32_t*>(&lo);
-      u.y = *reinterpret_cast<const uint32_t*>(&hi);
-      *reinterpret_cast<uint2*>(o) = u;
-    } else {
-      o[0] = __low2half(lo), o[1] = __high2half(lo), o[2] = __low2half(hi), o[3] = __high2half(hi);
-    }
-  } else {
-    float* o = static_cast<float*>(a.out[kv]) + at;
-    if (a.vec) {
-      *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
-    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = x[j];
+    for (int j = 0; j < kAhead; ++j) {
+      const int row = j * kPer + sub;
+      const float s = __uint_as_float(scale[j] << 16);
+      float x[kW];
+#pragma unroll
+      for (int e = 0; e < kW; ++e) {
+        if constexpr (kFmt == BQ4_CACHE_F16) {
+          x[e] = __half2float(__ushort_as_half((unsigned short)(held[j][e >> 1] >> 16 * (e & 1))));
+        } else if constexpr (kFmt == BQ4_CACHE_Q8) {
+          x[e] = (float)((int)(held[j][e >> 2] >> 8 * (e & 3) & 255) - 128) * s;
+        } else {
+          const int o = kW == 4 ? 4 * (L & 1) + e : e;
+          const int nibble = kv == 0 ? 4 * (o >> 1) + 16 * (o & 1) : 4 * e;
+          x[e] = (float)((int)(held[j][0] >> nibble & 15) - 8) * s;
+        }
+      }
+      const bool live = page >= 0 && base + row < end;
+      if (kFmt != BQ4_CACHE_F16 && !live) {  // the zero words stand for -128 (-8) and a scale of 0: make it +0
+#pragma unroll
+        for (int e = 0; e < kW; ++e) x[e] = 0.0f;
+      }
+      if (base + row < start || base + row >= to || d0 >= a.c.head_dim) continue;
+      const int64_t at = dst + (int64_t)row * a.stride[2];
+      if constexpr (kF16) {
+        uint32_t w[kW / 2];
+#pragma unroll
+        for (int e = 0; e < kW / 2; ++e) {
+          const __half2 h = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+          w[e] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        __half* o = static_cast<__half*>(a.out[kv]) + at;
+        if (a.vec) {
+          store_words<16>(reinterpret_cast<uint8_t*>(o), w);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kW; ++e) o[e] = __ushort_as_half((unsigned short)(w[e >> 1] >> 16 * (e & 1)));
+        }
+      } else {
+        float* o = static_cast<float*>(a.out[kv]) + at;
+        if (a.vec) {
+          *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kW; ++e) o[e] = x[e];
+        }
+      }
     }
   }
 }
@@ -346,23 +485,38 @@ bq4_status device_ready(int device) {
 }
 
 bool strides_vec(const void* base, const int64_t* st, int esize) {
-  return al(base, 4 * esize) && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
+  const int64_t n = 16 / esize;
+  return al(base, 16) && st[0] % n == 0 && st[1] % n == 0 && st[2] % n == 0;
 }
 
 template <int kFmt>
-void launch_append(const AppendArgs& a, bool f16, dim3 grid, cudaStream_t s) {
-  if (f16)
-    cache_append_kernel<kFmt, true><<<grid, kCThreads, 0, s>>>(a);
-  else
-    cache_append_kernel<kFmt, false><<<grid, kCThreads, 0, s>>>(a);
+void launch_append(const AppendArgs& a, bool f16, unsigned grid, cudaStream_t s) {
+  if (a.c.hp == 64) {
+    if (f16)
+      cache_append_kernel<kFmt, true, 64><<<grid, kCThreads, 0, s>>>(a);
+    else
+      cache_append_kernel<kFmt, false, 64><<<grid, kCThreads, 0, s>>>(a);
+  } else {
+    if (f16)
+      cache_append_kernel<kFmt, true, 128><<<grid, kCThreads, 0, s>>>(a);
+    else
+      cache_append_kernel<kFmt, false, 128><<<grid, kCThreads, 0, s>>>(a);
+  }
 }
 
 template <int kFmt>
-void launch_read(const ReadArgs& a, bool f16, dim3 grid, cudaStream_t s) {
-  if (f16)
-    cache_read_kernel<kFmt, true><<<grid, kCThreads, 0, s>>>(a);
-  else
-    cache_read_kernel<kFmt, false><<<grid, kCThreads, 0, s>>>(a);
+void launch_read(const ReadArgs& a, bool f16, unsigned grid, cudaStream_t s) {
+  if (a.c.hp == 64) {
+    if (f16)
+      cache_read_kernel<kFmt, true, 64><<<grid, kCThreads, 0, s>>>(a);
+    else
+      cache_read_kernel<kFmt, false, 64><<<grid, kCThreads, 0, s>>>(a);
+  } else {
+    if (f16)
+      cache_read_kernel<kFmt, true, 128><<<grid, kCThreads, 0, s>>>(a);
+    else
+      cache_read_kernel<kFmt, false, 128><<<grid, kCThreads, 0, s>>>(a);
+  }
 }
 
 // The sizes that both the workspace query and the calls check and plan with.
@@ -487,11 +641,14 @@ bq4_status bq4_cache_append(const bq4_cache* cache, const bq4_cache_sequences* s
   }
   a.vec = strides_vec(k, k_strides, es) && strides_vec(v, v_strides, es);
   a.tokens = (int)tokens;
-  a.rows = (unsigned)rows;
+  const int take = a.c.hp == 64 ? TakeAppend<64>::kTake : TakeAppend<128>::kTake;
+  a.steps = (int)((tokens + 2 * take - 2) / take);
+  if (!row_count(2 * seqs->batch, a.steps, cache->kv_heads, &rows))
+    return set_error(BQ4_EINVAL_SHAPE, "batch * tokens * kv_heads too large for one launch");
+  a.items = (unsigned)rows;
   a.err = device_error_word();
   if (!a.err) return set_error(BQ4_ECUDA, "device error word unavailable");
-  const int per = kCThreads / (a.c.hp / 4);
-  const dim3 grid((unsigned)((rows + per - 1) / per), 2);
+  const unsigned grid = (unsigned)((rows + kCThreads / 32 - 1) / (kCThreads / 32));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (cache->format == BQ4_CACHE_F16)
     launch_append<BQ4_CACHE_F16>(a, es == 2, grid, s);
@@ -532,11 +689,15 @@ bq4_status bq4_cache_read(const bq4_cache* cache, const bq4_cache_sequences* seq
   for (int i = 0; i < 3; ++i) a.stride[i] = strides[i];
   a.vec = strides_vec(k_out, strides, es) && strides_vec(v_out, strides, es);
   a.count = (int)count;
-  a.rows = (unsigned)rows;
+  const int take = es == 2 ? a.c.hp == 64 ? TakeRead<true, 64>::kTake : TakeRead<true, 128>::kTake
+                   : a.c.hp == 64 ? TakeRead<false, 64>::kTake : TakeRead<false, 128>::kTake;
+  a.steps = (int)((count + 2 * take - 2) / take);
+  if (!row_count(2 * seqs->batch, a.steps, cache->kv_heads, &rows))
+    return set_error(BQ4_EINVAL_SHAPE, "batch * count * kv_heads too large for one launch");
+  a.items = (unsigned)rows;
   a.err = device_error_word();
   if (!a.err) return set_error(BQ4_ECUDA, "device error word unavailable");
-  const int per = kCThreads / (a.c.hp / 4);
-  const dim3 grid((unsigned)((rows + per - 1) / per), 2);
+  const unsigned grid = (unsigned)((rows + kCThreads / 32 - 1) / (kCThreads / 32));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (cache->format == BQ4_CACHE_F16)
     launch_read<BQ4_CACHE_F16>(a, es == 2, grid, s);

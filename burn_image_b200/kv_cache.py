@@ -56,6 +56,7 @@ class KVCache:
         self.values = torch.zeros(nv.value, dtype=torch.uint8, device=dev)
         self.scales = torch.zeros(ns.value, dtype=torch.uint8, device=dev)
         c.values, c.scales, c.device = self.values.data_ptr(), self.scales.data_ptr() or None, dev.index
+        self._workspace = {}  # bytes that an attention call of these sizes needs
         self._c = c
         self._ref = ctypes.byref(c)
 
@@ -63,31 +64,39 @@ class KVCache:
     def device_bytes(self) -> int:
         return self.values.numel() + self.scales.numel()
 
+    # The checks below run on every call of a decode loop: they take the common case first and
+    # say what is wrong only when something is.
+
     def _stream(self):
         return torch.cuda.current_stream(self.device).cuda_stream
 
-    def _ints(self, t: torch.Tensor, what: str, dim: int) -> torch.Tensor:
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self.device or t.dim() != dim \
-                or (t.numel() > 1 and t.stride(-1) != 1):
-            raise Bq4Error(L.EINVAL_ARG,
-                           f"{what} must be int32 with {dim} dimension(s) and unit stride on {self.device}")
+    def _sequences(self, page_table: torch.Tensor, lengths: torch.Tensor, batch: Optional[int] = None):
+        if not (page_table.dtype is lengths.dtype is torch.int32 and page_table.device == self.device == lengths.device
+                and page_table.dim() == 2 and lengths.dim() == 1):
+            raise Bq4Error(L.EINVAL_ARG, f"page_table [B, W] and lengths [B] must be int32 on {self.device}")
+        b, w = page_table.shape
+        ts, ws = page_table.stride()
+        n = lengths.shape[0]
+        if (ws != 1 and w > 1) or (n > 1 and lengths.stride(0) != 1):
+            raise Bq4Error(L.EINVAL_ARG, "page_table rows and lengths must have unit stride")
+        if n != b or (batch is not None and batch != b):
+            raise Bq4Error(L.EINVAL_SHAPE, f"page_table holds {b} sequences, lengths {n}"
+                           + (f", the rows {batch}" if batch is not None else ""))
+        return L.CacheSequences(page_table.data_ptr() or None, ts, w, lengths.data_ptr() or None, b)
+
+    def _ints(self, t: torch.Tensor, what: str) -> torch.Tensor:
+        if t.dtype is not torch.int32 or t.device != self.device or t.dim() != 1 \
+                or (t.shape[0] > 1 and t.stride(0) != 1):
+            raise Bq4Error(L.EINVAL_ARG, f"{what} must be int32, one-dimensional and contiguous on {self.device}")
         return t
 
-    def _sequences(self, page_table: torch.Tensor, lengths: torch.Tensor, batch: Optional[int] = None):
-        self._ints(page_table, "page_table", 2)
-        self._ints(lengths, "lengths", 1)
-        b, w = page_table.shape
-        if lengths.shape[0] != b or (batch is not None and batch != b):
-            raise Bq4Error(L.EINVAL_SHAPE, f"page_table holds {b} sequences, lengths {lengths.shape[0]}"
-                           + (f", the rows {batch}" if batch is not None else ""))
-        return L.CacheSequences(page_table.data_ptr() or None, page_table.stride(0), w, lengths.data_ptr() or None, b)
-
     def _rows(self, t: torch.Tensor, what: str, heads: Optional[int]) -> torch.Tensor:
-        if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype not in _DTYPES:
+        if t.dtype not in _DTYPES or t.device != self.device:
             raise Bq4Error(L.EINVAL_ARG, f"{what} must be float32 or float16 on {self.device}")
-        if t.dim() != 4 or t.shape[3] != self.head_dim or (heads is not None and t.shape[2] != heads):
+        shape = t.shape
+        if len(shape) != 4 or shape[3] != self.head_dim or (heads is not None and shape[2] != heads):
             raise Bq4Error(L.EINVAL_SHAPE,
-                           f"{what} must be [B, S, {heads or 'heads'}, {self.head_dim}], got {tuple(t.shape)}")
+                           f"{what} must be [B, S, {heads or 'heads'}, {self.head_dim}], got {tuple(shape)}")
         return t if t.stride(3) == 1 or t.numel() == 0 else t.contiguous()
 
     def append(self, key: torch.Tensor, value: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor) -> None:
@@ -102,10 +111,9 @@ class KVCache:
         if v.shape != k.shape or v.dtype != k.dtype:
             raise Bq4Error(L.EINVAL_SHAPE, "key and value must have one shape and type")
         seqs = self._sequences(page_table, lengths, k.shape[0])
-        ks, vs = k.stride(), v.stride()
-        check(L.lib().bq4_cache_append(self._ref, ctypes.byref(seqs), k.data_ptr() or None,
-                                       _Strides(ks[0], ks[1], ks[2]), v.data_ptr() or None,
-                                       _Strides(vs[0], vs[1], vs[2]), _DTYPES[k.dtype], k.shape[1], self._stream()))
+        check(L.lib().bq4_cache_append(self._ref, ctypes.byref(seqs), k.data_ptr() or None, _Strides(*k.stride()[:3]),
+                                       v.data_ptr() or None, _Strides(*v.stride()[:3]), _DTYPES[k.dtype], k.shape[1],
+                                       self._stream()))
 
     def read(self, page_table: torch.Tensor, lengths: torch.Tensor, count: int,
              starts: Optional[torch.Tensor] = None,
@@ -119,15 +127,14 @@ class KVCache:
             raise Bq4Error(L.EINVAL_ARG, f"rows are read as float16 or float32, not {dtype}")
         if count < 0:
             raise Bq4Error(L.EINVAL_SHAPE, f"count={count}")
-        if starts is not None and self._ints(starts, "starts", 1).shape[0] != seqs.batch:
+        if starts is not None and self._ints(starts, "starts").shape[0] != seqs.batch:
             raise Bq4Error(L.EINVAL_SHAPE, f"starts holds {starts.shape[0]} sequences, page_table {seqs.batch}")
-        shape = (seqs.batch, self.kv_heads, count, self.head_dim)
-        k = torch.empty(shape, dtype=dtype, device=self.device)
-        v = torch.empty(shape, dtype=dtype, device=self.device)
-        st = k.stride()
+        H, D = self.kv_heads, self.head_dim
+        k = page_table.new_empty((seqs.batch, H, count, D), dtype=dtype)
+        v = torch.empty_like(k)
         check(L.lib().bq4_cache_read(self._ref, ctypes.byref(seqs), starts.data_ptr() if starts is not None else None,
-                                     count, k.data_ptr() or None, v.data_ptr() or None, _Strides(st[0], st[1], st[2]),
-                                     _DTYPES[dtype], self._stream()))
+                                     count, k.data_ptr() or None, v.data_ptr() or None,
+                                     _Strides(H * count * D, count * D, D), _DTYPES[dtype], self._stream()))
         return k, v
 
     def attention(self, query: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, causal: bool = True,
@@ -152,8 +159,8 @@ class KVCache:
         list prefix_pages (int32 [W]), read once for the whole batch, and then
         its own sequence; page_table, lengths, causal and max_length are about
         the sequences' own rows."""
-        self._ints(prefix_pages, "prefix_pages", 1)
-        if self._ints(prefix_length, "prefix_length", 1).shape[0] != 1:
+        self._ints(prefix_pages, "prefix_pages")
+        if self._ints(prefix_length, "prefix_length").shape[0] != 1:
             raise Bq4Error(L.EINVAL_SHAPE, "prefix_length must hold one value")
         return self._attention(query, prefix_pages, prefix_length, page_table, lengths, causal, scale, max_length, out)
 
@@ -164,23 +171,27 @@ class KVCache:
         B, S, Hq, D = q.shape
         seqs = self._sequences(page_table, lengths, B)
         if out is None:
-            out = torch.empty((B, S, Hq, D), dtype=torch.float16, device=self.device)
+            out = q.new_empty((B, S, Hq, D))
         elif out.shape != q.shape or out.dtype != torch.float16 or out.device != self.device or not out.is_contiguous():
             raise Bq4Error(L.EINVAL_ARG, f"out must be contiguous float16 {tuple(q.shape)} on {self.device}")
         held = seqs.table_width * self.page_size
         longest = held if max_length is None else max_length
         if longest < 0:
             raise Bq4Error(L.EINVAL_SHAPE, f"max_length={max_length}")
-        lib = L.lib()
-        n = ctypes.c_size_t()
         width = prefix_pages.shape[0] if prefix_pages is not None else 0
-        check(lib.bq4_cache_attention_workspace_size(self._ref, B, S, Hq, min(longest, held) or held,
-                                                     width * self.page_size, ctypes.byref(n)))
+        lib = L.lib()
+        sizes = (B, S, Hq, min(longest, held) or held, width * self.page_size)
+        nbytes = self._workspace.get(sizes)
+        if nbytes is None:
+            n = ctypes.c_size_t()
+            check(lib.bq4_cache_attention_workspace_size(self._ref, *sizes, ctypes.byref(n)))
+            if len(self._workspace) >= 1024:
+                self._workspace.clear()
+            nbytes = self._workspace[sizes] = n.value
         # a workspace of the call's own: calls on several streams, and graphs captured side by side, never share one
-        ws = torch.empty(n.value, dtype=torch.uint8, device=self.device) if n.value else None
-        qs = _Strides(*q.stride()[:3])
-        tail = (q.data_ptr() or None, qs, S, Hq, 1 if causal else 0, float(scale or 0.0), out.data_ptr() or None,
-                ws.data_ptr() if ws is not None else None, n.value, self._stream())
+        ws = q.new_empty(nbytes // 2) if nbytes else None
+        tail = (q.data_ptr() or None, _Strides(*q.stride()[:3]), S, Hq, 1 if causal else 0, scale or 0.0,
+                out.data_ptr() or None, ws.data_ptr() if ws is not None else None, nbytes, self._stream())
         if prefix_pages is None:
             check(lib.bq4_cache_attention(self._ref, ctypes.byref(seqs), longest, *tail))
         else:
