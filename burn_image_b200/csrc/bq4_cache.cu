@@ -13,6 +13,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 
 #include "bq4_cache.h"
@@ -474,6 +475,8 @@ bool row_count(int64_t a, int64_t b, int64_t c, int64_t* rows) {
 }
 
 bq4_status device_ready(int device) {
+  static std::atomic<uint64_t> ready{0};  // a bit for each device found fit before
+  if (device >= 0 && device < 64 && ready.load(std::memory_order_relaxed) >> device & 1) return BQ4_OK;
   int ndev = 0;
   if (cudaGetDeviceCount(&ndev) != cudaSuccess || device < 0 || device >= ndev) {
     cudaGetLastError();
@@ -481,6 +484,7 @@ bq4_status device_ready(int device) {
   }
   if (!device_is_sm100(device))
     return set_error(BQ4_EUNSUPPORTED, "device %d is not sm_100 (B200); libbq4 has no kernels for it", device);
+  if (device < 64) ready.fetch_or(1ull << device, std::memory_order_relaxed);
   return BQ4_OK;
 }
 
