@@ -75,6 +75,31 @@ struct CacheAttnCall {
   int* err;
 };
 
+// Where a row's partial results (m, l and O of some of its keys) lie: the
+// join kernel's input, one of the prefix's and one of the sequence's own keys.
+// Row r of a range (kv head, tile of tile_rows rows) is at slot * tile_rows + r:
+// pieces: slots first CTA + range .. last CTA + range of the split kernel's line;
+// else slots range * chunks .., one for each `span` keys that the tile sees.
+struct CacheJoinSource {
+  const float* part;
+  const float2* ml;
+  const int2* pieces;
+  int tile_rows, tiles, span, chunks, first_range;
+};
+
+// Launch plan of the many-row kernels (bq4_cache_tile.cu) for the prefix or the
+// sequences' own keys.
+struct CacheTilePlan {
+  bool prefix;
+  int sets, tiles, blocks, span, chunks;
+  int64_t records, q_tiles, slots;
+  size_t tile_bytes, consts_bytes, q_bytes, part_bytes, ml_bytes, workspace_bytes;
+};
+bool plan_cache_tile(const CacheAttnCall& a, bool prefix, int sms, CacheTilePlan* p);
+// finish: there is one chunk and no other source, and the rows are finished.
+bq4_status run_cache_tile(const CacheAttnCall& a, const CacheTilePlan& p, bool finish, void* workspace,
+                          CacheJoinSource* source, cudaStream_t stream);
+
 bq4_status cache_attn_workspace(const CacheAttnCall& c, int sms, size_t* bytes);
 bq4_status run_cache_attn(const CacheAttnCall& c, int sms, void* workspace, cudaStream_t s);
 

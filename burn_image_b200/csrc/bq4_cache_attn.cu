@@ -154,6 +154,7 @@ struct SplitArgs {
   int group;             // query heads of a kv head
   int p_tiles, s_tiles;  // row tiles of the prefix and of one sequence
   int q_vec;             // q rows lie on 8-byte boundaries
+  int finish;            // rows of one piece are finished (there is no other source)
   float* part;           // [grid + ranges][8 kNT][hp]: O of piece (CTA + range)
   float2* ml;            // [grid + ranges][8 kNT]: m, l
   int2* pieces;          // [ranges]: first and last CTA with keys of the range
@@ -731,7 +732,7 @@ __global__ void __launch_bounds__(kSThreads, kNT == 1 ? Layout<kFmt, kHP>::kPerS
     }
   __syncthreads();
   const int64_t piece = ((int64_t)blockIdx.x + range) * 8 * kNT;
-  const bool finish = whole && line_p == 0;
+  const bool finish = whole && s.finish && line_p == 0;
   for (int i = threadIdx.x; i < 8 * kNT * (kHP / 4); i += kSThreads) {
     const int r = i / (kHP / 4), d = 4 * (i - r * (kHP / 4));
     if (row0 + r >= rows) break;
@@ -784,47 +785,66 @@ __global__ void __launch_bounds__(kSThreads, kNT == 1 ? Layout<kFmt, kHP>::kPerS
   }
 }
 
-// Joins the pieces of a row, the prefix's and then its own in their order: one
-// warp a row, four values a lane.
-__global__ void __launch_bounds__(kSThreads) cache_join_kernel(const __grid_constant__ SplitArgs s, unsigned rows,
-                                                               int tile_rows) {
-  const CacheAttnCall& a = s.a;
+struct JoinArgs {
+  CacheAttnCall a;
+  CacheJoinSource p, s;  // of the prefix and of the sequences' own keys
+  int group, have_p, finish;
+};
+
+// Slots of row r (of `rows`) of kv head kvh that sees `see` keys: first and number.
+__device__ __forceinline__ int2 slots_of(const JoinArgs& g, const CacheJoinSource& s, int set, int kvh, int r, int rows,
+                                         int keys, bool causal) {
+  const int tile = r / s.tile_rows;
+  if (s.pieces) {
+    const int range = s.first_range + (set * g.a.c.kv_heads + kvh) * s.tiles + tile;
+    if (keys <= 0) return make_int2(0, 0);
+    const int2 cta = s.pieces[range];
+    return make_int2(cta.x + range, cta.y - cta.x + 1);
+  }
+  const int last_i = (min((tile + 1) * s.tile_rows, rows) - 1) / g.group;
+  const int end = max(0, causal ? keys - g.a.tokens + last_i + 1 : keys);
+  const int range = (set * s.tiles + tile) * g.a.c.kv_heads + kvh;
+  return make_int2(range * s.chunks, (((end + 127) / 128) * 128 + s.span - 1) / s.span);
+}
+
+// Joins a row's partial results, the prefix's and then its own in their order:
+// one warp a row, four values a lane.
+__global__ void __launch_bounds__(kSThreads) cache_join_kernel(const __grid_constant__ JoinArgs g, unsigned rows) {
+  const CacheAttnCall& a = g.a;
   const unsigned row = blockIdx.x * kSWarps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, d = 4 * lane;
   ptx::griddep_wait();
   if (row >= rows) return;
   const int bi = (int)(row / (unsigned)a.q_heads), h = (int)row - bi * a.q_heads;
-  const int b = bi / a.tokens, kvh = h / s.group;
-  const int own = (bi - b * a.tokens) * s.group + h - kvh * s.group;  // row among the sequence's
-  const int all = b * a.tokens * s.group + own;                       // among the prefix's
-  const bool have_p = prefix_rows(a) > 0, have_s = own_length(a, b) > 0;
-  int range[2], local[2];
-  int2 cta[2] = {make_int2(0, -1), make_int2(0, -1)};
-  range[0] = kvh * s.p_tiles + all / tile_rows;
-  local[0] = all % tile_rows;
-  range[1] = a.c.kv_heads * s.p_tiles + (b * a.c.kv_heads + kvh) * s.s_tiles + own / tile_rows;
-  local[1] = own % tile_rows;
-  if (have_p) cta[0] = s.pieces[range[0]];
-  if (have_s) cta[1] = s.pieces[range[1]];
-  if (!have_p && have_s && cta[1].x == cta[1].y) return;  // finished by the one piece
-  const int np = cta[0].y - cta[0].x + 1, nc = np + cta[1].y - cta[1].x + 1;
-  auto slot = [&](int i) {
-    return i < np ? ((int64_t)cta[0].x + i + range[0]) * tile_rows + local[0]
-                  : ((int64_t)cta[1].x + (i - np) + range[1]) * tile_rows + local[1];
+  const int b = bi / a.tokens, kvh = h / g.group, per = a.tokens * g.group;
+  const int own = (bi - b * a.tokens) * g.group + h - kvh * g.group;  // row among the sequence's
+  const int all = b * per + own;                                     // among the prefix's
+  int2 sp = make_int2(0, 0);
+  if (g.have_p) sp = slots_of(g, g.p, 0, kvh, all, a.s.batch * per, prefix_rows(a), false);
+  const int2 ss = slots_of(g, g.s, b, kvh, own, per, own_length(a, b), a.causal);
+  if (g.finish && sp.y == 0 && ss.y == 1) return;  // finished by its one piece
+  const int nc = sp.y + ss.y;
+  auto ml = [&](int i) {
+    return i < sp.y ? g.p.ml[((int64_t)sp.x + i) * g.p.tile_rows + all % g.p.tile_rows]
+                    : g.s.ml[((int64_t)ss.x + i - sp.y) * g.s.tile_rows + own % g.s.tile_rows];
+  };
+  auto part = [&](int i) {
+    return (i < sp.y ? g.p.part + (((int64_t)sp.x + i) * g.p.tile_rows + all % g.p.tile_rows) * a.c.hp
+                     : g.s.part + (((int64_t)ss.x + i - sp.y) * g.s.tile_rows + own % g.s.tile_rows) * a.c.hp) + d;
   };
   float top = kNone;
-  for (int i = lane; i < nc; i += 32) top = fmaxf(top, s.ml[slot(i)].x);
+  for (int i = lane; i < nc; i += 32) top = fmaxf(top, ml(i).x);
 #pragma unroll
   for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float lsum = 0.0f;
 #pragma unroll 4
   for (int i = 0; i < nc; ++i) {
-    const float2 e = s.ml[slot(i)];
+    const float2 e = ml(i);
     const float f = ex2(e.x - top);
     lsum += f * e.y;
     if (d < a.c.hp) {
-      const float4 y = *reinterpret_cast<const float4*>(s.part + slot(i) * a.c.hp + d);
+      const float4 y = *reinterpret_cast<const float4*>(part(i));
       sum.x += f * y.x, sum.y += f * y.y, sum.z += f * y.z, sum.w += f * y.w;
     }
   }
@@ -841,7 +861,6 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 struct SplitPlan {
   int nt, p_tiles, s_tiles, grid;
-  int64_t rows;
   size_t part_bytes, ml_bytes, pieces_bytes;
 };
 
@@ -854,7 +873,7 @@ bool plan_split(const CacheAttnCall& a, int sms, SplitPlan* p) {
   p->nt = (prefix > 0 ? all : own) > 8 ? 2 : 1;
   const int tile = 8 * p->nt;
   p->s_tiles = (int)((own + tile - 1) / tile);
-  p->p_tiles = (int)((all + tile - 1) / tile);
+  p->p_tiles = prefix > 0 ? (int)((all + tile - 1) / tile) : 0;
   const int64_t ranges = ((int64_t)p->p_tiles + (int64_t)a.s.batch * p->s_tiles) * a.c.kv_heads;
   const int64_t per = ((int64_t)a.max_length + kUnit - 1) / kUnit, per_p = (prefix + kUnit - 1) / kUnit;
   const int per_sm = p->nt == 2 ? 2 : a.c.format == BQ4_CACHE_F16 && a.c.hp == 128 ? 3 : 4;  // Layout::kPerSm
@@ -862,7 +881,6 @@ bool plan_split(const CacheAttnCall& a, int sms, SplitPlan* p) {
   const int64_t units = std::min(most, per_p * p->p_tiles * a.c.kv_heads) +
                         std::min(most, per * std::min(most, (int64_t)a.s.batch * p->s_tiles * a.c.kv_heads));
   p->grid = (int)std::max<int64_t>(1, std::min(most, units));
-  p->rows = (int64_t)a.s.batch * a.tokens * a.q_heads;
   const int64_t slots = (ranges + p->grid) * tile;
   if (ranges > 0x3fffffff || slots > ((int64_t)1 << 40)) return false;
   p->part_bytes = up256((size_t)slots * a.c.hp * 4);
@@ -902,18 +920,44 @@ cudaError_t launch_head(const SplitArgs& s, int nt, unsigned grid, cudaStream_t 
 
 }  // namespace
 
-bq4_status cache_attn_workspace(const CacheAttnCall& a, int sms, size_t* bytes) {
-  SplitPlan p;
-  if (!plan_split(a, sms, &p))
-    return set_error(BQ4_EINVAL_SHAPE, "cache attention: too many rows for one launch");
-  *bytes = p.part_bytes + p.ml_bytes + p.pieces_bytes;
+namespace {
+
+// Which kernels take the prefix's and the sequences' own keys, and their workspaces.
+struct CachePlan {
+  bool tile_p, tile_s;
+  CacheTilePlan p, s;
+  SplitPlan split;
+  CacheAttnCall call;  // of the split kernel: without a prefix that the tile kernel takes
+  size_t split_bytes, bytes;
+};
+
+// The tile kernels widen a key set once for all its rows and then take 256 rows
+// at a time; the split kernel widens it for every 16 rows.
+bool use_tile(const CacheAttnCall& a, bool prefix, int64_t rows, int64_t keys, int sms, CacheTilePlan* p) {
+  return rows >= 64 && keys >= 256 && plan_cache_tile(a, prefix, sms, p) && p->workspace_bytes <= (size_t)1 << 30;
+}
+
+bq4_status plan_cache(const CacheAttnCall& a, int sms, CachePlan* p) {
+  const int group = a.q_heads / a.c.kv_heads;
+  const int64_t own = (int64_t)a.tokens * group, all = own * a.s.batch;
+  const int64_t prefix = (int64_t)a.prefix_width * a.c.page_size;
+  p->tile_s = use_tile(a, false, own, a.max_length, sms, &p->s);
+  p->tile_p = prefix > 0 && use_tile(a, true, all, prefix, sms, &p->p);
+  if (prefix > 0 && !p->tile_p) p->tile_s = false;  // the split kernel takes both or the sequences' own
+  p->call = a;
+  if (p->tile_p) p->call.prefix_width = 0, p->call.prefix_table = nullptr, p->call.prefix_length = nullptr;
+  p->split_bytes = 0;
+  if (!p->tile_s) {
+    if (!plan_split(p->call, sms, &p->split))
+      return set_error(BQ4_EINVAL_SHAPE, "cache attention: too many rows for one launch");
+    p->split_bytes = p->split.part_bytes + p->split.ml_bytes + p->split.pieces_bytes;
+  }
+  p->bytes = p->split_bytes + (p->tile_s ? p->s.workspace_bytes : 0) + (p->tile_p ? p->p.workspace_bytes : 0);
   return BQ4_OK;
 }
 
-bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, cudaStream_t stream) {
-  SplitPlan p;
-  if (!plan_split(a, sms, &p))
-    return set_error(BQ4_EINVAL_SHAPE, "cache attention: too many rows for one launch");
+bq4_status run_split(const CacheAttnCall& a, const SplitPlan& p, bool finish, void* workspace, CacheJoinSource* prefix,
+                     CacheJoinSource* own, cudaStream_t stream) {
   SplitArgs s;
   s.a = a;
   const uint64_t unit = (uint64_t)(a.c.page_size / kStep);
@@ -925,6 +969,7 @@ bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, cuda
   s.s_tiles = p.s_tiles;
   s.q_vec = reinterpret_cast<uintptr_t>(a.q) % 8 == 0 && a.q_stride[0] % 4 == 0 && a.q_stride[1] % 4 == 0 &&
             a.q_stride[2] % 4 == 0;
+  s.finish = finish;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   s.part = reinterpret_cast<float*>(ws);
   s.ml = reinterpret_cast<float2*>(ws + p.part_bytes);
@@ -934,10 +979,57 @@ bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, cuda
                   : a.c.format == BQ4_CACHE_Q8 ? launch_head<BQ4_CACHE_Q8>(s, p.nt, grid, stream)
                                                : launch_head<BQ4_CACHE_Q4>(s, p.nt, grid, stream);
   note_launch();
-  if (e != cudaSuccess) return check_cuda(e, "cache attention launch");
-  // the join is launched ahead and waits on the device for the pieces
+  own->part = prefix->part = s.part;
+  own->ml = prefix->ml = s.ml;
+  own->pieces = prefix->pieces = s.pieces;
+  own->tile_rows = prefix->tile_rows = 8 * p.nt;
+  prefix->tiles = p.p_tiles;
+  prefix->first_range = 0;
+  own->tiles = p.s_tiles;
+  own->first_range = a.c.kv_heads * p.p_tiles;
+  return check_cuda(e, "cache attention launch");
+}
+
+}  // namespace
+
+bq4_status cache_attn_workspace(const CacheAttnCall& a, int sms, size_t* bytes) {
+  CachePlan p;
+  bq4_status st = plan_cache(a, sms, &p);
+  if (st) return st;
+  *bytes = p.bytes;
+  return BQ4_OK;
+}
+
+bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, cudaStream_t stream) {
+  CachePlan p;
+  bq4_status st = plan_cache(a, sms, &p);
+  if (st) return st;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  JoinArgs g = {};
+  g.a = a;
+  g.group = a.q_heads / a.c.kv_heads;
+  g.have_p = a.prefix_length && a.prefix_width > 0;
+  const bool alone = !p.tile_p;  // the split kernel has every source, or there is one
+  if (p.tile_p) {
+    st = run_cache_tile(a, p.p, false, ws, &g.p, stream);
+    if (st) return st;
+    ws += p.p.workspace_bytes;
+  }
+  if (p.tile_s) {
+    const bool finish = alone && p.s.chunks == 1;
+    st = run_cache_tile(a, p.s, finish, ws, &g.s, stream);
+    if (st || finish) return st;
+  } else {
+    g.finish = alone;
+    CacheJoinSource gp = {};
+    st = run_split(p.call, p.split, alone, ws, &gp, &g.s, stream);
+    if (st) return st;
+    if (alone) g.p = gp;
+  }
+  // the join is launched ahead and waits on the device for the partial results
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.rows + kSWarps - 1) / kSWarps));
+  const unsigned rows = (unsigned)((int64_t)a.s.batch * a.tokens * a.q_heads);
+  cfg.gridDim = dim3((rows + kSWarps - 1) / kSWarps);
   cfg.blockDim = dim3(kSThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -945,7 +1037,7 @@ bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, cuda
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, cache_join_kernel, s, (unsigned)p.rows, 8 * p.nt);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, cache_join_kernel, g, rows);
   note_launch();
   return check_cuda(e, "cache attention join launch");
 }
