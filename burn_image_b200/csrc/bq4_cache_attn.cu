@@ -807,14 +807,19 @@ __device__ __forceinline__ int2 slots_of(const JoinArgs& g, const CacheJoinSourc
   return make_int2(range * s.chunks, (((end + 127) / 128) * 128 + s.span - 1) / s.span);
 }
 
-// Joins a row's partial results, the prefix's and then its own in their order:
-// one warp a row, four values a lane.
+// Joins a row's partial results, the prefix's and then its own in their order.
+// kWarps warps of a CTA take turns at a row's slots (four when the rows are few:
+// what a row takes then is the latency of its loads; 17 slots 16.7 us one load
+// after the other, 4.4 us so), four values a lane and four slots' loads in flight;
+// the first joins what each has.
+template <int kWarps>
 __global__ void __launch_bounds__(kSThreads) cache_join_kernel(const __grid_constant__ JoinArgs g, unsigned rows) {
+  constexpr int kAhead = 4;
   const CacheAttnCall& a = g.a;
-  const unsigned row = blockIdx.x * kSWarps + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, d = 4 * lane;
+  const int warp = (threadIdx.x >> 5) % kWarps, lane = threadIdx.x & 31, d = 4 * lane;
+  const unsigned row = blockIdx.x * (kSWarps / kWarps) + (threadIdx.x >> 5) / kWarps;
   ptx::griddep_wait();
-  if (row >= rows) return;
+  if (row >= rows) return;  // a CTA of four warps a row has one row: all leave
   const int bi = (int)(row / (unsigned)a.q_heads), h = (int)row - bi * a.q_heads;
   const int b = bi / a.tokens, kvh = h / g.group, per = a.tokens * g.group;
   const int own = (bi - b * a.tokens) * g.group + h - kvh * g.group;  // row among the sequence's
@@ -823,28 +828,59 @@ __global__ void __launch_bounds__(kSThreads) cache_join_kernel(const __grid_cons
   if (g.have_p) sp = slots_of(g, g.p, 0, kvh, all, a.s.batch * per, prefix_rows(a), false);
   const int2 ss = slots_of(g, g.s, b, kvh, own, per, own_length(a, b), a.causal);
   if (g.finish && sp.y == 0 && ss.y == 1) return;  // finished by its one piece
-  const int nc = sp.y + ss.y;
-  auto ml = [&](int i) {
-    return i < sp.y ? g.p.ml[((int64_t)sp.x + i) * g.p.tile_rows + all % g.p.tile_rows]
-                    : g.s.ml[((int64_t)ss.x + i - sp.y) * g.s.tile_rows + own % g.s.tile_rows];
-  };
-  auto part = [&](int i) {
-    return (i < sp.y ? g.p.part + (((int64_t)sp.x + i) * g.p.tile_rows + all % g.p.tile_rows) * a.c.hp
-                     : g.s.part + (((int64_t)ss.x + i - sp.y) * g.s.tile_rows + own % g.s.tile_rows) * a.c.hp) + d;
-  };
-  float top = kNone;
-  for (int i = lane; i < nc; i += 32) top = fmaxf(top, ml(i).x);
-#pragma unroll
-  for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+  float top = kNone, lsum = 0.0f;
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float lsum = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < nc; ++i) {
-    const float2 e = ml(i);
-    const float f = ex2(e.x - top);
-    lsum += f * e.y;
-    if (d < a.c.hp) {
-      const float4 y = *reinterpret_cast<const float4*>(part(i));
+  auto take = [&](const CacheJoinSource& s, int2 slots, int local) {
+    const int64_t first = (int64_t)slots.x * s.tile_rows + local;
+    const float2* ml = s.ml + first;
+    const float* part = s.part + first * a.c.hp + d;
+    for (int i = warp; i < slots.y; i += kWarps * kAhead) {
+      float2 e[kAhead];
+      float4 y[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int k = i + u * kWarps;
+        e[u] = make_float2(kNone, 0.0f);
+        y[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (k < slots.y) {
+          e[u] = __ldcg(ml + (int64_t)k * s.tile_rows);
+          if (d < a.c.hp) y[u] = __ldcg(reinterpret_cast<const float4*>(part + (int64_t)k * s.tile_rows * a.c.hp));
+        }
+      }
+      float next = top;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) next = fmaxf(next, e[u].x);
+      const float f = ex2(top - next);
+      top = next;
+      lsum *= f;
+      sum.x *= f, sum.y *= f, sum.z *= f, sum.w *= f;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const float w = ex2(e[u].x - top);
+        lsum += w * e[u].y;
+        sum.x += w * y[u].x, sum.y += w * y[u].y, sum.z += w * y[u].z, sum.w += w * y[u].w;
+      }
+    }
+  };
+  if (sp.y) take(g.p, sp, all % g.p.tile_rows);
+  take(g.s, ss, own % g.s.tile_rows);
+  if constexpr (kWarps > 1) {
+    __shared__ float4 sums[kWarps][32];
+    __shared__ float2 mls[kWarps];
+    sums[warp][lane] = sum;
+    if (lane == 0) mls[warp] = make_float2(top, lsum);
+    __syncthreads();
+    if (warp) return;
+    top = kNone;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, mls[w].x);
+    lsum = 0.0f;
+    sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = ex2(mls[w].x - top);
+      const float4 y = sums[w][lane];
+      lsum += f * mls[w].y;
       sum.x += f * y.x, sum.y += f * y.y, sum.z += f * y.z, sum.w += f * y.w;
     }
   }
@@ -1029,7 +1065,8 @@ bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, cuda
   // the join is launched ahead and waits on the device for the partial results
   cudaLaunchConfig_t cfg = {};
   const unsigned rows = (unsigned)((int64_t)a.s.batch * a.tokens * a.q_heads);
-  cfg.gridDim = dim3((rows + kSWarps - 1) / kSWarps);
+  const bool few = rows <= 1024;
+  cfg.gridDim = dim3(few ? rows : (rows + kSWarps - 1) / kSWarps);
   cfg.blockDim = dim3(kSThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -1037,7 +1074,7 @@ bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, cuda
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, cache_join_kernel, g, rows);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, few ? cache_join_kernel<kSWarps> : cache_join_kernel<1>, g, rows);
   note_launch();
   return check_cuda(e, "cache attention join launch");
 }
