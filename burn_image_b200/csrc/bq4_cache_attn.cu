@@ -36,12 +36,13 @@
 //     its low bits (taking it out in every step, by a product with A = -128
 //     2^-24, left values of q = 0 up to 2^-17 of the offset away from 0).
 //   * k scales multiply the f32 scores.  v scales multiply the probabilities,
-//     over a running power of two that is at least the largest of them, so
-//     that the f16 rounding of p s_v is a relative one (2^-11; the only
-//     rounding to fewer than 32 bits besides the result's).
-//   * m only moves when a score passes it by 2^14 (a vote, no shuffles in the
-//     common step): p <= 2^14 fits f16, and m starts 2^6 below the first
-//     maximum so that small probabilities keep f16's range below them.
+//     p s_v as f16 (off by 2^-11 of it; the only rounding to fewer than 32 bits
+//     besides the result's).  To keep it in f16's range p is 2^(x - base), base
+//     being the running maximum of x plus log2 of a power of two above the v
+//     scales so far, less 6; l and O are both relative to base.
+//   * base only moves when some p s_v could pass 2^14 (a vote, no shuffles in
+//     the common step), and then 2^8 down at least.
+//   * Steps that every row sees whole run without any mask.
 //
 // What bounds it: HBM for a few rows (each byte of the chunk is read once),
 // instruction issue for 4-bit caches, the tensor core's legacy path when the
@@ -51,6 +52,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "bq4_cache.h"
 #include "sm100_ptx.cuh"
@@ -63,7 +65,7 @@ constexpr int kSThreads = 32 * kSWarps;
 constexpr int kStep = 16;                     // keys of a warp's step
 constexpr int kUnit = kStep * kSWarps;        // one step a warp
 constexpr float kNone = -1e30f;               // the maximum of no score (finite: differences stay defined)
-constexpr float kHead = 6.0f, kJump = 14.0f;  // log2 units; see above
+constexpr float kHead = 6.0f, kJump = 14.0f;  // log2 units: where base leaves p s_v, and where it moves
 
 // kWords 32-bit words from shared memory.
 template <int kWords>
@@ -111,6 +113,12 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// CTAs of the split kernel that an SM holds.
+constexpr int split_per_sm(int format, int hp, int nt) {
+  if (nt == 2) return hp == 64 ? 3 : 2;
+  return format == BQ4_CACHE_F16 && hp == 128 ? 3 : 4;
+}
+
 // Sizes that follow from the format and the padded head.
 template <int kFmt, int kHP>
 struct Layout {
@@ -130,10 +138,10 @@ struct Layout {
   static constexpr int kOffV = kStep * kRow;
   static constexpr int kOffS = 2 * kStep * kRow;
   static constexpr int kStage = kOffS + kStep * kScale;
-  // CTAs of an SM with 8 rows a warp, by registers and by the ring (two with 16 rows, by registers)
-  static constexpr int kPerSm = kFmt == BQ4_CACHE_F16 && kHP == 128 ? 3 : 4;
-  static constexpr int kStages = (kPerSm == 3 ? 72 : 54) * 1024 / (kSWarps * kStage) < 8
-                                     ? (kPerSm == 3 ? 72 : 54) * 1024 / (kSWarps * kStage) : 8;
+  // CTAs of an SM, by registers (512 threads of 128) and by the ring
+  static constexpr int per_sm(int nt) { return split_per_sm(kFmt, kHP, nt); }
+  static constexpr int kRing = (per_sm(1) == 3 ? 72 : 54) * 1024;  // bytes, about
+  static constexpr int kStages = kRing / (kSWarps * kStage) < 8 ? kRing / (kSWarps * kStage) : 8;
   // value d of the head that element e (0..3) of k step ks holds in lane t: at + e
   __device__ static int qd(int ks, int t) {
     return kFmt == BQ4_CACHE_Q8 ? 64 * (ks >> 2) + 16 * t + 4 * (ks & 3) : 32 * (ks >> 1) + 8 * t + 4 * (ks & 1);
@@ -194,38 +202,38 @@ __device__ __forceinline__ int prefix_rows(const CacheAttnCall& a) {
 }
 
 template <int kFmt, int kHP, int kNT>
-__global__ void __launch_bounds__(kSThreads, kNT == 1 ? Layout<kFmt, kHP>::kPerSm : 2)
+__global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
     cache_split_kernel(const __grid_constant__ SplitArgs s) {
   using Y = Layout<kFmt, kHP>;
   extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ unsigned before[kSThreads + 1];
+  __shared__ unsigned warp_sum[kSWarps];
+  __shared__ __align__(8) uint64_t bars[kSWarps * Y::kStages];
+  __shared__ int abort_flag;
   const CacheAttnCall& a = s.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   ptx::griddep_launch_dependents();
-
-  // ---- the line: units before each sequence (a thread adds up `per` of them)
-  __shared__ int64_t before[kSThreads + 1];
-  __shared__ int64_t warp_sum[kSWarps];
-  __shared__ __align__(8) uint64_t bars[kSWarps * Y::kStages];
-  __shared__ int abort_flag;
   if (threadIdx.x < kSWarps * Y::kStages) ptx::mbar_init(&bars[threadIdx.x], 1);
   if (threadIdx.x == 0) abort_flag = 0;
   ptx::fence_mbar_init();
+
+  // ---- the line: units before each sequence (a thread adds up `per` of them; the host
+  // bounds the line by 2^31)
   const int n_prefix = prefix_rows(a);
-  const int per_p = (n_prefix + kUnit - 1) / kUnit;
-  const int64_t line_p = (int64_t)per_p * a.c.kv_heads * s.p_tiles;
-  const int heads_tiles = a.c.kv_heads * s.s_tiles;
+  const unsigned per_p = (unsigned)(n_prefix + kUnit - 1) / kUnit;
+  const unsigned line_p = per_p * (unsigned)(a.c.kv_heads * s.p_tiles);
+  const unsigned heads_tiles = (unsigned)(a.c.kv_heads * s.s_tiles);
   const int per = (a.s.batch + kSThreads - 1) / kSThreads;
   {
-    int64_t mine = 0;
+    unsigned sum = 0;
     for (int i = 0; i < per; ++i) {
       const int sb = (int)threadIdx.x * per + i;
-      if (sb < a.s.batch) mine += (own_length(a, sb) + kUnit - 1) / kUnit;
+      if (sb < a.s.batch) sum += (unsigned)(own_length(a, sb) + kUnit - 1) / kUnit;
     }
-    mine *= heads_tiles;
-    int64_t sum = mine;
+    sum *= heads_tiles;
 #pragma unroll
     for (int w = 1; w < 32; w <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, sum, w);
+      const unsigned y = __shfl_up_sync(0xffffffffu, sum, w);
       if (lane >= w) sum += y;
     }
     if (lane == 31) warp_sum[warp] = sum;
@@ -235,20 +243,20 @@ __global__ void __launch_bounds__(kSThreads, kNT == 1 ? Layout<kFmt, kHP>::kPerS
     if (threadIdx.x == 0) before[0] = line_p;
     __syncthreads();
   }
-  const int64_t line = before[kSThreads], share = (line + gridDim.x - 1) / gridDim.x;
-  int64_t at_unit = blockIdx.x * share;
-  const int64_t to_unit = min(line, at_unit + share);
+  const unsigned line = before[kSThreads], share = (line + gridDim.x - 1) / gridDim.x;
+  unsigned at_unit = blockIdx.x * share;  // below line + share
+  const unsigned to_unit = min(line, at_unit + share);
   if (at_unit >= to_unit) return;
 
   // ---- the range that holds at_unit
   bool prefix = at_unit < line_p;
-  int b = 0, tile, kvh, n, units;
-  int64_t first;  // of the range, along the line
+  int b = 0, tile, kvh, n;
+  unsigned units, first;  // of the range, along the line
   if (prefix) {
     const int r = (int)(at_unit / per_p);
     tile = r % s.p_tiles;
     kvh = r / s.p_tiles;
-    first = (int64_t)r * per_p;
+    first = (unsigned)r * per_p;
     n = n_prefix;
     units = per_p;
   } else {
@@ -261,17 +269,17 @@ __global__ void __launch_bounds__(kSThreads, kNT == 1 ? Layout<kFmt, kHP>::kPerS
     b = lo * per;
     for (;; ++b) {
       n = own_length(a, b);
-      units = (n + kUnit - 1) / kUnit;
-      if (at_unit < first + (int64_t)units * heads_tiles) break;
-      first += (int64_t)units * heads_tiles;
+      units = (unsigned)(n + kUnit - 1) / kUnit;
+      if (at_unit < first + units * heads_tiles) break;
+      first += units * heads_tiles;
     }
     const int r = (int)((at_unit - first) / units);
     tile = r % s.s_tiles;
     kvh = r / s.s_tiles;
-    first += (int64_t)r * units;
+    first += (unsigned)r * units;
   }
 
-  // this warp's ring: stages filled and taken so far, as slot and parity
+  // this warp's ring: the stages to fill and to take next, and the parity of the latter
   const uint32_t ring = ptx::smem_u32(smem) + warp * Y::kStages * Y::kStage;
   uint64_t* full = bars + warp * Y::kStages;
   int put = 0, get = 0;
@@ -282,506 +290,502 @@ __global__ void __launch_bounds__(kSThreads, kNT == 1 ? Layout<kFmt, kHP>::kPerS
   const uint32_t v_at1 = Y::kOffV + cache_swizzle(1, Y::kRow, 2 * t + 1, g * Y::kVPiece);
 
   for (;;) {  // a piece a turn
-  const int range = prefix ? kvh * s.p_tiles + tile
-                           : a.c.kv_heads * s.p_tiles + (b * a.c.kv_heads + kvh) * s.s_tiles + tile;
-  const int64_t piece_to = min(to_unit, first + units);
-  const int key0 = (int)(at_unit - first) * kUnit;
-  const int rows = (prefix ? a.s.batch : 1) * a.tokens * s.group;
-  const int row0 = tile * 8 * kNT;
-  const bool causal = !prefix && a.causal;
-  // the keys that the tile's last row sees
-  const int last_i = (min(row0 + 8 * kNT, rows) - 1) / s.group;
-  const int end = min(min(n, (int)(piece_to - first) * kUnit), causal ? n - a.tokens + last_i + 1 : n);
-  const bool whole = at_unit == first && piece_to == first + units;
-  if (at_unit == first && threadIdx.x == 0)
-    s.pieces[range] = make_int2((int)blockIdx.x, (int)((first + units - 1) / share));
-  const int32_t* table = prefix ? a.prefix_table : a.s.table + b * a.s.table_stride;
+    const int range = prefix ? kvh * s.p_tiles + tile
+                             : a.c.kv_heads * s.p_tiles + (b * a.c.kv_heads + kvh) * s.s_tiles + tile;
+    const unsigned piece_to = min(to_unit, first + units);
+    const int key0 = (int)(at_unit - first) * kUnit;
+    const int rows = (prefix ? a.s.batch : 1) * a.tokens * s.group;
+    const int row0 = tile * 8 * kNT;
+    const bool causal = !prefix && a.causal;
+    // the keys that the tile's last row sees
+    const int last_i = (min(row0 + 8 * kNT, rows) - 1) / s.group;
+    const int end = min(min(n, (int)(piece_to - first) * kUnit), causal ? n - a.tokens + last_i + 1 : n);
+    const bool whole = at_unit == first && piece_to == first + units;
+    if (at_unit == first && threadIdx.x == 0)
+      s.pieces[range] = make_int2((int)blockIdx.x, (int)((first + units - 1) / share));
+    const int32_t* table = prefix ? a.prefix_table : a.s.table + b * a.s.table_stride;
 
-  // ---- pages of this warp's steps: lane j % 32 holds step j's, of the 32 steps fetched last
-  const int steps = end <= key0 ? 0 : (end - key0 + kStep - 1) / kStep;
-  const int mine = steps > warp ? (steps - warp + kSWarps - 1) / kSWarps : 0;
-  int page = 0, place = 0;
-  unsigned held = 0, held_before = 0;  // bit j % 32: step j's page exists; of the 32 steps before them
-
-  // ---- bulk copies of step j into the ring
-  const int64_t head_at = (int64_t)kvh * 2 * a.c.kv_bytes;
-  auto fetch = [&](int j) {
-    if (j >= mine) return;
-    if ((j & 31) == 0) {
-      bool ok = false;
+    // ---- steps of this warp; lane j % 32 knows where step j lies, for the 32 steps fetched last
+    const int steps = end <= key0 ? 0 : (end - key0 + kStep - 1) / kStep;
+    const int mine = steps > warp ? (steps - warp + kSWarps - 1) / kSWarps : 0;
+    const int at0 = key0 + warp * kStep;  // first key of step 0; step j lies kUnit j on
+    const uint8_t* k_src = nullptr;
+    const uint8_t* s_src = nullptr;
+    unsigned held = 0, held_before = 0;   // bit j % 32: step j's page exists; of the 32 steps before them
+    int plain = mine;                     // steps below it have a page and no mask
+    auto locate = [&](int j) {
+      bool ok = true;
       if (j + lane < mine) {
-        const unsigned u = (unsigned)(key0 / kStep) + (unsigned)(warp + kSWarps * (j + lane));
+        const unsigned u = (unsigned)(at0 / kStep + kSWarps * (j + lane));
         const int pi = (int)((u * s.page_magic) >> 38);
-        page = table[pi];
-        place = (int)u * kStep - pi * a.c.page_size;
+        int page = table[pi];
+        const int place = (int)u * kStep - pi * a.c.page_size;
         ok = page >= 0 && page < a.c.pages;
-        if (!ok) atomicCAS(a.err, 0, (int)BQ4_EINVAL_ARG);
+        if (!ok) {
+          atomicCAS(a.err, 0, (int)BQ4_EINVAL_ARG);
+          page = 0;
+        }
+        const int64_t ph = (int64_t)page * a.c.kv_heads + kvh;
+        k_src = a.c.values + ph * 2 * a.c.kv_bytes + place * Y::kRow;
+        if constexpr (Y::kQ)
+          s_src = reinterpret_cast<const uint8_t*>(a.c.scales) + (ph * a.c.page_size + place) * Y::kScale;
       }
       held_before = held;
       held = __ballot_sync(0xffffffffu, ok);
-    }
-    if (!(held >> (j & 31) & 1)) return;
-    const int pg = __shfl_sync(0xffffffffu, page, j & 31), pl = __shfl_sync(0xffffffffu, place, j & 31);
-    if (lane == 0) {
-      const uint8_t* k = a.c.values + (int64_t)pg * s.page_stride + head_at + pl * Y::kRow;
-      uint8_t* st = smem + (warp * Y::kStages + put) * Y::kStage;
-      ptx::mbar_arrive_expect_tx(&full[put], Y::kStage);
-      ptx::bulk_load(st, k, kStep * Y::kRow, &full[put]);
-      ptx::bulk_load(st + Y::kOffV, k + a.c.kv_bytes, kStep * Y::kRow, &full[put]);
-      if constexpr (Y::kQ)
-        ptx::bulk_load(st + Y::kOffS,
-                       reinterpret_cast<const uint8_t*>(a.c.scales) +
-                           (((int64_t)pg * a.c.kv_heads + kvh) * a.c.page_size + pl) * Y::kScale,
-                       kStep * Y::kScale, &full[put]);
-    }
-    put = put + 1 == Y::kStages ? 0 : put + 1;
-  };
-  for (int j = 0; j < Y::kStages - 1; ++j) fetch(j);
+      if (held != 0xffffffffu) plain = min(plain, j);
+    };
+    // three bulk copies bring step j, by the lane that knows it (of a step without a page, page
+    // 0's rows: they are masked)
+    auto fetch = [&](int j) {
+      if (j >= mine) return;
+      if ((j & 31) == 0) locate(j);
+      if (lane == (j & 31)) {
+        uint8_t* st = smem + (warp * Y::kStages + put) * Y::kStage;
+        ptx::mbar_arrive_expect_tx(&full[put], Y::kStage);
+        ptx::bulk_load(st, k_src, kStep * Y::kRow, &full[put]);
+        ptx::bulk_load(st + Y::kOffV, k_src + a.c.kv_bytes, kStep * Y::kRow, &full[put]);
+        if constexpr (Y::kQ) ptx::bulk_load(st + Y::kOffS, s_src, kStep * Y::kScale, &full[put]);
+      }
+      put = put + 1 == Y::kStages ? 0 : put + 1;
+    };
+    for (int j = 0; j < Y::kStages - 1; ++j) fetch(j);
 
-  // ---- q fragments; the offset's start values; what each row sees
-  uint32_t q[kNT][Y::kKS][2];
-  constexpr int kOffs = kFmt == BQ4_CACHE_Q4 ? Y::kNb : 1;  // start values of a row
-  float off[kNT][kOffs][2];
-  int see[kNT][2];
-  int see_all = 0x7fffffff;
+    // ---- q fragments; the offset's start values; what each row sees
+    uint32_t q[kNT][Y::kKS][2];
+    constexpr int kOffs = kFmt == BQ4_CACHE_Q4 ? Y::kNb : 1;  // start values of a row
+    float off[kNT][kOffs][2];
+    int see[kNT][2];
+    int see_all = 0x7fffffff;
 #pragma unroll
-  for (int nt = 0; nt < kNT; ++nt) {
-    const int r = row0 + 8 * nt + g;
-    const Row w = row_of(s, prefix, b, kvh, min(r, rows - 1));
-    const __half* p = reinterpret_cast<const __half*>(a.q) + w.b * a.q_stride[0] + w.i * a.q_stride[1] +
-                      w.h * a.q_stride[2];
+    for (int nt = 0; nt < kNT; ++nt) {
+      const int r = row0 + 8 * nt + g;
+      const Row w = row_of(s, prefix, b, kvh, min(r, rows - 1));
+      const __half* p = reinterpret_cast<const __half*>(a.q) + w.b * a.q_stride[0] + w.i * a.q_stride[1] +
+                        w.h * a.q_stride[2];
 #pragma unroll
-    for (int ks = 0; ks < Y::kKS; ++ks) {
-      const int d = Y::qd(ks, t);
-      uint2 u = make_uint2(0, 0);
-      if (r < rows && d < a.c.head_dim) {
-        if (s.q_vec) {
-          u = *reinterpret_cast<const uint2*>(p + d);
-        } else {
-          const unsigned short* e = reinterpret_cast<const unsigned short*>(p + d);
-          u = make_uint2(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16);
+      for (int ks = 0; ks < Y::kKS; ++ks) {
+        const int d = Y::qd(ks, t);
+        uint2 u = make_uint2(0, 0);
+        if (r < rows && d < a.c.head_dim) {
+          if (s.q_vec) {
+            u = *reinterpret_cast<const uint2*>(p + d);
+          } else {
+            const unsigned short* e = reinterpret_cast<const unsigned short*>(p + d);
+            u = make_uint2(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16);
+          }
+        }
+        q[nt][ks][0] = u.x;
+        q[nt][ks][1] = u.y;
+      }
+      if constexpr (Y::kQ) {
+#pragma unroll
+        for (int o = 0; o < kOffs; ++o) {
+          float sum = 0.0f;
+#pragma unroll
+          for (int ks = o * Y::kKS / kOffs; ks < (o + 1) * Y::kKS / kOffs; ++ks)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q[nt][ks][e]));
+              sum += f.x + f.y;
+            }
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);  // of row g, in all its lanes
+          constexpr float kZero = kFmt == BQ4_CACHE_Q8 ? -128.0f : -8.0f;
+          off[nt][o][0] = __shfl_sync(0xffffffffu, sum, 8 * t) * (kZero * 0x1p-24f);
+          off[nt][o][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4) * (kZero * 0x1p-24f);
+        }
+      } else {
+        off[nt][0][0] = off[nt][0][1] = 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int rr = row0 + 8 * nt + 2 * t + e;
+        see[nt][e] = !causal ? end : rr < rows ? min(end, n - a.tokens + rr / s.group + 1) : end;
+        see_all = min(see_all, see[nt][e]);
+      }
+    }
+    // the keys that every row of the tile sees (the same for the whole warp)
+    see_all = min(see_all, __shfl_xor_sync(0xffffffffu, see_all, 1));
+    see_all = min(see_all, __shfl_xor_sync(0xffffffffu, see_all, 2));
+    plain = min(plain, max(0, (see_all - at0 + kUnit - kStep) / kUnit));
+
+    // p = 2^(x - base): with vs a power of two above the v scales so far and m the maximum of x so
+    // far, base = m + log2(vs) - kHead when it moves, so that p s_v stays below 2^kJump.  l and O
+    // are both relative to it.
+    float base[kNT][2], l[kNT][2], o[kNT][Y::kMT][4];
+    float vs = Y::kQ ? 0x1p-100f : 1.0f, jump = Y::kQ ? kJump + 100.0f : kJump;  // jump = kJump - log2(vs)
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      base[nt][0] = base[nt][1] = kNone;
+      l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+      for (int mt = 0; mt < Y::kMT; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.0f;
+    }
+    const float c = Y::kQ ? s.c * 0x1p24f : s.c;
+
+    // One step: false when its rows did not come.  kEdge: some row does not see some key, or
+    // the step has no page.
+    auto step = [&](auto edge_tag, int j) -> bool {
+      constexpr bool kEdge = decltype(edge_tag)::value;
+      __syncwarp();  // the slot that is filled next has been read by every lane
+      fetch(j + Y::kStages - 1);
+      const int at = at0 + kUnit * j;
+      const uint32_t st = ring + get * Y::kStage;
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(&full[get], parity, &abort_flag))) return false;
+      if (++get == Y::kStages) get = 0, parity ^= 1;
+      int limit[kNT][2];  // keys of this step that a row sees, less this lane's g
+      if constexpr (kEdge) {
+        // the fetches are kStages - 1 steps ahead, perhaps among the next 32 already
+        const bool next = (min(j + Y::kStages - 1, mine - 1) >> 5) != (j >> 5);
+        const bool none = !((next ? held_before : held) >> (j & 31) & 1);
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) limit[nt][e] = none ? -16 : see[nt][e] - at - g;
+      }
+
+      // ---- scales of keys g, g + 8
+      float sk[2][Y::kQ ? Y::kNb : 1], sv[2][Y::kQ ? Y::kNb : 1];
+      if constexpr (Y::kQ) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          uint32_t w[Y::kNb];
+          lds(st + Y::kOffS + (g + 8 * r) * Y::kScale, w);
+          if constexpr (kFmt == BQ4_CACHE_Q8) {
+            sk[r][0] = __uint_as_float(w[0] << 16);
+            sv[r][0] = __uint_as_float(w[0] & 0xffff0000u);
+          } else {
+#pragma unroll
+            for (int e = 0; e < Y::kNb; ++e) {
+              const uint32_t kw = w[e >> 1], vw = w[(Y::kNb + e) >> 1];
+              sk[r][e] = __uint_as_float(e & 1 ? kw & 0xffff0000u : kw << 16);
+              sv[r][e] = __uint_as_float(e & 1 ? vw & 0xffff0000u : vw << 16);
+            }
+          }
+          if constexpr (kEdge) {  // rows behind the end hold anything
+            if (at + g + 8 * r >= end)
+#pragma unroll
+              for (int e = 0; e < Y::kNb; ++e) sv[r][e] = 0.0f;
+          }
         }
       }
-      q[nt][ks][0] = u.x;
-      q[nt][ks][1] = u.y;
-    }
-    if constexpr (Y::kQ) {
+
+      // ---- scores of keys g (0, 1) and g + 8 (2, 3) with rows 2t, 2t + 1
+      float x[kNT][4];
 #pragma unroll
-      for (int o = 0; o < kOffs; ++o) {
-        float sum = 0.0f;
+      for (int nt = 0; nt < kNT; ++nt) {
+        x[nt][0] = x[nt][2] = kFmt == BQ4_CACHE_Q4 ? 0.0f : off[nt][0][0];
+        x[nt][1] = x[nt][3] = kFmt == BQ4_CACHE_Q4 ? 0.0f : off[nt][0][1];
+      }
 #pragma unroll
-        for (int ks = o * Y::kKS / kOffs; ks < (o + 1) * Y::kKS / kOffs; ++ks)
+      for (int p = 0; p < Y::kKPieces; ++p) {
+        uint32_t w0[Y::kKPiece / 4], w1[Y::kKPiece / 4];
+        const uint32_t from = st + (k_at ^ p << 6);  // 4 pieces of 16 bytes on; the swizzle is in bit 6
+        lds(from, w0);
+        lds(from + 8 * Y::kRow, w1);
+        if constexpr (kFmt == BQ4_CACHE_F16) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q[nt][ks][e]));
-            sum += f.x + f.y;
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt)
+              mma16816(x[nt], w0[2 * h], w1[2 * h], w0[2 * h + 1], w1[2 * h + 1], q[nt][2 * p + h][0],
+                       q[nt][2 * p + h][1]);
+        } else if constexpr (kFmt == BQ4_CACHE_Q8) {
+#pragma unroll
+          for (int e = 0; e < Y::kKPiece / 4; ++e) {
+            const uint32_t a0 = __byte_perm(w0[e], 0, 0x4140), a2 = __byte_perm(w0[e], 0, 0x4342);
+            const uint32_t a1 = __byte_perm(w1[e], 0, 0x4140), a3 = __byte_perm(w1[e], 0, 0x4342);
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt)
+              mma16816(x[nt], a0, a1, a2, a3, q[nt][4 * p + e][0], q[nt][4 * p + e][1]);
           }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);  // of row g, in all its lanes
-        constexpr float kZero = kFmt == BQ4_CACHE_Q8 ? -128.0f : -8.0f;
-        off[nt][o][0] = __shfl_sync(0xffffffffu, sum, 8 * t) * (kZero * 0x1p-24f);
-        off[nt][o][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4) * (kZero * 0x1p-24f);
-      }
-    } else {
-      off[nt][0][0] = off[nt][0][1] = 0.0f;
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int rr = row0 + 8 * nt + 2 * t + e;
-      see[nt][e] = !causal ? end : rr < rows ? min(end, n - a.tokens + rr / s.group + 1) : end;
-      see_all = min(see_all, see[nt][e]);
-    }
-  }
-  // the keys that every row of the tile sees (the same for the whole warp)
-  see_all = min(see_all, __shfl_xor_sync(0xffffffffu, see_all, 1));
-  see_all = min(see_all, __shfl_xor_sync(0xffffffffu, see_all, 2));
-
-  float m[kNT][2], l[kNT][2], o[kNT][Y::kMT][4];
-  float vs = 0.0f, inv_vs = 0.0f;  // power of two above the v scales so far
-#pragma unroll
-  for (int nt = 0; nt < kNT; ++nt) {
-    m[nt][0] = m[nt][1] = kNone;
-    l[nt][0] = l[nt][1] = 0.0f;
-#pragma unroll
-    for (int mt = 0; mt < Y::kMT; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.0f;
-  }
-  const float c = Y::kQ ? s.c * 0x1p24f : s.c;
-
-  for (int j = 0; j < mine; ++j) {
-    __syncwarp();  // the slot that is filled next has been read by every lane
-    fetch(j + Y::kStages - 1);
-    const int at = key0 + (warp + kSWarps * j) * kStep;
-    {
-      // the fetches are kStages - 1 steps ahead, perhaps among the next 32 already
-      const bool next = (min(j + Y::kStages - 1, mine - 1) >> 5) != (j >> 5);
-      if (!((next ? held_before : held) >> (j & 31) & 1)) continue;  // a bad page holds nothing
-    }
-    const uint32_t st = ring + get * Y::kStage;
-    if (!__all_sync(0xffffffffu, ptx::mbar_wait(&full[get], parity, &abort_flag))) {
-      if (lane == 0) {
-        abort_flag = 1;
-        atomicCAS(a.err, 0, (int)BQ4_ETIMEOUT);
-      }
-      break;
-    }
-    if (++get == Y::kStages) get = 0, parity ^= 1;
-
-    // ---- scales of keys g, g + 8
-    float sk[2][Y::kQ ? Y::kNb : 1], sv[2][Y::kQ ? Y::kNb : 1];
-    if constexpr (Y::kQ) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        uint32_t w[Y::kNb];
-        lds(st + Y::kOffS + (g + 8 * r) * Y::kScale, w);
-        if constexpr (kFmt == BQ4_CACHE_Q8) {
-          sk[r][0] = __uint_as_float(w[0] << 16);
-          sv[r][0] = __uint_as_float(w[0] & 0xffff0000u);
         } else {
 #pragma unroll
           for (int e = 0; e < Y::kNb; ++e) {
-            const uint32_t kw = w[e >> 1], vw = w[(Y::kNb + e) >> 1];
-            sk[r][e] = __uint_as_float(e & 1 ? kw & 0xffff0000u : kw << 16);
-            sv[r][e] = __uint_as_float(e & 1 ? vw & 0xffff0000u : vw << 16);
-          }
-        }
-      }
-    }
-
-    // ---- scores x of keys g (c0, c1) and g + 8 (c2, c3) with rows 2t, 2t + 1
-    float x[kNT][4];
+            float y[kNT][4];
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-      x[nt][0] = x[nt][2] = kFmt == BQ4_CACHE_Q4 ? 0.0f : off[nt][0][0];
-      x[nt][1] = x[nt][3] = kFmt == BQ4_CACHE_Q4 ? 0.0f : off[nt][0][1];
-    }
+            for (int nt = 0; nt < kNT; ++nt) {
+              y[nt][0] = y[nt][2] = off[nt][e][0];
+              y[nt][1] = y[nt][3] = off[nt][e][1];
+            }
+            constexpr uint32_t kPair = 0x000F000Fu;
 #pragma unroll
-    for (int p = 0; p < Y::kKPieces; ++p) {
-      uint32_t w0[Y::kKPiece / 4], w1[Y::kKPiece / 4];
-      const uint32_t from = st + (k_at ^ p << 6);  // 4 pieces of 16 bytes on; the swizzle is in bit 6
-      lds(from, w0);
-      lds(from + 8 * Y::kRow, w1);
-      if constexpr (kFmt == BQ4_CACHE_F16) {
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t a0 = (w0[e] >> 8 * h) & kPair, a2 = (w0[e] >> (8 * h + 4)) & kPair;
+              const uint32_t a1 = (w1[e] >> 8 * h) & kPair, a3 = (w1[e] >> (8 * h + 4)) & kPair;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int nt = 0; nt < kNT; ++nt)
-            mma16816(x[nt], w0[2 * h], w1[2 * h], w0[2 * h + 1], w1[2 * h + 1], q[nt][2 * p + h][0],
-                     q[nt][2 * p + h][1]);
-      } else if constexpr (kFmt == BQ4_CACHE_Q8) {
-#pragma unroll
-        for (int e = 0; e < Y::kKPiece / 4; ++e) {
-          const uint32_t a0 = __byte_perm(w0[e], 0, 0x4140), a2 = __byte_perm(w0[e], 0, 0x4342);
-          const uint32_t a1 = __byte_perm(w1[e], 0, 0x4140), a3 = __byte_perm(w1[e], 0, 0x4342);
-#pragma unroll
-          for (int nt = 0; nt < kNT; ++nt)
-            mma16816(x[nt], a0, a1, a2, a3, q[nt][4 * p + e][0], q[nt][4 * p + e][1]);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < Y::kNb; ++e) {
-          float y[kNT][4];
-#pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) {
-            y[nt][0] = y[nt][2] = off[nt][e][0];
-            y[nt][1] = y[nt][3] = off[nt][e][1];
-          }
-          constexpr uint32_t kPair = 0x000F000Fu;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t a0 = (w0[e] >> 8 * h) & kPair, a2 = (w0[e] >> (8 * h + 4)) & kPair;
-            const uint32_t a1 = (w1[e] >> 8 * h) & kPair, a3 = (w1[e] >> (8 * h + 4)) & kPair;
+              for (int nt = 0; nt < kNT; ++nt)
+                mma16816(y[nt], a0, a1, a2, a3, q[nt][2 * e + h][0], q[nt][2 * e + h][1]);
+            }
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt)
-              mma16816(y[nt], a0, a1, a2, a3, q[nt][2 * e + h][0], q[nt][2 * e + h][1]);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) x[nt][u] = fmaf(y[nt][u], sk[u >> 1][e], x[nt][u]);
           }
-#pragma unroll
-          for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) x[nt][u] = fmaf(y[nt][u], sk[u >> 1][e], x[nt][u]);
         }
       }
-    }
-#pragma unroll
-    for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) x[nt][u] *= kFmt == BQ4_CACHE_Q8 ? sk[u >> 1][0] * c : c;
 
-    // ---- mask; a step below see_all has none
-    // (rows behind the end hold anything)
-    const bool edge = at + kStep > see_all;
-    if (edge) {
+      // ---- z = x - base, x in log2 units; a masked key's is -inf
+      const float c0 = kFmt == BQ4_CACHE_Q8 ? sk[0][0] * c : c, c1 = kFmt == BQ4_CACHE_Q8 ? sk[1][0] * c : c;
+      float z[kNT][4];
+      bool move = false;
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
+      for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (at + g + 8 * (u >> 1) >= see[nt][u & 1]) x[nt][u] = -INFINITY;
-    }
-
-    // ---- running maximum and v scale
-    bool move = false;
-#pragma unroll
-    for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) move |= fmaxf(x[nt][e], x[nt][e + 2]) > m[nt][e] + kJump;
-    float sv_top = 0.0f;
-    if constexpr (Y::kQ) {
-      if (edge) {
+        for (int u = 0; u < 4; ++u) {
+          z[nt][u] = fmaf(x[nt][u], u < 2 ? c0 : c1, -base[nt][u & 1]);
+          if (kEdge && limit[nt][u & 1] <= 8 * (u >> 1)) z[nt][u] = -INFINITY;
+        }
+        move |= fmaxf(fmaxf(z[nt][0], z[nt][1]), fmaxf(z[nt][2], z[nt][3])) > jump;
+      }
+      float sv_top = 0.0f;
+      if constexpr (Y::kQ) {
 #pragma unroll
         for (int r = 0; r < 2; ++r)
-          if (at + g + 8 * r >= end)
 #pragma unroll
-            for (int e = 0; e < Y::kNb; ++e) sv[r][e] = 0.0f;
+          for (int e = 0; e < Y::kNb; ++e) sv_top = fmaxf(sv_top, sv[r][e]);
+        move |= sv_top > vs;
       }
+      if (__any_sync(0xffffffffu, move)) {
+        if constexpr (Y::kQ) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int e = 0; e < Y::kNb; ++e) sv_top = fmaxf(sv_top, sv[r][e]);
-      move |= sv_top > vs;
-    }
-    if (__any_sync(0xffffffffu, move)) {
-      float beta = 1.0f;
-      if constexpr (Y::kQ) {
-#pragma unroll
-        for (int w = 4; w < 32; w <<= 1) sv_top = fmaxf(sv_top, __shfl_xor_sync(0xffffffffu, sv_top, w));
-        if (sv_top > vs) {
-          // the next power of two, kept where 1 / vs is a normal number too
-          const float up = __uint_as_float((__float_as_uint(sv_top) & 0x7f800000u) + 0x00800000u);
-          const float next = fminf(fmaxf(up, 0x1p-120f), 0x1p120f);
-          beta = vs / next;
-          vs = next;
-          inv_vs = 1.0f / next;
+          for (int w = 4; w < 32; w <<= 1) sv_top = fmaxf(sv_top, __shfl_xor_sync(0xffffffffu, sv_top, w));
+          if (sv_top > vs) {  // (held in [2^-100, 2^100]: p must not leave f32's range)
+            const int e = min(max((int)(__float_as_uint(sv_top) >> 23) - 126, -100), 100);
+            vs = __uint_as_float((uint32_t)(127 + e) << 23);
+            jump = kJump - (float)e;
+          }
         }
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x0 = x[nt][e] * c0, x1 = x[nt][e + 2] * c1;
+            if (kEdge && limit[nt][e] <= 0) x0 = -INFINITY;
+            if (kEdge && limit[nt][e] <= 8) x1 = -INFINITY;
+            float top = fmaxf(x0, x1);
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            float alpha = 1.0f;
+            if (top - base[nt][e] > jump) {
+              const float next = top - (jump - (kJump - kHead));
+              alpha = ex2(base[nt][e] - next);
+              base[nt][e] = next;
+            }
+            z[nt][e] = x0 - base[nt][e];
+            z[nt][e + 2] = x1 - base[nt][e];
+            l[nt][e] *= alpha;
+#pragma unroll
+            for (int mt = 0; mt < Y::kMT; ++mt) {
+              o[nt][mt][e] *= alpha;
+              o[nt][mt][e + 2] *= alpha;
+            }
+          }
       }
+
+      // ---- p, its sum, and p s_v as f16 in the B layout
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float top = fmaxf(x[nt][e], x[nt][e + 2]);
-#pragma unroll
-          for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-          float alpha = 1.0f;
-          if (top > m[nt][e] + kJump) {
-            alpha = ex2(m[nt][e] - (top - kHead));
-            m[nt][e] = top - kHead;
-          }
-          l[nt][e] *= alpha;
-#pragma unroll
-          for (int mt = 0; mt < Y::kMT; ++mt) {
-            o[nt][mt][e] *= alpha * beta;
-            o[nt][mt][e + 2] *= alpha * beta;
-          }
+        for (int u = 0; u < 4; ++u) {
+          z[nt][u] = ex2(z[nt][u]);
+          l[nt][u & 1] += z[nt][u];
         }
-    }
-
-    // ---- p = 2^(x - m), its sum, and p (s_v / vs) as f16 in the B layout
-#pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        x[nt][u] = ex2(x[nt][u] - m[nt][u & 1]);
-        l[nt][u & 1] += x[nt][u];
-      }
-    }
-    uint32_t pb[kNT][2];
-    auto weigh = [&](int e) {
-      if constexpr (Y::kQ) {
-        const float f0 = sv[0][e] * inv_vs, f1 = sv[1][e] * inv_vs;
+      uint32_t pb[kNT][2];
+      auto weigh = [&](int e) {
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
-          float y[4] = {x[nt][0] * f0, x[nt][1] * f0, x[nt][2] * f1, x[nt][3] * f1};
-          if (edge) {
-            // a masked key's scale may be NaN
+          float y[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (at + g + 8 * (u >> 1) >= see[nt][u & 1]) y[u] = 0.0f;
+          for (int u = 0; u < 4; ++u) {
+            y[u] = Y::kQ ? z[nt][u] * sv[u >> 1][Y::kQ ? e : 0] : z[nt][u];
+            // a masked key's scale may be NaN
+            if (kEdge && Y::kQ && limit[nt][u & 1] <= 8 * (u >> 1)) y[u] = 0.0f;
           }
           pb[nt][0] = transpose8(pack_h2(y[0], y[1]));
           pb[nt][1] = transpose8(pack_h2(y[2], y[3]));
         }
-      } else {
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
-          pb[nt][0] = transpose8(pack_h2(x[nt][0], x[nt][1]));
-          pb[nt][1] = transpose8(pack_h2(x[nt][2], x[nt][3]));
-        }
-      }
-    };
+      };
 
-    // ---- O^T += V^T P^T
-    uint32_t v[4][Y::kVPieces][Y::kVPiece / 4];
+      // ---- O^T += V^T P^T
+      uint32_t v[4][Y::kVPieces][Y::kVPiece / 4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int p = 0; p < Y::kVPieces; ++p)
-        lds(st + (r & 1 ? v_at1 : v_at0) + (r >> 1) * 8 * Y::kRow + p * 128, v[r][p]);
-    if constexpr (kFmt == BQ4_CACHE_F16) {
-      weigh(0);
+        for (int p = 0; p < Y::kVPieces; ++p)
+          lds(st + (r & 1 ? v_at1 : v_at0) + (r >> 1) * 8 * Y::kRow + p * 128, v[r][p]);
+      if constexpr (kFmt == BQ4_CACHE_F16) {
+        weigh(0);
 #pragma unroll
-      for (int p = 0; p < Y::kVPieces; ++p)
+        for (int p = 0; p < Y::kVPieces; ++p)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t f[4] = {__byte_perm(v[0][p][e], v[1][p][e], 0x5410), __byte_perm(v[0][p][e], v[1][p][e], 0x7632),
-                           __byte_perm(v[2][p][e], v[3][p][e], 0x5410), __byte_perm(v[2][p][e], v[3][p][e], 0x7632)};
-          const int mt = 4 * p + e;
-          if (edge) {
-            // A key that some row does not see may hold infinities or NaN: they leave the
-            // product, which would carry 0 * NaN into that row, and reach the rows that
-            // see the key one by one.  f[r]: keys 2t, 2t + 1 (r < 2) or + 8, value d + (r & 1).
-            bool odd = false;
+          for (int e = 0; e < 4; ++e) {
+            uint32_t f[4] = {__byte_perm(v[0][p][e], v[1][p][e], 0x5410), __byte_perm(v[0][p][e], v[1][p][e], 0x7632),
+                             __byte_perm(v[2][p][e], v[3][p][e], 0x5410), __byte_perm(v[2][p][e], v[3][p][e], 0x7632)};
+            const int mt = 4 * p + e;
+            if constexpr (kEdge) {
+              // A key that some row does not see may hold infinities or NaN: they leave the
+              // product, which would carry 0 * NaN into that row, and reach the rows that
+              // see the key one by one.  f[r]: keys 2t, 2t + 1 (r < 2) or + 8, value d + (r & 1).
+              bool odd = false;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const uint32_t lo = f[r] & 0x00007c00u, hi = f[r] & 0x7c000000u;
-              odd |= lo == 0x00007c00u || hi == 0x7c000000u;
-            }
-            if (__any_sync(0xffffffffu, odd)) {
+              for (int r = 0; r < 4; ++r)
+                odd |= (f[r] & 0x00007c00u) == 0x00007c00u || (f[r] & 0x7c000000u) == 0x7c000000u;
+              if (__any_sync(0xffffffffu, odd)) {
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const uint32_t bad = ((f[r] & 0x00007c00u) == 0x00007c00u ? f[r] & 0xffffu : 0) |
-                                     ((f[r] & 0x7c000000u) == 0x7c000000u ? f[r] & 0xffff0000u : 0);
-                if ((f[r] & 0x00007c00u) == 0x00007c00u) f[r] &= 0xffff0000u;
-                if ((f[r] & 0x7c000000u) == 0x7c000000u) f[r] &= 0x0000ffffu;
-                for (int w = 0; w < 4; ++w) {  // lane t = w of this g holds keys 2w, 2w + 1 (+ 8)
-                  const uint32_t from = __shfl_sync(0xffffffffu, bad, 4 * g + w);
+                for (int r = 0; r < 4; ++r) {
+                  const uint32_t bad = ((f[r] & 0x00007c00u) == 0x00007c00u ? f[r] & 0xffffu : 0) |
+                                       ((f[r] & 0x7c000000u) == 0x7c000000u ? f[r] & 0xffff0000u : 0);
+                  if ((f[r] & 0x00007c00u) == 0x00007c00u) f[r] &= 0xffff0000u;
+                  if ((f[r] & 0x7c000000u) == 0x7c000000u) f[r] &= 0x0000ffffu;
+                  for (int w = 0; w < 4; ++w) {  // lane t = w of this g holds keys 2w, 2w + 1 (+ 8)
+                    const uint32_t from = __shfl_sync(0xffffffffu, bad, 4 * g + w);
 #pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    const uint32_t bits = from >> 16 * h & 0xffffu;
-                    const int key = at + 2 * w + h + 8 * (r >> 1);
-                    const float add = __half2float(__ushort_as_half((unsigned short)bits));
-                    if (bits) {
+                    for (int h = 0; h < 2; ++h) {
+                      const uint32_t bits = from >> 16 * h & 0xffffu;
+                      const int key = 2 * w + h + 8 * (r >> 1);
+                      const float add = __half2float(__ushort_as_half((unsigned short)bits));
+                      if (bits) {
 #pragma unroll
-                      for (int nt = 0; nt < kNT; ++nt)
+                        for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-                        for (int e2 = 0; e2 < 2; ++e2)
-                          if (key < see[nt][e2]) o[nt][mt][e2 + 2 * (r & 1)] += add;
+                          for (int e2 = 0; e2 < 2; ++e2)
+                            if (key < limit[nt][e2] + g) o[nt][mt][e2 + 2 * (r & 1)] += add;
+                      }
                     }
                   }
                 }
               }
             }
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt) mma16816(o[nt][mt], f[0], f[1], f[2], f[3], pb[nt][0], pb[nt][1]);
           }
+      } else if constexpr (kFmt == BQ4_CACHE_Q8) {
+        weigh(0);
+        constexpr uint32_t kZero = 0x80808080u;  // two halves of -128 2^-24
 #pragma unroll
-          for (int nt = 0; nt < kNT; ++nt)
-            mma16816(o[nt][mt], f[0], f[1], f[2], f[3], pb[nt][0], pb[nt][1]);
-        }
-    } else if constexpr (kFmt == BQ4_CACHE_Q8) {
-      weigh(0);
-      constexpr uint32_t kZero = 0x80808080u;  // two halves of -128 2^-24
+        for (int e = 0; e < Y::kVPiece / 4; ++e)
 #pragma unroll
-      for (int e = 0; e < Y::kVPiece / 4; ++e)
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t y0 = __byte_perm(v[0][0][e], v[1][0][e], h ? 0x7632 : 0x5410);
+            const uint32_t y1 = __byte_perm(v[2][0][e], v[3][0][e], h ? 0x7632 : 0x5410);
+            const uint32_t f0 = add_h2(y0 & 0x00ff00ffu, kZero), f1 = add_h2(__byte_perm(y0, 0, 0x4341), kZero);
+            const uint32_t f2 = add_h2(y1 & 0x00ff00ffu, kZero), f3 = add_h2(__byte_perm(y1, 0, 0x4341), kZero);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t y0 = __byte_perm(v[0][0][e], v[1][0][e], h ? 0x7632 : 0x5410);
-          const uint32_t y1 = __byte_perm(v[2][0][e], v[3][0][e], h ? 0x7632 : 0x5410);
-          const uint32_t f0 = add_h2(y0 & 0x00ff00ffu, kZero), f1 = add_h2(__byte_perm(y0, 0, 0x4341), kZero);
-          const uint32_t f2 = add_h2(y1 & 0x00ff00ffu, kZero), f3 = add_h2(__byte_perm(y1, 0, 0x4341), kZero);
+            for (int nt = 0; nt < kNT; ++nt) mma16816(o[nt][2 * e + h], f0, f1, f2, f3, pb[nt][0], pb[nt][1]);
+          }
+      } else {
+        constexpr uint32_t kPair = 0x000F000Fu, kZero = 0x80088008u, kZero16 = 0x80808080u;
 #pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) mma16816(o[nt][2 * e + h], f0, f1, f2, f3, pb[nt][0], pb[nt][1]);
-        }
-    } else {
-      constexpr uint32_t kPair = 0x000F000Fu, kZero = 0x80088008u, kZero16 = 0x80808080u;
+        for (int e = 0; e < Y::kNb; ++e) {
+          weigh(e);
+          const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
+          const uint32_t y0 = __byte_perm(v[0][0][e >> 1], v[1][0][e >> 1], sel);
+          const uint32_t y1 = __byte_perm(v[2][0][e >> 1], v[3][0][e >> 1], sel);
 #pragma unroll
-      for (int e = 0; e < Y::kNb; ++e) {
-        weigh(e);
-        const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
-        const uint32_t y0 = __byte_perm(v[0][0][e >> 1], v[1][0][e >> 1], sel);
-        const uint32_t y1 = __byte_perm(v[2][0][e >> 1], v[3][0][e >> 1], sel);
+          for (int h = 0; h < 2; ++h) {
+            // the odd value's nibble is taken where it lies, 16 times too large; undone at the end
+            const uint32_t z0 = y0 >> 8 * h, z1 = y1 >> 8 * h;
+            const uint32_t f0 = add_h2(z0 & kPair, kZero), f1 = add_h2(z0 & kPair << 4, kZero16);
+            const uint32_t f2 = add_h2(z1 & kPair, kZero), f3 = add_h2(z1 & kPair << 4, kZero16);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          // the odd value's nibble is taken where it lies, 16 times too large; undone at the end
-          const uint32_t z0 = y0 >> 8 * h, z1 = y1 >> 8 * h;
-          const uint32_t f0 = add_h2(z0 & kPair, kZero), f1 = add_h2(z0 & kPair << 4, kZero16);
-          const uint32_t f2 = add_h2(z1 & kPair, kZero), f3 = add_h2(z1 & kPair << 4, kZero16);
-#pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) mma16816(o[nt][2 * e + h], f0, f1, f2, f3, pb[nt][0], pb[nt][1]);
+            for (int nt = 0; nt < kNT; ++nt) mma16816(o[nt][2 * e + h], f0, f1, f2, f3, pb[nt][0], pb[nt][1]);
+          }
         }
       }
+      return true;
+    };
+    int j = 0;
+    while (j < plain && step(std::false_type{}, j)) ++j;
+    if (j >= plain)
+      while (j < mine && step(std::true_type{}, j)) ++j;
+    if (j < mine && lane == 0) {  // rows that did not come
+      abort_flag = 1;
+      atomicCAS(a.err, 0, (int)BQ4_ETIMEOUT);
     }
-  }
 
-  // ---- join the four warps through shared memory, in warp order
-  __syncthreads();
-  if (abort_flag) {
-    // a copy did not come: wait once more for those under way, then leave
-    __shared__ int never;
-    if (threadIdx.x == 0) never = 0;
+    // ---- join the four warps through shared memory, in warp order
     __syncthreads();
-    for (; get != put; get = get + 1 == Y::kStages ? 0 : get + 1) {
-      ptx::mbar_wait(&full[get], parity, &never);
-      if (get + 1 == Y::kStages) parity ^= 1;
+    if (abort_flag) {
+      // wait once more for the copies under way, then leave
+      __shared__ int never;
+      if (threadIdx.x == 0) never = 0;
+      __syncthreads();
+      for (; get != put; get = get + 1 == Y::kStages ? 0 : get + 1) {
+        ptx::mbar_wait(&full[get], parity, &never);
+        if (get + 1 == Y::kStages) parity ^= 1;
+      }
+      return;
     }
-    return;
-  }
-  float* om = reinterpret_cast<float*>(smem);                                  // [warp][row][kHP + 4]
-  float2* mlw = reinterpret_cast<float2*>(om + kSWarps * 8 * kNT * (kHP + 4));  // [warp][row]
-  const float unit = Y::kQ ? vs * 0x1p24f : 1.0f;
+    float* om = reinterpret_cast<float*>(smem);                                  // [warp][row][kHP + 4]
+    float2* mlw = reinterpret_cast<float2*>(om + kSWarps * 8 * kNT * (kHP + 4));  // [warp][row]
+    constexpr float kLo = Y::kQ ? 0x1p24f : 1.0f, kHi = kFmt == BQ4_CACHE_Q4 ? 0x1p20f : kLo;
 #pragma unroll
-  for (int nt = 0; nt < kNT; ++nt)
+    for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float sum = l[nt][e];
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[nt][e];
 #pragma unroll
-      for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-      const int r = (warp * kNT + nt) * 8 + 2 * t + e;
-      if (g == 0) mlw[r] = make_float2(m[nt][e], sum);
+        for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        const int r = (warp * kNT + nt) * 8 + 2 * t + e;
+        if (g == 0) mlw[r] = make_float2(base[nt][e], sum);
 #pragma unroll
-      for (int mt = 0; mt < Y::kMT; ++mt) {
-        const float hi = kFmt == BQ4_CACHE_Q4 ? unit * 0.0625f : unit;
-        *reinterpret_cast<float2*>(om + r * (kHP + 4) + Y::od(mt, g)) =
-            make_float2(o[nt][mt][e] * unit, o[nt][mt][e + 2] * hi);
+        for (int mt = 0; mt < Y::kMT; ++mt)
+          *reinterpret_cast<float2*>(om + r * (kHP + 4) + Y::od(mt, g)) =
+              make_float2(o[nt][mt][e] * kLo, o[nt][mt][e + 2] * kHi);
+      }
+    __syncthreads();
+    const int64_t piece = ((int64_t)blockIdx.x + range) * 8 * kNT;
+    const bool finish = whole && s.finish && line_p == 0;
+    for (int i = threadIdx.x; i < 8 * kNT * (kHP / 4); i += kSThreads) {
+      const int r = i / (kHP / 4), d = 4 * (i - r * (kHP / 4));
+      if (row0 + r >= rows) break;
+      float top = kNone;
+#pragma unroll
+      for (int w = 0; w < kSWarps; ++w) top = fmaxf(top, mlw[w * 8 * kNT + r].x);
+      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float lsum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kSWarps; ++w) {
+        const float2 e = mlw[w * 8 * kNT + r];
+        const float f = ex2(e.x - top);
+        const float4 y = *reinterpret_cast<const float4*>(om + (w * 8 * kNT + r) * (kHP + 4) + d);
+        lsum += f * e.y;
+        sum.x += f * y.x, sum.y += f * y.y, sum.z += f * y.z, sum.w += f * y.w;
+      }
+      if (finish) {
+        if (d < a.c.head_dim) {
+          const Row w = row_of(s, prefix, b, kvh, row0 + r);
+          const int64_t row = ((int64_t)w.b * a.tokens + w.i) * a.q_heads + w.h;
+          const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+          const uint2 u = make_uint2(pack_h2(sum.x * inv, sum.y * inv), pack_h2(sum.z * inv, sum.w * inv));
+          *reinterpret_cast<uint2*>(a.out + row * a.c.head_dim + d) = u;
+        }
+      } else {
+        *reinterpret_cast<float4*>(s.part + (piece + r) * kHP + d) = sum;
+        if (d == 0) s.ml[piece + r] = make_float2(top, lsum);
       }
     }
-  __syncthreads();
-  const int64_t piece = ((int64_t)blockIdx.x + range) * 8 * kNT;
-  const bool finish = whole && s.finish && line_p == 0;
-  for (int i = threadIdx.x; i < 8 * kNT * (kHP / 4); i += kSThreads) {
-    const int r = i / (kHP / 4), d = 4 * (i - r * (kHP / 4));
-    if (row0 + r >= rows) break;
-    float top = kNone;
-#pragma unroll
-    for (int w = 0; w < kSWarps; ++w) top = fmaxf(top, mlw[w * 8 * kNT + r].x);
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float lsum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kSWarps; ++w) {
-      const float2 e = mlw[w * 8 * kNT + r];
-      const float f = ex2(e.x - top);
-      const float4 y = *reinterpret_cast<const float4*>(om + (w * 8 * kNT + r) * (kHP + 4) + d);
-      lsum += f * e.y;
-      sum.x += f * y.x, sum.y += f * y.y, sum.z += f * y.z, sum.w += f * y.w;
-    }
-    if (finish) {
-      if (d < a.c.head_dim) {
-        const Row w = row_of(s, prefix, b, kvh, row0 + r);
-        const int64_t row = ((int64_t)w.b * a.tokens + w.i) * a.q_heads + w.h;
-        const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-        const uint2 u = make_uint2(pack_h2(sum.x * inv, sum.y * inv), pack_h2(sum.z * inv, sum.w * inv));
-        *reinterpret_cast<uint2*>(a.out + row * a.c.head_dim + d) = u;
-      }
-    } else {
-      *reinterpret_cast<float4*>(s.part + (piece + r) * kHP + d) = sum;
-      if (d == 0) s.ml[piece + r] = make_float2(top, lsum);
-    }
-  }
 
-  // ---- the next range of the line
-  at_unit = piece_to;
-  if (at_unit >= to_unit) return;
-  ptx::fence_proxy_async_smem();  // the copies write where the warps were joined
-  __syncthreads();
-  first += units;
-  if (++tile == (prefix ? s.p_tiles : s.s_tiles)) {
-    tile = 0;
-    if (++kvh == a.c.kv_heads) {
-      kvh = 0;
-      b = prefix ? 0 : b + 1;
-      prefix = false;
-      for (;; ++b) {
-        n = own_length(a, b);
-        units = (n + kUnit - 1) / kUnit;
-        if (units) break;
+    // ---- the next range of the line
+    at_unit = piece_to;
+    if (at_unit >= to_unit) return;
+    ptx::fence_proxy_async_smem();  // the copies write where the warps were joined
+    __syncthreads();
+    first += units;
+    if (++tile == (prefix ? s.p_tiles : s.s_tiles)) {
+      tile = 0;
+      if (++kvh == a.c.kv_heads) {
+        kvh = 0;
+        b = prefix ? 0 : b + 1;
+        prefix = false;
+        for (;; ++b) {
+          n = own_length(a, b);
+          units = (unsigned)(n + kUnit - 1) / kUnit;
+          if (units) break;
+        }
       }
     }
-  }
   }
 }
 
@@ -912,13 +916,15 @@ bool plan_split(const CacheAttnCall& a, int sms, SplitPlan* p) {
   p->p_tiles = prefix > 0 ? (int)((all + tile - 1) / tile) : 0;
   const int64_t ranges = ((int64_t)p->p_tiles + (int64_t)a.s.batch * p->s_tiles) * a.c.kv_heads;
   const int64_t per = ((int64_t)a.max_length + kUnit - 1) / kUnit, per_p = (prefix + kUnit - 1) / kUnit;
-  const int per_sm = p->nt == 2 ? 2 : a.c.format == BQ4_CACHE_F16 && a.c.hp == 128 ? 3 : 4;  // Layout::kPerSm
-  const int64_t most = (int64_t)per_sm * sms;
+  const int64_t most = (int64_t)split_per_sm(a.c.format, a.c.hp, p->nt) * sms;
   const int64_t units = std::min(most, per_p * p->p_tiles * a.c.kv_heads) +
                         std::min(most, per * std::min(most, (int64_t)a.s.batch * p->s_tiles * a.c.kv_heads));
   p->grid = (int)std::max<int64_t>(1, std::min(most, units));
   const int64_t slots = (ranges + p->grid) * tile;
-  if (ranges > 0x3fffffff || slots > ((int64_t)1 << 40)) return false;
+  // the line's units and the ranges are counted in 32 bits
+  if (ranges > 0x3fffffff || per_p * p->p_tiles * a.c.kv_heads > 0x3fffffff ||
+      (per > 0 && (int64_t)a.s.batch * p->s_tiles * a.c.kv_heads > 0x3fffffff / per))
+    return false;
   p->part_bytes = up256((size_t)slots * a.c.hp * 4);
   p->ml_bytes = up256((size_t)slots * 8);
   p->pieces_bytes = up256((size_t)ranges * 8);
