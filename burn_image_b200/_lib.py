@@ -91,7 +91,7 @@ SIGNATURES = {
     "bq4_packed_f16_conv2d": (_st, [_p, _i64, _i64, _i64, _i64, _p, _i64, _i32, _i32, _p, _p, _p, _p, _sz, _p]),
     "bq4_attention_workspace_size": (_st, [_i64, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_sz)]),
     "bq4_attention": (_st, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _p, _p, _sz, _p]),
-    "bq4_cache_sizes": (_st, [_p, ctypes.POINTER(_sz), ctypes.POINTER(_sz)]),
+    "bq4_cache_size": (_st, [_p, ctypes.POINTER(_sz)]),
     "bq4_cache_append": (_st, [_p, _p, _p, _p, _p, _p, _i32, _i64, _p]),
     "bq4_cache_read": (_st, [_p, _p, _p, _i64, _p, _p, _p, _i32, _p]),
     "bq4_cache_attention_workspace_size": (_st, [_p, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_sz)]),
@@ -115,9 +115,9 @@ class Conv2dOptions(ctypes.Structure):
 
 
 class Cache(ctypes.Structure):
-    """bq4_cache: the buffers and geometry of a paged key/value cache."""
-    _fields_ = [("values", _p), ("scales", _p), ("pages", _i64), ("page_size", _i32), ("kv_heads", _i32),
-                ("head_dim", _i32), ("format", _i32), ("device", _i32)]
+    """bq4_cache: the buffer and geometry of a paged key/value cache."""
+    _fields_ = [("data", _p), ("pages", _i64), ("page_size", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+                ("format", _i32), ("device", _i32)]
 
 
 class CacheSequences(ctypes.Structure):

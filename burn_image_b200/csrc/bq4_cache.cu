@@ -24,17 +24,17 @@ namespace {
 constexpr int kCThreads = 256;
 
 struct CacheRow {
-  uint8_t* rows;   // k or v rows of the page and head
-  uint16_t* scales;
+  uint8_t* rows;     // k or v rows of the step
+  uint16_t* scales;  // of its row at `place`
 };
 
-// Rows of (page, head) and the scales of the row at `place`; kv: 0 k, 1 v.  The next
-// row's scales lie 2 nb on.
+// Rows of the step of (page, head) that holds `place`; kv: 0 k, 1 v.  The next row's
+// scales lie 2 nb on.
 __device__ __forceinline__ CacheRow cache_row(const CacheView& c, int page, int head, int place, int kv) {
-  const int64_t ph = (int64_t)page * c.kv_heads + head;
+  uint8_t* step = cache_step(c, page, head, place);
   CacheRow r;
-  r.rows = c.values + (ph * 2 + kv) * c.kv_bytes;
-  r.scales = c.scales + ((ph * c.page_size + place) * 2 + kv) * c.nb;
+  r.rows = step + kv * 16 * c.row_bytes;
+  r.scales = reinterpret_cast<uint16_t*>(step + 32 * c.row_bytes) + ((place & 15) * 2 + kv) * c.nb;
   return r;
 }
 
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kCThreads) cache_append_kernel(const __grid_co
       const bool live = base + row >= first && base + row < end;
       if (!__any_sync(0xffffffffu, live)) continue;
       float(&x)[kW] = xs[j];
-      auto dst = [&](int at) { return r.rows + cache_swizzle(kv, kRow, place0 + row, at); };
+      auto dst = [&](int at) { return r.rows + cache_swizzle(kv, kRow, (place0 & 15) + row, at); };
       uint16_t* sc = r.scales + row * 2 * kNb;
       if constexpr (kFmt == BQ4_CACHE_F16) {
         uint32_t w[kW / 2];
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kCThreads) cache_read_kernel(const __grid_cons
       for (int e = 0; e < kWords; ++e) held[j][e] = 0;
       scale[j] = 0;
       if (live) {
-        auto src = [&](int at) { return r.rows + cache_swizzle(kv, kRow, place0 + row, at); };
+        auto src = [&](int at) { return r.rows + cache_swizzle(kv, kRow, (place0 & 15) + row, at); };
         const uint16_t* sc = r.scales + row * 2 * kNb;
         if constexpr (kFmt == BQ4_CACHE_F16) {
           load_words<kHeld>(src(2 * d0), held[j]);
@@ -421,8 +421,7 @@ bq4_status check_geometry(const bq4_cache* c) {
 
 CacheView view_of(const bq4_cache* c) {
   CacheView v;
-  v.values = static_cast<uint8_t*>(c->values);
-  v.scales = static_cast<uint16_t*>(c->scales);
+  v.data = static_cast<uint8_t*>(c->data);
   v.pages = (int32_t)c->pages;
   v.page_size = c->page_size;
   v.kv_heads = c->kv_heads;
@@ -431,17 +430,15 @@ CacheView view_of(const bq4_cache* c) {
   v.nb = cache_nb(c->format, v.hp);
   v.row_bytes = cache_row_bytes(c->format, v.hp);
   v.format = c->format;
-  v.kv_bytes = (int64_t)c->page_size * v.row_bytes;
+  v.step_bytes = cache_step_bytes(v.row_bytes, v.nb);
   return v;
 }
 
 bq4_status check_cache(const bq4_cache* c) {
   bq4_status st = check_geometry(c);
   if (st) return st;
-  if (!c->values || (!c->scales && c->format != BQ4_CACHE_F16))
-    return set_error(BQ4_EINVAL_ARG, "the cache's values/scales are NULL");
-  if (!al(c->values, 256) || !al(c->scales, 256))
-    return set_error(BQ4_EALIGN, "the cache's buffers must be 256-byte aligned");
+  if (!c->data) return set_error(BQ4_EINVAL_ARG, "the cache's data is NULL");
+  if (!al(c->data, 256)) return set_error(BQ4_EALIGN, "the cache's data must be 256-byte aligned");
   return BQ4_OK;
 }
 
@@ -604,14 +601,11 @@ using namespace bq4;
 
 extern "C" {
 
-bq4_status bq4_cache_sizes(const bq4_cache* cache, size_t* values_bytes, size_t* scales_bytes) {
+bq4_status bq4_cache_size(const bq4_cache* cache, size_t* bytes) {
   bq4_status st = check_geometry(cache);
   if (st) return st;
-  if (!values_bytes || !scales_bytes) return set_error(BQ4_EINVAL_ARG, "values_bytes/scales_bytes is NULL");
-  const CacheView v = view_of(cache);
-  const size_t rows = (size_t)cache->pages * cache->kv_heads * 2 * cache->page_size;
-  *values_bytes = rows * v.row_bytes;
-  *scales_bytes = rows * v.nb * 2;
+  if (!bytes) return set_error(BQ4_EINVAL_ARG, "bytes is NULL");
+  *bytes = (size_t)cache->pages * cache->kv_heads * (cache->page_size / kCachePageUnit) * view_of(cache).step_bytes;
   return BQ4_OK;
 }
 

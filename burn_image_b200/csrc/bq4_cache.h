@@ -1,10 +1,12 @@
 // bq4_cache.h -- layout of the paged key/value cache, shared by its kernels.
 //
 // One page holds page_size consecutive tokens of one sequence, for every kv
-// head.  Rows are padded to HP = 64 or 128 values (head_dim rounded up):
-//   values u8  [pages][kv_heads][2 (k, v)][page_size][row_bytes]
-//   scales u16 [pages][kv_heads][page_size][2 (k, v)][nb]        (bf16 bits)
-// so that the k rows (and the v rows) of one page and head are contiguous.
+// head.  Rows are padded to HP = 64 or 128 values (head_dim rounded up).  The 16
+// tokens of a step lie together, so that one bulk copy brings them:
+//   data u8 [pages][kv_heads][page_size / 16][step bytes], a step being
+//     k rows [16][row bytes], v rows [16][row bytes],
+//     scales u16 [16][2 (k, v)][nb] (bf16 bits)
+// Rows:
 //   f16: 2 HP bytes, no scales.
 //   q8:  byte d holds q_d + 128; one scale for the row (nb = 1).
 //   q4:  a nibble holds q + 8; one scale for each 32 values (nb = HP / 32).
@@ -29,12 +31,11 @@ constexpr int kCachePageUnit = 16;    // page sizes are multiples of this
 constexpr int kCacheMaxHeadDim = 128;
 
 struct CacheView {
-  uint8_t* values;
-  uint16_t* scales;
+  uint8_t* data;
   int32_t pages, page_size, kv_heads, head_dim;
   int32_t hp, nb, row_bytes;  // padded head, scales of a row, bytes of a row
   int32_t format;
-  int64_t kv_bytes;           // k (or v) rows of one page and head
+  int32_t step_bytes;
 };
 
 struct SeqView {
@@ -52,11 +53,19 @@ inline int cache_row_bytes(int format, int hp) {
   return format == BQ4_CACHE_F16 ? 2 * hp : format == BQ4_CACHE_Q8 ? hp : hp / 2;
 }
 
-// Byte of the k (v) rows of a page and head where byte `at` of row r lies.
+// Byte of the k (v) rows of a step where byte `at` of row r lies.
 __host__ __device__ __forceinline__ constexpr int cache_swizzle(int kv, int row_bytes, int r, int at) {
   const int f = kv == 0 ? (row_bytes >= 128 ? 4 * (r & 1) : 0)
                         : row_bytes >= 64 ? 2 * (r >> 1 & 3) : 2 * (r >> 2 & 1);
   return (r * row_bytes + at) ^ f << 4;
+}
+
+inline int cache_step_bytes(int row_bytes, int nb) { return 16 * (2 * row_bytes + 4 * nb); }
+
+// The step that holds `place` of (page, head).
+__device__ __forceinline__ uint8_t* cache_step(const CacheView& c, int page, int head, int place) {
+  const int64_t steps = ((int64_t)page * c.kv_heads + head) * (c.page_size >> 4) + (place >> 4);
+  return c.data + steps * c.step_bytes;
 }
 
 // Arguments of one attention call (bq4_cache_attn.cu).

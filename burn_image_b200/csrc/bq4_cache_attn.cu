@@ -20,9 +20,9 @@
 //     query heads fills half of N = 8, not a quarter of M = 16, and the widened
 //     cache values (A) are made once for all rows.
 //   * The 16 rows of a step lie together in their page (k, v and scales): one
-//     lane brings them to a ring of the warp's own with three bulk copies,
-//     some steps ahead; an mbarrier says when they are there.  No warp waits
-//     for another in the loop.
+//     lane brings them to a ring of the warp's own with one bulk copy, some
+//     steps ahead; an mbarrier says when they are there.  No warp waits for
+//     another in the loop.
 //   * Lane (g = lane / 4, t = lane % 4) reads quarter t of k rows g and g + 8
 //     and eighth g of v rows 2t, 2t + 1, 2t + 8, 2t + 9, 16 bytes at a time.  Any
 //     order of the head's values inside a fragment is as good as another as
@@ -157,7 +157,6 @@ struct Layout {
 struct SplitArgs {
   CacheAttnCall a;
   uint64_t page_magic;   // floor(u / (page_size / 16)) = u * page_magic >> 38
-  int64_t page_stride;   // bytes of a page
   float c;               // scale * log2(e)
   int group;             // query heads of a kv head
   int p_tiles, s_tiles;  // row tiles of the prefix and of one sequence
@@ -309,8 +308,7 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
     const int steps = end <= key0 ? 0 : (end - key0 + kStep - 1) / kStep;
     const int mine = steps > warp ? (steps - warp + kSWarps - 1) / kSWarps : 0;
     const int at0 = key0 + warp * kStep;  // first key of step 0; step j lies kUnit j on
-    const uint8_t* k_src = nullptr;
-    const uint8_t* s_src = nullptr;
+    const uint8_t* src = nullptr;
     unsigned held = 0, held_before = 0;   // bit j % 32: step j's page exists; of the 32 steps before them
     int plain = mine;                     // steps below it have a page and no mask
     auto locate = [&](int j) {
@@ -325,26 +323,20 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
           atomicCAS(a.err, 0, (int)BQ4_EINVAL_ARG);
           page = 0;
         }
-        const int64_t ph = (int64_t)page * a.c.kv_heads + kvh;
-        k_src = a.c.values + ph * 2 * a.c.kv_bytes + place * Y::kRow;
-        if constexpr (Y::kQ)
-          s_src = reinterpret_cast<const uint8_t*>(a.c.scales) + (ph * a.c.page_size + place) * Y::kScale;
+        src = cache_step(a.c, page, kvh, place);
       }
       held_before = held;
       held = __ballot_sync(0xffffffffu, ok);
       if (held != 0xffffffffu) plain = min(plain, j);
     };
-    // three bulk copies bring step j, by the lane that knows it (of a step without a page, page
-    // 0's rows: they are masked)
+    // one bulk copy brings step j, by the lane that knows it (of a step without a page, page 0's
+    // rows: they are masked)
     auto fetch = [&](int j) {
       if (j >= mine) return;
       if ((j & 31) == 0) locate(j);
       if (lane == (j & 31)) {
-        uint8_t* st = smem + (warp * Y::kStages + put) * Y::kStage;
         ptx::mbar_arrive_expect_tx(&full[put], Y::kStage);
-        ptx::bulk_load(st, k_src, kStep * Y::kRow, &full[put]);
-        ptx::bulk_load(st + Y::kOffV, k_src + a.c.kv_bytes, kStep * Y::kRow, &full[put]);
-        if constexpr (Y::kQ) ptx::bulk_load(st + Y::kOffS, s_src, kStep * Y::kScale, &full[put]);
+        ptx::bulk_load(smem + (warp * Y::kStages + put) * Y::kStage, src, Y::kStage, &full[put]);
       }
       put = put + 1 == Y::kStages ? 0 : put + 1;
     };
@@ -445,7 +437,7 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
       }
 
       // ---- scales of keys g, g + 8
-      float sk[2][Y::kQ ? Y::kNb : 1], sv[2][Y::kQ ? Y::kNb : 1];
+      float sk[2][Y::kQ ? Y::kNb : 1] = {}, sv[2][Y::kQ ? Y::kNb : 1] = {};
       if constexpr (Y::kQ) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -538,7 +530,7 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
         }
         move |= fmaxf(fmaxf(z[nt][0], z[nt][1]), fmaxf(z[nt][2], z[nt][3])) > jump;
       }
-      float sv_top = 0.0f;
+      [[maybe_unused]] float sv_top = 0.0f;
       if constexpr (Y::kQ) {
 #pragma unroll
         for (int r = 0; r < 2; ++r)
@@ -1004,7 +996,6 @@ bq4_status run_split(const CacheAttnCall& a, const SplitPlan& p, bool finish, vo
   s.a = a;
   const uint64_t unit = (uint64_t)(a.c.page_size / kStep);
   s.page_magic = ((1ull << 38) + unit - 1) / unit;
-  s.page_stride = (int64_t)a.c.kv_heads * 2 * a.c.kv_bytes;
   s.c = a.scale * 1.4426950408889634f;  // log2(e)
   s.group = a.q_heads / a.c.kv_heads;
   s.p_tiles = p.p_tiles;

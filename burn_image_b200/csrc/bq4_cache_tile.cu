@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
   }
 
   // ---- a record
-  __shared__ int64_t at[kKeys];                // k rows of the key's page and head, -1: no such row
+  __shared__ int64_t at[kKeys];                // byte of the key's step in the cache, -1: no such row
   __shared__ int place[kKeys];
   __shared__ float sk[kKeys][kNb], sv[kKeys][kNb], ck[kKeys];
   __shared__ float top[4];
@@ -152,10 +152,10 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
       const int page = s.prefix ? s.a.prefix_table[pi] : s.a.s.table[set * s.a.s.table_stride + pi];
       place[tid] = pos - pi * c.page_size;
       if (page >= 0 && page < c.pages) {
-        const int64_t ph = (int64_t)page * c.kv_heads + kvh;
-        where = ph * 2 * c.kv_bytes;
+        const uint8_t* step = cache_step(c, page, kvh, place[tid]);
+        where = step - c.data;
         if constexpr (kFmt != BQ4_CACHE_F16) {
-          const uint16_t* sc = c.scales + (ph * c.page_size + place[tid]) * 2 * kNb;
+          const uint16_t* sc = reinterpret_cast<const uint16_t*>(step + 32 * kRow) + (place[tid] & 15) * 2 * kNb;
           float ktop = 0.0f;
           bool odd = false;
 #pragma unroll
@@ -212,9 +212,9 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
     uint32_t kw[4] = {0, 0, 0, 0}, vw[4] = {0, 0, 0, 0};  // 8 halves of k and v
     const int64_t where = at[key];
     if (where >= 0) {
-      const uint8_t* kr = c.values + where;
-      const uint8_t* vr = kr + c.kv_bytes;
-      const int pl = place[key];
+      const uint8_t* kr = c.data + where;
+      const uint8_t* vr = kr + 16 * kRow;
+      const int pl = place[key] & 15;
       if constexpr (kFmt == BQ4_CACHE_F16) {
         const uint4 a = *reinterpret_cast<const uint4*>(kr + cache_swizzle(0, kRow, pl, 16 * ch));
         const uint4 b = *reinterpret_cast<const uint4*>(vr + cache_swizzle(1, kRow, pl, 16 * ch));
@@ -240,7 +240,8 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
           }
         } else {
           const int blk = ch >> 2;
-          const uint32_t a = *reinterpret_cast<const uint32_t*>(kr + cache_swizzle(0, kRow, pl, 4 * ((ch & 3) * kNb + blk)));
+          const uint32_t a =
+              *reinterpret_cast<const uint32_t*>(kr + cache_swizzle(0, kRow, pl, 4 * ((ch & 3) * kNb + blk)));
           const float wk = sk[key][blk], wv = sv[key][blk] * unit;
           uint32_t b = 0;
 #pragma unroll

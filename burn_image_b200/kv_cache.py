@@ -47,9 +47,9 @@ class KVCache:
                  device: Optional[torch.device] = None):
         if format not in FORMATS:
             raise Bq4Error(L.EINVAL_ARG, f"format {format!r} is not one of {', '.join(FORMATS)}")
-        c = L.Cache(None, None, pages, page_size, kv_heads, head_dim, FORMATS[format], 0)
-        nv, ns = ctypes.c_size_t(), ctypes.c_size_t()
-        check(L.lib().bq4_cache_sizes(ctypes.byref(c), ctypes.byref(nv), ctypes.byref(ns)))
+        c = L.Cache(None, pages, page_size, kv_heads, head_dim, FORMATS[format], 0)
+        n = ctypes.c_size_t()
+        check(L.lib().bq4_cache_size(ctypes.byref(c), ctypes.byref(n)))
         dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         if dev.type != "cuda":
             raise Bq4Error(L.EINVAL_ARG, "a key/value cache lives on a CUDA device")
@@ -58,16 +58,15 @@ class KVCache:
         self.pages, self.page_size, self.format = pages, page_size, format
         self.kv_heads, self.head_dim = kv_heads, head_dim
         self.device, self._index = dev, dev.index
-        self.values = torch.zeros(nv.value, dtype=torch.uint8, device=dev)
-        self.scales = torch.zeros(ns.value, dtype=torch.uint8, device=dev)
-        c.values, c.scales, c.device = self.values.data_ptr(), self.scales.data_ptr() or None, dev.index
+        self.data = torch.zeros(n.value, dtype=torch.uint8, device=dev)
+        c.data, c.device = self.data.data_ptr(), dev.index
         self._workspace = {}  # bytes that an attention call of these sizes needs
         self._c = c
         self._ref = ctypes.byref(c)
 
     @property
     def device_bytes(self) -> int:
-        return self.values.numel() + self.scales.numel()
+        return self.data.numel()
 
     # The checks below run on every call of a decode loop: they take the common case first and
     # say what is wrong only when something is.

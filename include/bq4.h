@@ -586,17 +586,15 @@ BQ4_API bq4_status bq4_attention(const uint32_t* q, const uint32_t* k, const uin
  * quotient), qmax = 127 or 7; scale 0 gives q = 0.  A block with a non-finite
  * value gets the scale NaN and reads back as NaN.
  *
- * `values` and `scales` are device buffers of bq4_cache_sizes bytes on
- * `device`, 256-byte aligned (scales may be NULL for F16); what they hold is
- * read through the calls below.  A page holds page_size (a multiple of 16,
- * at most 65536) consecutive tokens of one sequence for every kv head;
- * head_dim is a multiple of 8 of at most 128 (rows are stored padded to 64 or
- * 128 values).
+ * `data` is a device buffer of bq4_cache_size bytes on `device`, 256-byte
+ * aligned; what it holds is read through the calls below.  A page holds
+ * page_size (a multiple of 16, at most 65536) consecutive tokens of one
+ * sequence for every kv head; head_dim is a multiple of 8 of at most 128 (rows
+ * are stored padded to 64 or 128 values).
  */
 typedef enum { BQ4_CACHE_F16 = 0, BQ4_CACHE_Q8 = 1, BQ4_CACHE_Q4 = 2 } bq4_cache_format;
 typedef struct {
-  void* values;
-  void* scales;
+  void* data;
   int64_t pages;
   int32_t page_size, kv_heads, head_dim;
   int32_t format; /* bq4_cache_format */
@@ -615,8 +613,8 @@ typedef struct {
   int64_t batch;
 } bq4_cache_sequences;
 
-/* Bytes of a cache's two buffers (its pointers and device are not read). */
-BQ4_API bq4_status bq4_cache_sizes(const bq4_cache* cache, size_t* values_bytes, size_t* scales_bytes);
+/* Bytes of a cache's buffer (its data and device are not read). */
+BQ4_API bq4_status bq4_cache_size(const bq4_cache* cache, size_t* bytes);
 
 /* Quantises the newest `tokens` rows of every sequence into the cache: row i
  * of sequence b goes to position lengths[b] - tokens + i (lengths count the

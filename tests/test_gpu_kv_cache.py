@@ -101,8 +101,7 @@ class Book:
         self.plen = torch.tensor([prefix], dtype=torch.int32, device=DEV)
         self.cache = KVCache(pages, page, Hkv, D, fmt, DEV)
         if poison:  # NaN in every place that a length leaves out
-            self.cache.values.view(torch.uint8).fill_(0xFF)
-            self.cache.scales.fill_(0xFF)
+            self.cache.data.fill_(0xFF)
         self.k, self.v = [], []
         for b, n in enumerate(lengths):
             k, v = self.rows(n, Hkv, D), self.rows(n, Hkv, D)
@@ -184,7 +183,7 @@ def test_strided_sources_and_untouched_rows(fmt):
     table = torch.tensor([[5, 0], [3, 1]], dtype=torch.int32, device=DEV)
     n = torch.tensor([18, 5], dtype=torch.int32, device=DEV)
     plain = KVCache(6, 16, H, D, fmt, DEV)
-    plain.values.fill_(0x5A), plain.scales.fill_(0x3C)
+    plain.data.fill_(0x5A)
     before = plain.read(torch.arange(6, dtype=torch.int32, device=DEV)[:, None], torch.full((6,), 16, dtype=torch.int32,
                                                                                            device=DEV), 16)
     plain.append(k.contiguous(), v.contiguous(), table, n)
@@ -192,9 +191,9 @@ def test_strided_sources_and_untouched_rows(fmt):
     turned = v.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
     for kk, vv in ((k, v), (odd, turned), (k.transpose(-1, -2).contiguous().transpose(-1, -2), v)):
         c = KVCache(6, 16, H, D, fmt, DEV)
-        c.values.fill_(0x5A), c.scales.fill_(0x3C)
+        c.data.fill_(0x5A)
         c.append(kk, vv, table, n)
-        assert torch.equal(c.values, plain.values) and torch.equal(c.scales, plain.scales)
+        assert torch.equal(c.data, plain.data)
     after = plain.read(torch.arange(6, dtype=torch.int32, device=DEV)[:, None], torch.full((6,), 16, dtype=torch.int32,
                                                                                           device=DEV), 16)
     touched = torch.zeros((6, 16), dtype=torch.bool, device=DEV)
@@ -350,7 +349,7 @@ def test_bad_pages_and_lengths_are_reported():
     ones = torch.ones((2, 32, 2, 128), device=DEV).half()
     c.append(ones, ones, good, i32(32, 32))
     q4.poll_device_error()
-    before = c.values.clone()
+    before = c.data.clone()
     for bad in (i32([4, 4], [-1, -1]), i32([2 ** 31 - 1, -2 ** 31], [4, 5])):
         c.append(x, x, bad, i32(20, 20))
         reported()
@@ -363,7 +362,7 @@ def test_bad_pages_and_lengths_are_reported():
         out = c.prefix_attention(q, bad[0], i32(32), good, i32(0, 32))
         reported()
         assert out[0].abs().sum() == 0 and torch.equal(out[1], torch.ones_like(out[1]))
-    assert torch.equal(c.values, before)
+    assert torch.equal(c.data, before)
     for n in (i32(33, 2), i32(-1, 2), i32(2 ** 31 - 1, 2)):
         c.read(good, n, 8)
         reported()
@@ -380,7 +379,7 @@ def test_cache_past_four_gib():
     # 5 GiB of pages: offsets of the last ones pass 32 bits
     pages, page, H, D = 20480, 64, 16, 128
     c = KVCache(pages, page, H, D, "q8", DEV)
-    assert c.values.numel() >= 2 ** 32 + 2 ** 30
+    assert c.data.numel() >= 2 ** 32 + 2 ** 30
     table = torch.tensor([[pages - 1, 3, pages - 2]], dtype=torch.int32, device=DEV)
     n = torch.tensor([150], dtype=torch.int32, device=DEV)
     g = torch.Generator(device=DEV).manual_seed(0)
@@ -395,7 +394,7 @@ def test_cache_past_four_gib():
     out = c.prefix_attention(q, table[0], n, table[:, :0], n * 0)
     check(out, *attend(q.double(), [held(k[0], "q8")[:0]], [held(v[0], "q8")[:0]], False, held(k[0], "q8"),
                        held(v[0], "q8")))
-    assert int(c.values.view(pages, -1).any(1).sum()) == 3  # nothing went to another page
+    assert int(c.data.view(pages, -1).any(1).sum()) == 3  # nothing went to another page
 
 
 # --------------------------------------------------------------------- in use

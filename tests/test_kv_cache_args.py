@@ -14,7 +14,7 @@ S3 = (ctypes.c_int64 * 3)(1024, 1024, 128)
 
 
 def cache(**kw):
-    f = dict(values=FAKE, scales=FAKE, pages=4, page_size=16, kv_heads=2, head_dim=128, format=L.CACHE_Q8, device=0)
+    f = dict(data=FAKE, pages=4, page_size=16, kv_heads=2, head_dim=128, format=L.CACHE_Q8, device=0)
     f.update(kw)
     return L.Cache(**f)
 
@@ -58,33 +58,31 @@ GEOMETRY = [(dict(format=3), L.EINVAL_ARG), (dict(format=-1), L.EINVAL_ARG), (di
 @pytest.mark.parametrize("change,status", GEOMETRY)
 def test_geometry_is_checked_by_every_call(change, status):
     c = cache(**change)
-    a, b = ctypes.c_size_t(), ctypes.c_size_t()
-    assert L.lib().bq4_cache_sizes(ctypes.byref(c), ctypes.byref(a), ctypes.byref(b)) == status
+    a = ctypes.c_size_t()
+    assert L.lib().bq4_cache_size(ctypes.byref(c), ctypes.byref(a)) == status
     assert append(c) == read(c) == attention(c) == prefix(c) == status
     assert L.lib().bq4_cache_attention_workspace_size(ctypes.byref(c), 1, 1, 4, 16, 0, ctypes.byref(a)) == status
 
 
-def test_sizes():
-    a, b = ctypes.c_size_t(), ctypes.c_size_t()
+def test_size():
+    a = ctypes.c_size_t()
     for fmt, dim, row, scales in ((L.CACHE_F16, 120, 256, 0), (L.CACHE_Q8, 128, 128, 1), (L.CACHE_Q8, 64, 64, 1),
                                   (L.CACHE_Q4, 128, 64, 4), (L.CACHE_Q4, 72, 64, 4), (L.CACHE_Q4, 40, 32, 2)):
-        c = cache(format=fmt, head_dim=dim, values=None, scales=None)
-        assert L.lib().bq4_cache_sizes(ctypes.byref(c), ctypes.byref(a), ctypes.byref(b)) == L.OK
-        assert (a.value, b.value) == (4 * 2 * 2 * 16 * row, 4 * 2 * 2 * 16 * scales * 2)
-    assert L.lib().bq4_cache_sizes(None, ctypes.byref(a), ctypes.byref(b)) == L.EINVAL_ARG
-    assert L.lib().bq4_cache_sizes(ctypes.byref(c), None, ctypes.byref(b)) == L.EINVAL_ARG
+        c = cache(format=fmt, head_dim=dim, data=None)
+        assert L.lib().bq4_cache_size(ctypes.byref(c), ctypes.byref(a)) == L.OK
+        assert a.value == 4 * 2 * 2 * 16 * (row + 2 * scales)
+    assert L.lib().bq4_cache_size(None, ctypes.byref(a)) == L.EINVAL_ARG
+    assert L.lib().bq4_cache_size(ctypes.byref(c), None) == L.EINVAL_ARG
     # 2^34 rows: past 32 bits
     c = cache(pages=1 << 20, page_size=4096, kv_heads=4)
-    assert L.lib().bq4_cache_sizes(ctypes.byref(c), ctypes.byref(a), ctypes.byref(b)) == L.OK
-    assert a.value == (1 << 32) * 4 * 2 * 128
+    assert L.lib().bq4_cache_size(ctypes.byref(c), ctypes.byref(a)) == L.OK
+    assert a.value == (1 << 32) * 4 * 2 * 130
 
 
 @pytest.mark.parametrize("call", [append, read, attention, prefix])
 def test_buffers_and_sequences_are_checked(call):
-    assert call(cache(values=None)) == L.EINVAL_ARG
-    assert call(cache(scales=None)) == L.EINVAL_ARG
-    assert call(cache(values=FAKE + 16)) == L.EALIGN
-    assert call(cache(scales=FAKE + 2)) == L.EALIGN
+    assert call(cache(data=None)) == L.EINVAL_ARG
+    assert call(cache(data=FAKE + 16)) == L.EALIGN
     assert call(s=seqs(lengths=None)) == L.EINVAL_ARG
     assert call(s=seqs(page_table=None)) == L.EINVAL_ARG
     assert call(s=seqs(lengths=FAKE + 2)) == L.EALIGN
