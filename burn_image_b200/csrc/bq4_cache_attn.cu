@@ -113,10 +113,14 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// CTAs of the split kernel that an SM holds.
+// CTAs of the split kernel that an SM holds: 384 threads leave 168 registers
+// each, 512 leave 128.  16 rows a warp spill a few at 168 and still gain (24
+// rows of 8 bits 32.0 -> 28.5 us against two CTAs of 255); 8 rows of 4 bits
+// keep their start values in registers at 168 (93.0 -> 91.3 us); f16's ring
+// allows three.
 constexpr int split_per_sm(int format, int hp, int nt) {
-  if (nt == 2) return hp == 64 ? 3 : 2;
-  return format == BQ4_CACHE_F16 && hp == 128 ? 3 : 4;
+  if (nt == 2) return 3;
+  return format != BQ4_CACHE_Q8 && hp == 128 ? 3 : 4;
 }
 
 // Sizes that follow from the format and the padded head.
@@ -138,7 +142,7 @@ struct Layout {
   static constexpr int kOffV = kStep * kRow;
   static constexpr int kOffS = 2 * kStep * kRow;
   static constexpr int kStage = kOffS + kStep * kScale;
-  // CTAs of an SM, by registers (512 threads of 128) and by the ring
+  // CTAs of an SM, by registers and by the ring
   static constexpr int per_sm(int nt) { return split_per_sm(kFmt, kHP, nt); }
   static constexpr int kRing = (per_sm(1) == 3 ? 72 : 54) * 1024;  // bytes, about
   static constexpr int kStages = kRing / (kSWarps * kStage) < 8 ? kRing / (kSWarps * kStage) : 8;
