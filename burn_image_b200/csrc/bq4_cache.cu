@@ -193,42 +193,44 @@ __global__ void __launch_bounds__(kCThreads) cache_append_kernel(const __grid_co
         if (live) store_words<2 * kW>(dst(2 * d0), w);
       } else {
         constexpr float kTop = kFmt == BQ4_CACHE_Q8 ? 127.0f : 7.0f;
-        float top = 0.0f;
-        bool odd = false;
+        // magnitudes as their bits, which order like them, infinities and NaN on top
+        uint32_t most = 0;
 #pragma unroll
-        for (int e = 0; e < kW; ++e) {
-          top = fmaxf(top, fabsf(x[e]));
-          odd |= !(fabsf(x[e]) <= 3.402823466e38f);
-        }
-        if (odd) top = INFINITY;  // infinities and NaN
+        for (int e = 0; e < kW; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
 #pragma unroll
         for (int o = (kFmt == BQ4_CACHE_Q8 ? kLanes : kCacheBlock / kW) >> 1; o; o >>= 1)
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
         // f32 quotients, rounded to nearest: the scale and every q follow from the
         // definition bit for bit.
-        const __nv_bfloat16 sb = __float2bfloat16_rn(top == INFINITY ? __int_as_float(0x7fc00000)
-                                                                     : __fdiv_rn(top, kTop));
+        const float top = __uint_as_float(most);
+        const __nv_bfloat16 sb =
+            __float2bfloat16_rn(most >= 0x7f800000u ? __int_as_float(0x7fc00000) : __fdiv_rn(top, kTop));
         const float s = __bfloat162float(sb);
-        uint32_t q[kW];  // u = q + 128 or q + 8
-        // x (1 / s) is the quotient but for three roundings, 2^-22 of at most 2^7.1: where it lies
-        // 2^-14 or more from a half, both round to the same whole number.  The divisions are
-        // left for a lane that holds another one, and for scales whose inverse is not normal.
+        // x (1 / s) is the quotient but for three roundings, 2^-22 of at most kTop (1 + 2^-9):
+        // where it lies 2^-14 or more from a half, both round to the same whole number, which
+        // needs no clamping.  The divisions are left for a lane that holds another one, and for
+        // scales whose inverse is not normal.  y + 1.5 2^23 rounds y to a whole number in the
+        // low bits of the sum.
+        constexpr float kRound = 12582912.0f;
+        constexpr uint32_t kZero = kFmt == BQ4_CACHE_Q8 ? 128 : 8;
         const float inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
-        bool near = s > 0.0f && !(s >= 0x1p-120f && s <= 0x1p120f);
-        float whole[kW];
+        uint32_t q[kW];  // u = q + 128 or q + 8
+        float far = s > 0.0f && !(s >= 0x1p-120f && s <= 0x1p120f) ? 1.0f : 0.0f;
 #pragma unroll
         for (int e = 0; e < kW; ++e) {
-          const float y = x[e] * inv;
-          whole[e] = rintf(y);
-          near |= fabsf(y - whole[e]) > 0.5f - 0x1p-14f;
+          const float y = x[e] * inv, t = y + kRound;
+          q[e] = __float_as_uint(t) - (__float_as_uint(kRound) - kZero);
+          far = fmaxf(far, fabsf(y - (t - kRound)));
         }
-        if (near) {
+        if (far > 0.5f - 0x1p-14f) {
 #pragma unroll
-          for (int e = 0; e < kW; ++e) whole[e] = rintf(__fdiv_rn(x[e], s));
+          for (int e = 0; e < kW; ++e)
+            q[e] = (uint32_t)((int)fminf(fmaxf(rintf(__fdiv_rn(x[e], s)), -kTop), kTop) + (int)kZero);
         }
+        if (!(s > 0.0f)) {  // a scale of 0, or NaN
 #pragma unroll
-        for (int e = 0; e < kW; ++e)
-          q[e] = (uint32_t)((int)fminf(fmaxf(whole[e], -kTop), kTop) + (kFmt == BQ4_CACHE_Q8 ? 128 : 8));
+          for (int e = 0; e < kW; ++e) q[e] = kZero;
+        }
         if constexpr (kFmt == BQ4_CACHE_Q8) {
           uint32_t w[kW / 4];
 #pragma unroll
@@ -341,11 +343,12 @@ __global__ void __launch_bounds__(kCThreads) cache_read_kernel(const __grid_cons
         if constexpr (kFmt == BQ4_CACHE_F16) {
           x[e] = __half2float(__ushort_as_half((unsigned short)(held[j][e >> 1] >> 16 * (e & 1))));
         } else if constexpr (kFmt == BQ4_CACHE_Q8) {
-          x[e] = (float)((int)(held[j][e >> 2] >> 8 * (e & 3) & 255) - 128) * s;
+          // byte u under the exponent of 2^23: 2^23 + u, exactly
+          x[e] = (__uint_as_float(__byte_perm(held[j][e >> 2], 0x4b000000u, 0x7540 + (e & 3))) - 8388736.0f) * s;
         } else {
           const int o = kW == 4 ? 4 * (L & 1) + e : e;
           const int nibble = kv == 0 ? 4 * (o >> 1) + 16 * (o & 1) : 4 * e;
-          x[e] = (float)((int)(held[j][0] >> nibble & 15) - 8) * s;
+          x[e] = (__uint_as_float((held[j][0] >> nibble & 15) | 0x4b000000u) - 8388616.0f) * s;
         }
       }
       const bool live = page >= 0 && base + row < end;

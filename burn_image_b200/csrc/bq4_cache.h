@@ -106,7 +106,8 @@ struct CacheTilePlan {
 };
 bool plan_cache_tile(const CacheAttnCall& a, bool prefix, int sms, CacheTilePlan* p);
 // finish: there is one chunk and no other source, and the rows are finished.
-bq4_status run_cache_tile(const CacheAttnCall& a, const CacheTilePlan& p, bool finish, void* workspace,
+// beside: the kernel before on the stream is independent, and may run at the same time.
+bq4_status run_cache_tile(const CacheAttnCall& a, const CacheTilePlan& p, bool finish, bool beside, void* workspace,
                           CacheJoinSource* source, cudaStream_t stream);
 
 bq4_status cache_attn_workspace(const CacheAttnCall& c, int sms, size_t* bytes);

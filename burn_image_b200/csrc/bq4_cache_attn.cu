@@ -1059,21 +1059,25 @@ bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, cuda
   g.group = a.q_heads / a.c.kv_heads;
   g.have_p = a.prefix_length && a.prefix_width > 0;
   const bool alone = !p.tile_p;  // the split kernel has every source, or there is one
-  if (p.tile_p) {
-    st = run_cache_tile(a, p.p, false, ws, &g.p, stream);
-    if (st) return st;
-    ws += p.p.workspace_bytes;
-  }
-  if (p.tile_s) {
-    const bool finish = alone && p.s.chunks == 1;
-    st = run_cache_tile(a, p.s, finish, ws, &g.s, stream);
-    if (st || finish) return st;
-  } else {
+  if (!p.tile_s) {
     g.finish = alone;
     CacheJoinSource gp = {};
     st = run_split(p.call, p.split, alone, ws, &gp, &g.s, stream);
     if (st) return st;
     if (alone) g.p = gp;
+    ws += p.split_bytes;
+  }
+  if (p.tile_p) {
+    // the prefix's keys are widened while the sequences' own CTAs end: 128 sequences behind 16384
+    // rows 99 -> 95 us
+    st = run_cache_tile(a, p.p, false, !p.tile_s, ws, &g.p, stream);
+    if (st) return st;
+    ws += p.p.workspace_bytes;
+  }
+  if (p.tile_s) {
+    const bool finish = alone && p.s.chunks == 1;
+    st = run_cache_tile(a, p.s, finish, false, ws, &g.s, stream);
+    if (st || finish) return st;
   }
   // the join is launched ahead and waits on the device for the partial results
   cudaLaunchConfig_t cfg = {};

@@ -127,6 +127,8 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
       }
       *reinterpret_cast<uint4*>(dst + (ch >> 3) * (128 * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = u;
     }
+    // this grid does not end before the one that it was launched beside
+    if (blockIdx.x == gridDim.x - 1) ptx::griddep_wait();
     return;
   }
 
@@ -667,11 +669,17 @@ cudaError_t launch_tile(const TileArgs& s, unsigned grid, cudaStream_t stream) {
 }
 
 template <int kFmt>
-void launch_widen(const TileArgs& s, unsigned grid, cudaStream_t stream) {
-  if (s.a.c.hp == 64)
-    cache_widen_kernel<kFmt, 64><<<grid, 256, 0, stream>>>(s);
-  else
-    cache_widen_kernel<kFmt, 128><<<grid, 256, 0, stream>>>(s);
+cudaError_t launch_widen(const TileArgs& s, unsigned grid, bool beside, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = beside ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, s.a.c.hp == 64 ? cache_widen_kernel<kFmt, 64> : cache_widen_kernel<kFmt, 128>, s);
 }
 
 }  // namespace
@@ -711,7 +719,7 @@ bool plan_cache_tile(const CacheAttnCall& a, bool prefix, int sms, CacheTilePlan
   return heads * tiles * p->chunks <= 0x7fffffff && p->records + p->q_tiles <= 0x7fffffff;
 }
 
-bq4_status run_cache_tile(const CacheAttnCall& a, const CacheTilePlan& p, bool finish, void* workspace,
+bq4_status run_cache_tile(const CacheAttnCall& a, const CacheTilePlan& p, bool finish, bool beside, void* workspace,
                           CacheJoinSource* source, cudaStream_t stream) {
   TileArgs s;
   s.a = a;
@@ -736,14 +744,10 @@ bq4_status run_cache_tile(const CacheAttnCall& a, const CacheTilePlan& p, bool f
   s.part = reinterpret_cast<float*>(s.q + p.q_bytes);
   s.ml = reinterpret_cast<float2*>(s.q + p.q_bytes + p.part_bytes);
   const unsigned widen = (unsigned)(p.records + p.q_tiles);
-  if (a.c.format == BQ4_CACHE_F16)
-    launch_widen<BQ4_CACHE_F16>(s, widen, stream);
-  else if (a.c.format == BQ4_CACHE_Q8)
-    launch_widen<BQ4_CACHE_Q8>(s, widen, stream);
-  else
-    launch_widen<BQ4_CACHE_Q4>(s, widen, stream);
+  cudaError_t e = a.c.format == BQ4_CACHE_F16  ? launch_widen<BQ4_CACHE_F16>(s, widen, beside, stream)
+                  : a.c.format == BQ4_CACHE_Q8 ? launch_widen<BQ4_CACHE_Q8>(s, widen, beside, stream)
+                                               : launch_widen<BQ4_CACHE_Q4>(s, widen, beside, stream);
   note_launch();
-  cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return check_cuda(e, "cache widening launch");
   const unsigned grid = (unsigned)((int64_t)p.sets * p.tiles * a.c.kv_heads * p.chunks);
   e = a.c.hp == 64 ? launch_tile<64>(s, grid, stream) : launch_tile<128>(s, grid, stream);
