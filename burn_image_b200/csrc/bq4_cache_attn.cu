@@ -40,11 +40,11 @@
 //     2^-24, left values of q = 0 up to 2^-17 of the offset away from 0).
 //   * k scales multiply the f32 scores.  v scales multiply the probabilities,
 //     p s_v as f16 (off by 2^-11 of it; the only rounding to fewer than 32 bits
-//     besides the result's).  To keep it in f16's range p is 2^(x - base), base
-//     being the running maximum of x plus log2 of a power of two above the v
-//     scales so far, less 6; l and O are both relative to base.
-//   * base only moves when some p s_v could pass 2^14 (a vote, no shuffles in
-//     the common step), and then 2^8 down at least.
+//     besides the result's).  To fill f16's range p is 2^(x - base), where base
+//     is 2^6 below the running maximum of s_v 2^x; l and O are both relative to
+//     it.
+//   * base only moves when some p s_v would pass 2^14 (a vote, no shuffles in
+//     the common step).
 //   * Steps that every row sees whole run without any mask.
 //
 // What bounds it: HBM for a few rows (each byte of the chunk is read once),
@@ -86,6 +86,12 @@ __device__ __forceinline__ void lds(uint32_t at, uint32_t (&w)[kWords]) {
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -414,11 +420,7 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
     see_all = min(see_all, __shfl_xor_sync(0xffffffffu, see_all, 2));
     plain = min(plain, max(0, (see_all - at0 + kUnit - kStep) / kUnit));
 
-    // p = 2^(x - base): with vs a power of two above the v scales so far and m the maximum of x so
-    // far, base = m + log2(vs) - kHead when it moves, so that p s_v stays below 2^kJump.  l and O
-    // are both relative to it.
-    float base[kNT][2], l[kNT][2], o[kNT][Y::kMT][4];
-    float vs = Y::kQ ? 0x1p-100f : 1.0f, jump = Y::kQ ? kJump + 100.0f : kJump;  // jump = kJump - log2(vs)
+    float base[kNT][2], l[kNT][2], o[kNT][Y::kMT][4];  // p = 2^(x - base)
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
       base[nt][0] = base[nt][1] = kNone;
@@ -532,6 +534,18 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
 
       // ---- z = x - base, x in log2 units; a masked key's is -inf
       const float c0 = kFmt == BQ4_CACHE_Q8 ? sk[0][0] * c : c, c1 = kFmt == BQ4_CACHE_Q8 ? sk[1][0] * c : c;
+      // log2 of the keys' largest v scales; not below -100, so that p stays in f32's range beside
+      // a v of 0
+      float lg[2] = {0.0f, 0.0f};
+      if constexpr (Y::kQ) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float top = sv[r][0];
+#pragma unroll
+          for (int e = 1; e < Y::kNb; ++e) top = fmaxf(top, sv[r][e]);
+          lg[r] = fmaxf(lg2(top), -100.0f);
+        }
+      }
       float z[kNT][4];
       bool move = false;
 #pragma unroll
@@ -541,26 +555,9 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
           z[nt][u] = fmaf(x[nt][u], u < 2 ? c0 : c1, -base[nt][u & 1]);
           if (kEdge && limit[nt][u & 1] <= 8 * (u >> 1)) z[nt][u] = -INFINITY;
         }
-        move |= fmaxf(fmaxf(z[nt][0], z[nt][1]), fmaxf(z[nt][2], z[nt][3])) > jump;
-      }
-      [[maybe_unused]] float sv_top = 0.0f;
-      if constexpr (Y::kQ) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int e = 0; e < Y::kNb; ++e) sv_top = fmaxf(sv_top, sv[r][e]);
-        move |= sv_top > vs;
+        move |= fmaxf(fmaxf(z[nt][0], z[nt][1]) + lg[0], fmaxf(z[nt][2], z[nt][3]) + lg[1]) > kJump;
       }
       if (__any_sync(0xffffffffu, move)) {
-        if constexpr (Y::kQ) {
-#pragma unroll
-          for (int w = 4; w < 32; w <<= 1) sv_top = fmaxf(sv_top, __shfl_xor_sync(0xffffffffu, sv_top, w));
-          if (sv_top > vs) {  // (held in [2^-100, 2^100]: p must not leave f32's range)
-            const int e = min(max((int)(__float_as_uint(sv_top) >> 23) - 126, -100), 100);
-            vs = __uint_as_float((uint32_t)(127 + e) << 23);
-            jump = kJump - (float)e;
-          }
-        }
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
@@ -568,14 +565,13 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
             float x0 = x[nt][e] * c0, x1 = x[nt][e + 2] * c1;
             if (kEdge && limit[nt][e] <= 0) x0 = -INFINITY;
             if (kEdge && limit[nt][e] <= 8) x1 = -INFINITY;
-            float top = fmaxf(x0, x1);
+            float top = fmaxf(x0 + lg[0], x1 + lg[1]);
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
             float alpha = 1.0f;
-            if (top - base[nt][e] > jump) {
-              const float next = top - (jump - (kJump - kHead));
-              alpha = ex2(base[nt][e] - next);
-              base[nt][e] = next;
+            if (top - base[nt][e] > kJump) {
+              alpha = ex2(base[nt][e] - (top - kHead));
+              base[nt][e] = top - kHead;
             }
             z[nt][e] = x0 - base[nt][e];
             z[nt][e + 2] = x1 - base[nt][e];

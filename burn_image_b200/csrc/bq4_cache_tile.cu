@@ -26,8 +26,8 @@
 //   warp 1        S_t = q_t k^T and O_t += P_t v for the two 128-row tiles in
 //                 turn, so that one tile's softmax runs beside the other's products
 //   warps 4..11   a thread a row: y = S ck (+ lv), p = 2^(y + e - m) as f16 into
-//                 TMEM, l += p 2^-e; O is rescaled only when the maximum of
-//                 y + e passes m by 2^8
+//                 TMEM, l += p 2^-e; O is rescaled only when some p would
+//                 pass 2^14
 // Every wait is bounded (BQ4_ETIMEOUT), as in bq4_attn_fused.cu.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -47,7 +47,10 @@ constexpr int kTThreads = 384;
 constexpr int kRing = 2;                     // stages of k and of v
 constexpr uint32_t kConsts = kKeys * 8 + 16;  // bytes of a record's consts
 constexpr float kTNone = -1e30f;             // the maximum of no score
-constexpr float kTJump = 8.0f;               // log2 units: p <= 2^8 fits f16
+// log2 units: m is set 2^6 below the maximum and moves when p would pass 2^14, so
+// that f16 holds p to its 2^-11 down to 2^-20 of the row's largest (a small p
+// may meet a large v)
+constexpr float kTHead = 6.0f, kTJump = 14.0f;
 
 struct Consts {
   float ck[kKeys], lv[kKeys];
@@ -566,7 +569,7 @@ __global__ void __launch_bounds__(kTThreads, 1) cache_tile_kernel(const __grid_c
       attn_ld64(t_s + 64, r);  // kept for the P pass
       top = fmaxf(top, plain ? scores64<true>(r, k, 64, valid) : scores64<false>(r, k, 64, valid)) + e;
       const bool jump = top > m + kTJump;
-      const float m_use = jump ? top : m;
+      const float m_use = jump ? top - kTHead : m;
       const float alpha = jump ? attn_ex2(m - m_use) : 1.0f;
       if (j > 0 && __any_sync(0xffffffffu, jump)) {
         // O_t holds P_t(j-1) v_{j-1} (s_full's commit for S_t(j) covered it)

@@ -60,7 +60,8 @@ class KVCache:
         self.device, self._index = dev, dev.index
         self.data = torch.zeros(n.value, dtype=torch.uint8, device=dev)
         c.data, c.device = self.data.data_ptr(), dev.index
-        self._workspace = {}  # bytes that an attention call of these sizes needs
+        self._plans = {}  # of attention calls, by their sizes
+        self._lib = L.lib()
         self._c = c
         self._ref = ctypes.byref(c)
 
@@ -83,7 +84,7 @@ class KVCache:
         if n != b or (batch is not None and batch != b):
             raise Bq4Error(L.EINVAL_SHAPE, f"page_table holds {b} sequences, lengths {n}"
                            + (f", the rows {batch}" if batch is not None else ""))
-        return L.CacheSequences(page_table.data_ptr() or None, ts, w, lengths.data_ptr() or None, b)
+        return L.CacheSequences(page_table.data_ptr(), ts, w, lengths.data_ptr(), b)
 
     def _ints(self, t: torch.Tensor, what: str) -> torch.Tensor:
         if t.dtype is not torch.int32 or t.device != self.device or t.dim() != 1 \
@@ -112,9 +113,9 @@ class KVCache:
         if v.shape != k.shape or v.dtype != k.dtype:
             raise Bq4Error(L.EINVAL_SHAPE, "key and value must have one shape and type")
         seqs = self._sequences(page_table, lengths, k.shape[0])
-        check(L.lib().bq4_cache_append(self._ref, ctypes.byref(seqs), k.data_ptr() or None, _Strides(*k.stride()[:3]),
-                                       v.data_ptr() or None, _Strides(*v.stride()[:3]), _DTYPES[k.dtype], k.shape[1],
-                                       _raw_stream(self._index)))
+        check(self._lib.bq4_cache_append(self._ref, ctypes.byref(seqs), k.data_ptr(), _Strides(*k.stride()[:3]),
+                                         v.data_ptr(), _Strides(*v.stride()[:3]), _DTYPES[k.dtype], k.shape[1],
+                                         _raw_stream(self._index)))
 
     def read(self, page_table: torch.Tensor, lengths: torch.Tensor, count: int,
              starts: Optional[torch.Tensor] = None,
@@ -133,9 +134,9 @@ class KVCache:
         H, D = self.kv_heads, self.head_dim
         k = page_table.new_empty((seqs.batch, H, count, D), dtype=dtype)
         v = torch.empty_like(k)
-        check(L.lib().bq4_cache_read(self._ref, ctypes.byref(seqs), starts.data_ptr() if starts is not None else None,
-                                     count, k.data_ptr() or None, v.data_ptr() or None,
-                                     _Strides(H * count * D, count * D, D), _DTYPES[dtype], _raw_stream(self._index)))
+        check(self._lib.bq4_cache_read(self._ref, ctypes.byref(seqs), starts.data_ptr() if starts is not None else None,
+                                       count, k.data_ptr(), v.data_ptr(), _Strides(H * count * D, count * D, D),
+                                       _DTYPES[dtype], _raw_stream(self._index)))
         return k, v
 
     def attention(self, query: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, causal: bool = True,
@@ -167,35 +168,41 @@ class KVCache:
 
     def _attention(self, query, prefix_pages, prefix_length, page_table, lengths, causal, scale, max_length, out):
         q = self._rows(query, "query", None)
-        if q.dtype != torch.float16:
+        if q.dtype is not torch.float16:
             raise Bq4Error(L.EINVAL_ARG, "query must be float16")
-        B, S, Hq, D = q.shape
-        seqs = self._sequences(page_table, lengths, B)
+        shape = q.shape
+        seqs = self._sequences(page_table, lengths, shape[0])
+        plain = q.is_contiguous()
         if out is None:
-            out = q.new_empty((B, S, Hq, D))
-        elif out.shape != q.shape or out.dtype != torch.float16 or out.device != self.device or not out.is_contiguous():
-            raise Bq4Error(L.EINVAL_ARG, f"out must be contiguous float16 {tuple(q.shape)} on {self.device}")
-        held = seqs.table_width * self.page_size
+            out = torch.empty_like(q) if plain else q.new_empty(shape)
+        elif out.shape != shape or out.dtype != torch.float16 or out.device != self.device or not out.is_contiguous():
+            raise Bq4Error(L.EINVAL_ARG, f"out must be contiguous float16 {tuple(shape)} on {self.device}")
+        width = prefix_pages.shape[0] if prefix_pages is not None else 0
+        key = (shape, seqs.table_width, width, max_length)
+        plan = self._plans.get(key) or self._plan(key)
+        longest, nbytes, strides = plan
+        # a workspace of the call's own: calls on several streams, and graphs captured side by side, never share one
+        ws = q.new_empty(nbytes // 2)
+        tail = (q.data_ptr(), strides if plain else _Strides(*q.stride()[:3]), shape[1], shape[2], causal, scale or 0.0,
+                out.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(self._index))
+        if prefix_pages is None:
+            check(self._lib.bq4_cache_attention(self._ref, ctypes.byref(seqs), longest, *tail))
+        else:
+            check(self._lib.bq4_cache_prefix_attention(self._ref, prefix_pages.data_ptr(), width,
+                                                       prefix_length.data_ptr(), ctypes.byref(seqs), longest, *tail))
+        return out
+
+    def _plan(self, key):
+        """Bound of the lengths, workspace bytes and contiguous strides of an attention call of these sizes."""
+        (B, S, Hq, D), table_width, width, max_length = key
+        held = table_width * self.page_size
         longest = held if max_length is None else max_length
         if longest < 0:
             raise Bq4Error(L.EINVAL_SHAPE, f"max_length={max_length}")
-        width = prefix_pages.shape[0] if prefix_pages is not None else 0
-        lib = L.lib()
-        sizes = (B, S, Hq, min(longest, held) or held, width * self.page_size)
-        nbytes = self._workspace.get(sizes)
-        if nbytes is None:
-            n = ctypes.c_size_t()
-            check(lib.bq4_cache_attention_workspace_size(self._ref, *sizes, ctypes.byref(n)))
-            if len(self._workspace) >= 1024:
-                self._workspace.clear()
-            nbytes = self._workspace[sizes] = n.value
-        # a workspace of the call's own: calls on several streams, and graphs captured side by side, never share one
-        ws = q.new_empty(nbytes // 2) if nbytes else None
-        tail = (q.data_ptr() or None, _Strides(*q.stride()[:3]), S, Hq, 1 if causal else 0, scale or 0.0,
-                out.data_ptr() or None, ws.data_ptr() if ws is not None else None, nbytes, _raw_stream(self._index))
-        if prefix_pages is None:
-            check(lib.bq4_cache_attention(self._ref, ctypes.byref(seqs), longest, *tail))
-        else:
-            check(lib.bq4_cache_prefix_attention(self._ref, prefix_pages.data_ptr() or None, width,
-                                                 prefix_length.data_ptr(), ctypes.byref(seqs), longest, *tail))
-        return out
+        n = ctypes.c_size_t()
+        check(self._lib.bq4_cache_attention_workspace_size(self._ref, B, S, Hq, min(longest, held) or held,
+                                                           width * self.page_size, ctypes.byref(n)))
+        if len(self._plans) >= 1024:
+            self._plans.clear()
+        plan = self._plans[key] = (longest, n.value, _Strides(S * Hq * D, Hq * D, D))
+        return plan

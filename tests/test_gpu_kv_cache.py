@@ -18,6 +18,9 @@ factor 1 + e.  A score is at most SCORE in size (asserted) with sums of |q k|
 at most 8 SCORE, over at most 32 roundings of 2^-24: e <= 2^-16 SCORE for the
 numerator, the same for the sum; plus 2^-14 for the exponential, the online
 rescalings and f32 sums of up to 2^10 steps of 2^-24.
+Calls of 64 rows a kv head and more on 256 keys and more also round the widened
+v of an 8-bit cache to f16 (at most half a step, 2^-11 of each value): where
+`staged` is given, another 2^-11 a.
 """
 import math
 
@@ -76,9 +79,10 @@ def attend(q, ks, vs, causal, pk=None, pv=None, scale=None):
     return out, mag, top
 
 
-def check(got, exact, mag, top):
+def check(got, exact, mag, top, staged=False):
     q4.poll_device_error()
-    tol = 2.0 ** -11 * exact.abs() + (2.0 ** -11 + 2.0 ** -15 * top + 2.0 ** -14) * mag + 2.0 ** -25
+    rounded = 2.0 ** -10 if staged else 2.0 ** -11
+    tol = 2.0 ** -11 * exact.abs() + (rounded + 2.0 ** -15 * top + 2.0 ** -14) * mag + 2.0 ** -25
     err = (got.double() - exact).abs()
     assert not got.isnan().any()
     worst = (err / tol).max().item() if err.numel() else 0.0
@@ -333,6 +337,91 @@ def test_masked_nan_and_held_nan():
     check(out[:, :1], *exact)           # query 0 sees 19 rows
 
 
+@pytest.mark.parametrize("fmt", ["f16", "q8", "q4"])
+@pytest.mark.parametrize("page", [16, 48, 4096])
+def test_prefix_and_own_keys_both_long(fmt, page):
+    # 160 rows of each sequence and 480 of the batch on hundreds of keys: both by the many-row kernels
+    book = Book(fmt, [700, 263, 39], 2, 128, page, prefix=600, seed=page, poison=True)
+    q = book.query(40, 8)
+    for causal in (True, False):
+        got = book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths, causal=causal)
+        check(got, *attend(q.double(), book.k, book.v, causal, book.pk, book.pv), staged=True)
+    got = book.cache.attention(q, book.table, book.lengths)
+    check(got, *attend(q.double(), book.k, book.v, True), staged=True)
+    for _ in range(3):
+        assert torch.equal(got, book.cache.attention(q, book.table, book.lengths))
+    odd = torch.zeros((3, 40, 8, 129), dtype=torch.float16, device=DEV)[..., 1:]
+    odd.copy_(q)  # rows on no 16-byte boundary
+    assert torch.equal(got, book.cache.attention(odd, book.table, book.lengths))
+
+
+@pytest.mark.parametrize("fmt", ["q8", "q4", "f16"])
+def test_many_rows_with_rows_of_any_size(fmt):
+    # k from 2^-30 to 2^4 and v from 2^-12 to 2^17 (f32 rows; f16 caches hold up to 2^15): the
+    # widened tiles keep them in f16's range by factors of two
+    n, S = 600, 20
+    book = Book(fmt, [n], 1, 128, 64, seed=21)
+    g = book.g
+    k = torch.randn((n, 1, 128), generator=g, device=DEV) * 2.0 ** torch.randint(-30, 3, (n, 1, 1), generator=g, device=DEV)
+    hi = 15 if fmt == "f16" else 18
+    v = torch.randn((n, 1, 128), generator=g, device=DEV).clamp(-1.9, 1.9) * \
+        2.0 ** torch.randint(-12, hi - 1, (n, 1, 1), generator=g, device=DEV)
+    book.cache.append(k[None], v[None], book.table, book.lengths)
+    hk, hv = held(k, fmt), held(v, fmt)
+    for Hq in (4, 1):  # 80 rows, then 20 (the few-row kernel)
+        q = torch.randn((1, S, Hq, 128), generator=g, device=DEV).half()
+        got = book.cache.attention(q, book.table, book.lengths)
+        exact, mag, top = attend(q.double(), [hk], [hv], True)
+        fits = exact.abs() < 65504
+        assert fits.float().mean() > 0.9
+        zero = torch.zeros((), dtype=torch.float64, device=DEV)
+        # rows a factor 2^20 below the block's largest are rounded to steps of 2^-25 of 2^15
+        check(torch.where(fits, got.double(), zero), torch.where(fits, exact, zero), mag, top, staged=True)
+
+
+def test_many_rows_with_nan_and_bad_pages():
+    n, S = 400, 30
+    for fmt in ("f16", "q8", "q4"):
+        book = Book(fmt, [n, n], 1, 128, 16, seed=31, poison=True)
+        q = book.query(S, 4)
+        want = book.cache.attention(q, book.table, book.lengths)
+        # the newest row but 9 gets a NaN v: queries before it do not see it
+        x = torch.ones((1, 1, 1, 128), device=DEV).half()
+        bad = x.clone()
+        bad[0, 0, 0, 77] = math.nan
+        at = torch.tensor([n - 9], dtype=torch.int32, device=DEV)
+        book.cache.append(x, bad, book.table[:1], at)
+        got = book.cache.attention(q, book.table, book.lengths)
+        q4.poll_device_error()
+        assert torch.equal(got[1], want[1]) and torch.equal(got[0, :S - 10], want[0, :S - 10])
+        assert got[0, S - 10:, :, 77].isnan().all()
+        # a page outside the cache holds nothing: the rest is as without its rows
+        table = book.table.clone()
+        table[1, 3] = 10 ** 6
+        got = book.cache.attention(q[1:], table[1:], book.lengths[1:])
+        reported()
+        keep = [i for i in range(n) if i // 16 != 3]
+        k, v = book.k[1][keep], book.v[1][keep]
+        check(got, *attend(q[1:].double(), [k], [v], True), staged=True)
+
+
+def test_more_sequences_than_threads():
+    # 300 sequences, most of them empty or short, in one line of work
+    lengths = [(7 * i) % 90 if i % 3 else 0 for i in range(300)]
+    book = Book("q8", [max(lengths)], 2, 64, 16, seed=41)
+    n = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    table = book.table.expand(300, -1)  # every sequence reads the same pages, to its own length
+    q = torch.randn((300, 1, 4, 64), generator=book.g, device=DEV).half()
+    got = book.cache.attention(q, table, n)
+    ks, vs = [book.k[0][:x] for x in lengths], [book.v[0][:x] for x in lengths]
+    check(got, *attend(q.double(), ks, vs, True))
+    q = torch.randn((300, 33, 4, 64), generator=book.g, device=DEV).half()  # 66 rows: the bound of the lengths decides
+    wide = torch.cat([book.table] * 5, 1).expand(300, -1)
+    got = book.cache.attention(q, wide, n)
+    check(got, *attend(q.double(), ks, vs, True), staged=True)
+    assert torch.equal(got, book.cache.attention(q, wide, n))
+
+
 # --------------------------------------------------------------------- bad pages, long caches
 
 def reported():
@@ -494,6 +583,29 @@ def test_streams_and_graphs():
         assert torch.equal(out, want)
         check(out2, *attend(q.double(), ks, vs, True, book.pk, book.pv))
     q4.poll_device_error()
+
+
+def test_many_rows_in_a_graph():
+    book = Book("q4", [500, 300], 2, 128, 16, prefix=400, seed=13)
+    c, S = book.cache, 24
+    q = book.query(S, 8)
+    lengths = book.lengths.clone()
+    c.prefix_attention(q, book.ptable, book.plen, book.table, lengths)
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        out = c.prefix_attention(q, book.ptable, book.plen, book.table, lengths)
+        own = c.attention(q, book.table, lengths)
+    for less in (0, 111, 300):
+        lengths.copy_(book.lengths - less)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        torch.cuda.synchronize()
+        ks = [x[:x.shape[0] - less] for x in book.k]
+        vs = [x[:x.shape[0] - less] for x in book.v]
+        check(out, *attend(q.double(), ks, vs, True, book.pk, book.pv), staged=True)
+        check(own, *attend(q.double(), ks, vs, True), staged=True)
 
 
 def test_same_bits_every_time():
