@@ -55,6 +55,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cstdlib>
 #include <type_traits>
 
 #include "bq4_cache.h"
@@ -124,11 +125,12 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 }
 
 // CTAs of the split kernel that an SM holds: 384 threads leave 168 registers
-// each, 512 leave 128.  16 rows a warp spill a few at 168 and still gain (24
-// rows of 8 bits 32.0 -> 28.5 us against two CTAs of 255); 8 rows of 4 bits
-// keep their start values in registers at 168 (93.0 -> 91.3 us); f16's ring
-// allows three.
+// each, 512 leave 128.  16 rows a warp spill a few at 168 and still gain (a
+// draft of 24 rows, 8 bits, 32.0 -> 28.5 us against two CTAs of 255); 8 rows of
+// 4 bits keep their start values in registers at 168 (93.0 -> 91.3 us); f16's
+// ring allows three; 24 rows need 255.
 constexpr int split_per_sm(int format, int hp, int nt) {
+  if (nt == 3) return 2;
   if (nt == 2) return 3;
   return format != BQ4_CACHE_Q8 && hp == 128 ? 3 : 4;
 }
@@ -907,13 +909,23 @@ struct SplitPlan {
   size_t part_bytes, ml_bytes, pieces_bytes;
 };
 
+// Rows of a warp, in eights: a step costs about as much for its widening as for
+// 16 rows, so the tiles are those that cost least together (24 rows as one tile
+// 25.5 us, as two of 16 27.1).
+int row_tile(int64_t rows) {
+  int best = 1;
+  for (int nt = 2; nt <= 3; ++nt)
+    if ((rows + 8 * nt - 1) / (8 * nt) * (2 + nt) < (rows + 8 * best - 1) / (8 * best) * (2 + best)) best = nt;
+  return best;
+}
+
 // CTAs: what the GPU holds at a time, or fewer where the lengths' bounds give
 // fewer units.
 bool plan_split(const CacheAttnCall& a, int sms, SplitPlan* p) {
   const int group = a.q_heads / a.c.kv_heads;
   const int64_t own = (int64_t)a.tokens * group, all = own * a.s.batch;
   const int64_t prefix = (int64_t)a.prefix_width * a.c.page_size;
-  p->nt = (prefix > 0 ? all : own) > 8 ? 2 : 1;
+  p->nt = row_tile(prefix > 0 ? all : own);
   const int tile = 8 * p->nt;
   p->s_tiles = (int)((own + tile - 1) / tile);
   p->p_tiles = prefix > 0 ? (int)((all + tile - 1) / tile) : 0;
@@ -945,7 +957,8 @@ cudaError_t launch_split(const SplitArgs& s, unsigned grid, cudaStream_t stream)
   static std::atomic<uint64_t> ready{0};  // a bit for each device
   int dev = 0;
   cudaGetDevice(&dev);
-  if (kSmem > 46 * 1024 /* the static part comes on top */ && (dev < 0 || dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
+  // (the static part comes on top)
+  if (kSmem > 46 * 1024 && (dev < 0 || dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
@@ -956,7 +969,9 @@ cudaError_t launch_split(const SplitArgs& s, unsigned grid, cudaStream_t stream)
 
 template <int kFmt, int kHP>
 cudaError_t launch_rows(const SplitArgs& s, int nt, unsigned grid, cudaStream_t stream) {
-  return nt == 1 ? launch_split<kFmt, kHP, 1>(s, grid, stream) : launch_split<kFmt, kHP, 2>(s, grid, stream);
+  return nt == 1   ? launch_split<kFmt, kHP, 1>(s, grid, stream)
+         : nt == 2 ? launch_split<kFmt, kHP, 2>(s, grid, stream)
+                   : launch_split<kFmt, kHP, 3>(s, grid, stream);
 }
 
 template <int kFmt>
@@ -978,9 +993,24 @@ struct CachePlan {
 };
 
 // The tile kernels widen a key set once for all its rows and then take 256 rows
-// at a time; the split kernel widens it for every 16 rows.
+// at a time; the split kernel widens it for every 8 to 24 rows.  Their times in
+// us, fitted to calls of 16 to 256 rows on 300 to 4000 keys (`keys` over all
+// sets and kv heads, as both take them):
+//   split  9 + 2.6e-6 rows (keys + 256 a set and head)
+//   tile  14 + (230e-6 + 35e-6 ceil(rows / 128)) keys
+// Measured, 8 kv heads of 8 bits, split against tile: one sequence of 1000 keys,
+// 256 rows 18.0 / 21.4; of 4000 keys 96 rows 20.5 / 21.0, 256 rows 32.6 / 30.5; 16
+// sequences of 1000 keys 64 rows 40.5 / 46.8, 96 rows 51.7 / 47.2; of 4000 keys
+// 96 rows 132 / 152, 128 rows 191 / 152.  BQ4_CACHE_TILE=0 or 1 chooses for
+// every call whose workspace stays within 1 GB (tests).
 bool use_tile(const CacheAttnCall& a, bool prefix, int64_t rows, int64_t keys, int sms, CacheTilePlan* p) {
-  return rows >= 64 && keys >= 256 && plan_cache_tile(a, prefix, sms, p) && p->workspace_bytes <= (size_t)1 << 30;
+  const double heads = (double)a.c.kv_heads * (prefix ? 1 : a.s.batch), all = heads * (double)keys;
+  const double split = 9.0 + 2.6e-6 * (double)rows * (all + 256.0 * heads);
+  const double tile = 14.0 + (230e-6 + 35e-6 * (double)((rows + 127) / 128)) * all;
+  bool take = tile < split;
+  if (const char* f = getenv("BQ4_CACHE_TILE")) take = f[0] != '0';
+  return take && rows > 0 && keys > 0 && plan_cache_tile(a, prefix, sms, p) &&
+         p->workspace_bytes <= (size_t)1 << 30;
 }
 
 bq4_status plan_cache(const CacheAttnCall& a, int sms, CachePlan* p) {

@@ -18,9 +18,9 @@ factor 1 + e.  A score is at most SCORE in size (asserted) with sums of |q k|
 at most 8 SCORE, over at most 32 roundings of 2^-24: e <= 2^-16 SCORE for the
 numerator, the same for the sum; plus 2^-14 for the exponential, the online
 rescalings and f32 sums of up to 2^10 steps of 2^-24.
-Calls of 64 rows a kv head and more on 256 keys and more also round the widened
-v of an 8-bit cache to f16 (at most half a step, 2^-11 of each value): where
-`staged` is given, another 2^-11 a.
+The kernels for many rows a kv head also round the widened v of an 8-bit cache to
+f16 (at most half a step, 2^-11 of each value): where `staged` is given, another
+2^-11 a.  BQ4_CACHE_TILE=1 takes them for every call, 0 for none.
 """
 import math
 
@@ -215,10 +215,10 @@ def test_strided_sources_and_untouched_rows(fmt):
 
 # --------------------------------------------------------------------- attention
 
-def run_attention(book, S, Hq, causal=True, scale=None, **kw):
+def run_attention(book, S, Hq, causal=True, scale=None, staged=False):
     q = book.query(S, Hq)
-    got = book.cache.attention(q, book.table, book.lengths, causal=causal, scale=scale, **kw)
-    check(got, *attend(q.double(), book.k, book.v, causal, scale=scale))
+    got = book.cache.attention(q, book.table, book.lengths, causal=causal, scale=scale)
+    check(got, *attend(q.double(), book.k, book.v, causal, scale=scale), staged=staged)
     return q, got
 
 
@@ -245,10 +245,16 @@ def test_one_long_context(fmt):
     run_attention(book, 4, 16)
 
 
-def test_many_query_tokens():
+@pytest.fixture(params=["0", "1"], ids=["split", "tile"])
+def path(request, monkeypatch):
+    monkeypatch.setenv("BQ4_CACHE_TILE", request.param)
+    return request.param
+
+
+def test_many_query_tokens(path):
     for fmt, S, n, D, causal in (("q8", 300, 1111, 128, True), ("q4", 129, 129, 64, True),
                                  ("f16", 256, 700, 120, False), ("q8", 513, 2000, 120, True)):
-        run_attention(Book(fmt, [n, max(0, n - 130), 40], 2, D, 32, seed=S, poison=True), S, 8, causal)
+        run_attention(Book(fmt, [n, max(0, n - 130), 40], 2, D, 32, seed=S, poison=True), S, 8, causal, staged=True)
 
 
 def test_scale_and_running_maximum():
@@ -282,20 +288,20 @@ def test_values_of_very_different_size(fmt):
 @pytest.mark.parametrize("fmt", ["f16", "q8", "q4"])
 @pytest.mark.parametrize("S,Hq,Hkv,D,prefix", [(1, 8, 2, 128, 700), (1, 28, 7, 120, 17), (4, 8, 8, 64, 333),
                                                (3, 8, 1, 128, 1), (40, 8, 2, 128, 260)])
-def test_shared_prefix(fmt, S, Hq, Hkv, D, prefix):
+def test_shared_prefix(fmt, S, Hq, Hkv, D, prefix, path):
     book = Book(fmt, [0, 1, 100, 37, 64, S], Hkv, D, 16, prefix=prefix, seed=S + D, poison=True)
     q = book.query(S, Hq)
     for causal in (True, False):
         got = book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths, causal=causal)
         exact = attend(q.double(), book.k, book.v, causal, book.pk, book.pv)
-        check(got, *exact)
+        check(got, *exact, staged=True)
     # an empty prefix is plain attention; an empty table is the prefix alone
     none = torch.zeros(1, dtype=torch.int32, device=DEV)
     got = book.cache.prefix_attention(q, book.ptable, none, book.table, book.lengths)
-    check(got, *attend(q.double(), book.k, book.v, True))
+    check(got, *attend(q.double(), book.k, book.v, True), staged=True)
     got = book.cache.prefix_attention(q, book.ptable, book.plen, book.table[:, :0], torch.zeros_like(book.lengths))
     empty = [x[:0] for x in book.k]
-    check(got, *attend(q.double(), empty, empty, False, book.pk, book.pv))
+    check(got, *attend(q.double(), empty, empty, False, book.pk, book.pv), staged=True)
 
 
 def test_shared_prefix_of_a_large_batch():
@@ -339,8 +345,8 @@ def test_masked_nan_and_held_nan():
 
 @pytest.mark.parametrize("fmt", ["f16", "q8", "q4"])
 @pytest.mark.parametrize("page", [16, 48, 4096])
-def test_prefix_and_own_keys_both_long(fmt, page):
-    # 160 rows of each sequence and 480 of the batch on hundreds of keys: both by the many-row kernels
+def test_prefix_and_own_keys_both_long(fmt, page, path):
+    # 160 rows of each sequence and 480 of the batch on hundreds of keys
     book = Book(fmt, [700, 263, 39], 2, 128, page, prefix=600, seed=page, poison=True)
     q = book.query(40, 8)
     for causal in (True, False):
@@ -356,19 +362,20 @@ def test_prefix_and_own_keys_both_long(fmt, page):
 
 
 @pytest.mark.parametrize("fmt", ["q8", "q4", "f16"])
-def test_many_rows_with_rows_of_any_size(fmt):
+def test_many_rows_with_rows_of_any_size(fmt, path):
     # k from 2^-30 to 2^4 and v from 2^-12 to 2^17 (f32 rows; f16 caches hold up to 2^15): the
     # widened tiles keep them in f16's range by factors of two
     n, S = 600, 20
     book = Book(fmt, [n], 1, 128, 64, seed=21)
     g = book.g
-    k = torch.randn((n, 1, 128), generator=g, device=DEV) * 2.0 ** torch.randint(-30, 3, (n, 1, 1), generator=g, device=DEV)
+    k = torch.randn((n, 1, 128), generator=g, device=DEV)
+    k *= 2.0 ** torch.randint(-30, 3, (n, 1, 1), generator=g, device=DEV)
     hi = 15 if fmt == "f16" else 18
-    v = torch.randn((n, 1, 128), generator=g, device=DEV).clamp(-1.9, 1.9) * \
-        2.0 ** torch.randint(-12, hi - 1, (n, 1, 1), generator=g, device=DEV)
+    v = torch.randn((n, 1, 128), generator=g, device=DEV).clamp(-1.9, 1.9)
+    v *= 2.0 ** torch.randint(-12, hi - 1, (n, 1, 1), generator=g, device=DEV)
     book.cache.append(k[None], v[None], book.table, book.lengths)
     hk, hv = held(k, fmt), held(v, fmt)
-    for Hq in (4, 1):  # 80 rows, then 20 (the few-row kernel)
+    for Hq in (4, 1):  # 80 rows, then 20
         q = torch.randn((1, S, Hq, 128), generator=g, device=DEV).half()
         got = book.cache.attention(q, book.table, book.lengths)
         exact, mag, top = attend(q.double(), [hk], [hv], True)
@@ -379,7 +386,7 @@ def test_many_rows_with_rows_of_any_size(fmt):
         check(torch.where(fits, got.double(), zero), torch.where(fits, exact, zero), mag, top, staged=True)
 
 
-def test_many_rows_with_nan_and_bad_pages():
+def test_many_rows_with_nan_and_bad_pages(path):
     n, S = 400, 30
     for fmt in ("f16", "q8", "q4"):
         book = Book(fmt, [n, n], 1, 128, 16, seed=31, poison=True)
@@ -394,7 +401,7 @@ def test_many_rows_with_nan_and_bad_pages():
         got = book.cache.attention(q, book.table, book.lengths)
         q4.poll_device_error()
         assert torch.equal(got[1], want[1]) and torch.equal(got[0, :S - 10], want[0, :S - 10])
-        assert got[0, S - 10:, :, 77].isnan().all()
+        assert got[0, S - 10:, :, 77].isnan().all()  # (the many-row kernels give the whole row NaN)
         # a page outside the cache holds nothing: the rest is as without its rows
         table = book.table.clone()
         table[1, 3] = 10 ** 6
@@ -405,7 +412,7 @@ def test_many_rows_with_nan_and_bad_pages():
         check(got, *attend(q[1:].double(), [k], [v], True), staged=True)
 
 
-def test_more_sequences_than_threads():
+def test_more_sequences_than_threads(path):
     # 300 sequences, most of them empty or short, in one line of work
     lengths = [(7 * i) % 90 if i % 3 else 0 for i in range(300)]
     book = Book("q8", [max(lengths)], 2, 64, 16, seed=41)
@@ -415,11 +422,10 @@ def test_more_sequences_than_threads():
     got = book.cache.attention(q, table, n)
     ks, vs = [book.k[0][:x] for x in lengths], [book.v[0][:x] for x in lengths]
     check(got, *attend(q.double(), ks, vs, True))
-    q = torch.randn((300, 33, 4, 64), generator=book.g, device=DEV).half()  # 66 rows: the bound of the lengths decides
-    wide = torch.cat([book.table] * 5, 1).expand(300, -1)
-    got = book.cache.attention(q, wide, n)
+    q = torch.randn((300, 33, 4, 64), generator=book.g, device=DEV).half()
+    got = book.cache.attention(q, table, n)
     check(got, *attend(q.double(), ks, vs, True), staged=True)
-    assert torch.equal(got, book.cache.attention(q, wide, n))
+    assert torch.equal(got, book.cache.attention(q, table, n))
 
 
 # --------------------------------------------------------------------- bad pages, long caches
@@ -464,7 +470,7 @@ def test_bad_pages_and_lengths_are_reported():
     q4.poll_device_error()
 
 
-def test_cache_past_four_gib():
+def test_cache_past_four_gib(path):
     # 5 GiB of pages: offsets of the last ones pass 32 bits
     pages, page, H, D = 20480, 64, 16, 128
     c = KVCache(pages, page, H, D, "q8", DEV)
@@ -585,7 +591,7 @@ def test_streams_and_graphs():
     q4.poll_device_error()
 
 
-def test_many_rows_in_a_graph():
+def test_many_rows_in_a_graph(path):
     book = Book("q4", [500, 300], 2, 128, 16, prefix=400, seed=13)
     c, S = book.cache, 24
     q = book.query(S, 8)
