@@ -576,6 +576,9 @@ __global__ void __launch_bounds__(kTThreads, 1) cache_tile_kernel(const __grid_c
       const bool plain = !k->partial && __all_sync(0xffffffffu, valid >= kKeys);
       attn_ld64(t_s, r);
       float top = plain ? scores64<true>(r, k, 0, valid) : scores64<false>(r, k, 0, valid);
+#pragma unroll
+      for (int i = 0; i < 64; i += 16)  // y of keys 0..63 goes back over S until the P pass
+        ptx::tmem_st_32x32b_x16(t_s + i, *reinterpret_cast<uint32_t(*)[16]>(r + i));
       attn_ld64(t_s + 64, r);  // kept for the P pass
       top = fmaxf(top, plain ? scores64<true>(r, k, 64, valid) : scores64<false>(r, k, 64, valid)) + e;
       const bool jump = top > m + kTJump;
@@ -599,12 +602,8 @@ __global__ void __launch_bounds__(kTThreads, 1) cache_tile_kernel(const __grid_c
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&p_half[t]);
-      // keys 0..63 (read again) -> P columns 64..95
+      // keys 0..63 (y stored above, and the wait for P's stores since) -> P columns 64..95
       attn_ld64(t_s, r);
-      if (plain)
-        scores64<true>(r, k, 0, valid);
-      else
-        scores64<false>(r, k, 0, valid);
       sum += probs64(r, e - m_use, t_s + 64);
       l = l * alpha + sum * attn_ex2(-e);
       m = m_use;
