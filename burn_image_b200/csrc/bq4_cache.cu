@@ -5,9 +5,9 @@
 // Both kernels move each byte once and compute next to nothing, so HBM (and,
 // for a decode step's few rows, the launch) bounds them: 8 x 4352 rows of 8 kv
 // heads, 8 bits to f16, are read in 45 us (211 MB, 4.7 TB/s, 0.71 of the copy
-// rate); 4352 f32 rows are written in 4 bits in 14.7 us (41 MB; some 120
+// rate); 4352 f32 rows are written in 4 bits in 14.1 us (41 MB; some 110
 // instructions a row for two roundings and the packing); a decode step of 32
-// sequences takes 3.2 us to write and 2.8 to read back, an empty launch 1.4.
+// sequences takes 3.0 us to write and 2.8 to read back, an empty launch 1.4.
 // A warp takes 4 to 16 neighbouring positions of one page, for one head's k or
 // v, as many as it loads before it uses the first: page, row and sequence are
 // worked out once for them.  A row of HP values is taken by HP / W lanes, W
@@ -211,14 +211,16 @@ __global__ void __launch_bounds__(kCThreads) cache_append_kernel(const __grid_co
         const __nv_bfloat16 sb =
             __float2bfloat16_rn(most >= 0x7f800000u ? __int_as_float(0x7fc00000) : __fdiv_rn(top, kTop));
         const float s = __bfloat162float(sb);
-        // x (1 / s) is the quotient but for three roundings, 2^-22 of at most kTop (1 + 2^-9):
-        // where it lies 2^-14 or more from a half, both round to the same whole number, which
-        // needs no clamping.  The divisions are left for a lane that holds another one, and for
-        // scales whose inverse is not normal.  y + 1.5 2^23 rounds y to a whole number in the
-        // low bits of the sum.
+        // x (1 / s) is the quotient but for 2^-23 of the inverse and two roundings, 2^-22 in all of
+        // at most kTop (1 + 2^-9): where it lies 2^-14 or more from a half, both round to the same
+        // whole number, which needs no clamping.  The divisions are left for a lane that holds
+        // another one, and for scales whose inverse is not normal.  y + 1.5 2^23 rounds y to a
+        // whole number in the low bits of the sum.
         constexpr float kRound = 12582912.0f;
         constexpr uint32_t kZero = kFmt == BQ4_CACHE_Q8 ? 128 : 8;
-        const float inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
+        float inv;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+        if (!(s > 0.0f)) inv = 0.0f;
         uint32_t q[kW];  // u = q + 128 or q + 8
         float far = s > 0.0f && !(s >= 0x1p-120f && s <= 0x1p120f) ? 1.0f : 0.0f;
 #pragma unroll

@@ -33,7 +33,8 @@
 //     long as q follows it.
 //   * Stored values are whole numbers u = q + 128 (q + 8).  Zero-extended to
 //     16 bits they are the subnormal halves u 2^-24, exact in the tensor core:
-//     widening a pair of k values is one byte permute (q8) or mask (q4).  The
+//     widening a pair of k values is one byte permute (q8) or mask (q4, every
+//     second pair 16 times too large, against a sixteenth of q).  The
 //     offset leaves the scores through the accumulator's start value -128
 //     2^-24 sum(q) (f32; q4: for each scale's 32 values).  v is made signed, one
 //     add a pair: in O = sum p v, over many keys, an offset would cost the sum
@@ -51,8 +52,8 @@
 // What bounds it (148 SMs, 6.57 TB/s copied): HBM for f16 rows (16 sequences of
 // 3000 to 4352 rows of 64 values, 118 MB: 26 us, 0.68 of the copy rate); the
 // issue of instructions for 4 bits (64 sequences of 300 to 8192 rows, 314 MB:
-// 86 us, 0.55; some 400 instructions a warp and step of 2304 bytes, of which
-// 80 widen k, 70 v and 40 weigh p for the four v scales); latency for one short
+// 85 us, 0.56; some 350 instructions a warp and step of 2304 bytes, of which
+// 50 widen k, 70 v and 40 weigh p for the four v scales); latency for one short
 // sequence (1000 rows: 7.6 us, of which 3 are two launches' starts).
 // Taken on the way, device time: one warp a row 692 / 8502 us for one sequence
 // of 1000 rows / the 64 sequences; these tiles with 16-byte copies by each lane
@@ -375,6 +376,7 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
     uint32_t q[kNT][Y::kKS][2];
     constexpr int kOffs = kFmt == BQ4_CACHE_Q4 ? Y::kNb : 1;  // start values of a row
     float off[kNT][kOffs][2];
+    float unit[kNT][2];  // 4 bits: log2-unit scores of rows 2t, 2t + 1 from their sums
     int see[kNT][2];
     int see_all = 0x7fffffff;
 #pragma unroll
@@ -398,6 +400,31 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
         q[nt][ks][0] = u.x;
         q[nt][ks][1] = u.y;
       }
+      if constexpr (kFmt == BQ4_CACHE_Q4) {
+        // q times a power of two that brings the row's largest into [2^9, 2^10): then every second
+        // pair can be divided by 16 (below) without leaving f16's range
+        uint32_t most = 0;
+#pragma unroll
+        for (int ks = 0; ks < Y::kKS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            most = max(most, max(q[nt][ks][e] & 0x7fffu, q[nt][ks][e] >> 16 & 0x7fffu));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));  // of row g
+        const float top = __half2float(__ushort_as_half((unsigned short)most));
+        const int lift = most ? 9 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;  // [-7, 33]
+        const float up = __uint_as_float((uint32_t)(127 + lift) << 23);
+        const float down = __uint_as_float((uint32_t)(127 - lift) << 23);
+        unit[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t) * (s.c * 0x1p24f);
+        unit[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4) * (s.c * 0x1p24f);
+#pragma unroll
+        for (int ks = 0; ks < Y::kKS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q[nt][ks][e]));
+            q[nt][ks][e] = pack_h2(f.x * up, f.y * up);
+          }
+      }
       if constexpr (Y::kQ) {
 #pragma unroll
         for (int o = 0; o < kOffs; ++o) {
@@ -414,6 +441,13 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
           constexpr float kZero = kFmt == BQ4_CACHE_Q8 ? -128.0f : -8.0f;
           off[nt][o][0] = __shfl_sync(0xffffffffu, sum, 8 * t) * (kZero * 0x1p-24f);
           off[nt][o][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4) * (kZero * 0x1p-24f);
+        }
+        if constexpr (kFmt == BQ4_CACHE_Q4) {
+#pragma unroll
+          for (int ks = 0; ks < Y::kKS; ++ks) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q[nt][ks][1]));
+            q[nt][ks][1] = pack_h2(f.x * 0.0625f, f.y * 0.0625f);
+          }
         }
       } else {
         off[nt][0][0] = off[nt][0][1] = 0.0f;
@@ -528,8 +562,9 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
             constexpr uint32_t kPair = 0x000F000Fu;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t a0 = (w0[e] >> 8 * h) & kPair, a2 = (w0[e] >> (8 * h + 4)) & kPair;
-              const uint32_t a1 = (w1[e] >> 8 * h) & kPair, a3 = (w1[e] >> (8 * h + 4)) & kPair;
+              // every second pair is taken where it lies, 16 times too large, against q / 16
+              const uint32_t z0 = w0[e] >> 8 * h, z1 = w1[e] >> 8 * h;
+              const uint32_t a0 = z0 & kPair, a2 = z0 & kPair << 4, a1 = z1 & kPair, a3 = z1 & kPair << 4;
 #pragma unroll
               for (int nt = 0; nt < kNT; ++nt)
                 mma16816(y[nt], a0, a1, a2, a3, q[nt][2 * e + h][0], q[nt][2 * e + h][1]);
@@ -562,7 +597,7 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
       for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          z[nt][u] = fmaf(x[nt][u], u < 2 ? c0 : c1, -base[nt][u & 1]);
+          z[nt][u] = fmaf(x[nt][u], kFmt == BQ4_CACHE_Q4 ? unit[nt][u & 1] : u < 2 ? c0 : c1, -base[nt][u & 1]);
           if (kEdge && limit[nt][u & 1] <= 8 * (u >> 1)) z[nt][u] = -INFINITY;
         }
         move |= fmaxf(fmaxf(z[nt][0], z[nt][1]) + lg[0], fmaxf(z[nt][2], z[nt][3]) + lg[1]) > kJump;
@@ -572,7 +607,8 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
         for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x0 = x[nt][e] * c0, x1 = x[nt][e + 2] * c1;
+            float x0 = x[nt][e] * (kFmt == BQ4_CACHE_Q4 ? unit[nt][e] : c0);
+            float x1 = x[nt][e + 2] * (kFmt == BQ4_CACHE_Q4 ? unit[nt][e] : c1);
             if (kEdge && limit[nt][e] <= 0) x0 = -INFINITY;
             if (kEdge && limit[nt][e] <= 8) x1 = -INFINITY;
             float top = fmaxf(x0 + lg[0], x1 + lg[1]);

@@ -176,6 +176,26 @@ def test_extreme_values(fmt):
         assert torch.equal(y[0, 0].isnan(), want.isnan())
 
 
+@pytest.mark.parametrize("fmt", ["q8", "q4"])
+def test_many_values_and_ties(fmt):
+    # 2^23 values of rows from 2^-140 to 2^100, and rows of exact halves of their scale
+    g = torch.Generator(device=DEV).manual_seed(17)
+    c = KVCache(64, 256, 4, 128, fmt, DEV)
+    x = torch.randn((64, 256, 4, 128), generator=g, device=DEV)
+    x *= 2.0 ** torch.randint(-140, 101, (64, 256, 4, 1), generator=g, device=DEV).double().float()
+    s = 2.0 ** torch.randint(-20, 20, (8, 256, 4, 1), generator=g, device=DEV).float()
+    top = int(QMAX[fmt])
+    x[:8] = (torch.randint(-top, top, (8, 256, 4, 128), generator=g, device=DEV) + 0.5) * s
+    x[:8, :, :, ::32] = QMAX[fmt] * s  # the largest of every block: the scale is s
+    table = torch.arange(64, dtype=torch.int32, device=DEV)[:, None]
+    n = torch.full((64,), 256, dtype=torch.int32, device=DEV)
+    for v in (x, x.clamp(-6e4, 6e4).half()):
+        c.append(v, v, table, n)
+        for y in c.read(table, n, 256, dtype=torch.float32):
+            assert torch.equal(y, held(v, fmt).float().transpose(1, 2))
+    q4.poll_device_error()
+
+
 @pytest.mark.parametrize("fmt", ["q8", "q4", "f16"])
 def test_strided_sources_and_untouched_rows(fmt):
     # k and v as sections of one projection output, head-major views, an odd offset (scalar loads)
