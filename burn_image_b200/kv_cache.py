@@ -60,7 +60,8 @@ class KVCache:
         self.device, self._index = dev, dev.index
         self.data = torch.zeros(n.value, dtype=torch.uint8, device=dev)
         c.data, c.device = self.data.data_ptr(), dev.index
-        self._plans = {}  # of attention calls, by their sizes
+        self._plans = {}       # of attention calls, by their sizes
+        self._contiguous = {}  # strides of contiguous rows, by their shape
         self._lib = L.lib()
         self._c = c
         self._ref = ctypes.byref(c)
@@ -101,6 +102,18 @@ class KVCache:
                            f"{what} must be [B, S, {heads or 'heads'}, {self.head_dim}], got {tuple(shape)}")
         return t if t.stride(3) == 1 or t.numel() == 0 else t.contiguous()
 
+    def _strides(self, t: torch.Tensor):
+        """The first three strides of a 4-D tensor; those of contiguous ones are made once a shape."""
+        if not t.is_contiguous():
+            return _Strides(*t.stride()[:3])
+        shape = t.shape
+        got = self._contiguous.get(shape)
+        if got is None:
+            if len(self._contiguous) >= 1024:
+                self._contiguous.clear()
+            got = self._contiguous[shape] = _Strides(*t.stride()[:3])
+        return got
+
     def append(self, key: torch.Tensor, value: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor) -> None:
         """Quantise the newest rows of every sequence into the cache: key and
         value [B, S, kv_heads, head_dim] (float32 or float16, any strides; a
@@ -109,13 +122,14 @@ class KVCache:
         aligns its rows at their ends.  Sequences that share a page must not
         write the same row."""
         k = self._rows(key, "key", self.kv_heads)
-        v = self._rows(value, "value", self.kv_heads)
-        if v.shape != k.shape or v.dtype != k.dtype:
-            raise Bq4Error(L.EINVAL_SHAPE, "key and value must have one shape and type")
+        v = value
+        if v.shape != k.shape or v.dtype is not k.dtype or v.device != self.device:
+            raise Bq4Error(L.EINVAL_SHAPE, "key and value must have one shape and type, on one device")
+        if v.stride(3) != 1 and v.numel():
+            v = v.contiguous()
         seqs = self._sequences(page_table, lengths, k.shape[0])
-        check(self._lib.bq4_cache_append(self._ref, ctypes.byref(seqs), k.data_ptr(), _Strides(*k.stride()[:3]),
-                                         v.data_ptr(), _Strides(*v.stride()[:3]), _DTYPES[k.dtype], k.shape[1],
-                                         _raw_stream(self._index)))
+        check(self._lib.bq4_cache_append(self._ref, ctypes.byref(seqs), k.data_ptr(), self._strides(k), v.data_ptr(),
+                                         self._strides(v), _DTYPES[k.dtype], k.shape[1], _raw_stream(self._index)))
 
     def read(self, page_table: torch.Tensor, lengths: torch.Tensor, count: int,
              starts: Optional[torch.Tensor] = None,
@@ -135,7 +149,7 @@ class KVCache:
         k = page_table.new_empty((seqs.batch, H, count, D), dtype=dtype)
         v = torch.empty_like(k)
         check(self._lib.bq4_cache_read(self._ref, ctypes.byref(seqs), starts.data_ptr() if starts is not None else None,
-                                       count, k.data_ptr(), v.data_ptr(), _Strides(H * count * D, count * D, D),
+                                       count, k.data_ptr(), v.data_ptr(), self._strides(k),
                                        _DTYPES[dtype], _raw_stream(self._index)))
         return k, v
 
@@ -172,18 +186,17 @@ class KVCache:
             raise Bq4Error(L.EINVAL_ARG, "query must be float16")
         shape = q.shape
         seqs = self._sequences(page_table, lengths, shape[0])
-        plain = q.is_contiguous()
         if out is None:
-            out = torch.empty_like(q) if plain else q.new_empty(shape)
+            out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
         elif out.shape != shape or out.dtype != torch.float16 or out.device != self.device or not out.is_contiguous():
             raise Bq4Error(L.EINVAL_ARG, f"out must be contiguous float16 {tuple(shape)} on {self.device}")
         width = prefix_pages.shape[0] if prefix_pages is not None else 0
         key = (shape, seqs.table_width, width, max_length)
         plan = self._plans.get(key) or self._plan(key)
-        longest, nbytes, strides = plan
+        longest, nbytes = plan
         # a workspace of the call's own: calls on several streams, and graphs captured side by side, never share one
         ws = q.new_empty(nbytes // 2)
-        tail = (q.data_ptr(), strides if plain else _Strides(*q.stride()[:3]), shape[1], shape[2], causal, scale or 0.0,
+        tail = (q.data_ptr(), self._strides(q), shape[1], shape[2], causal, scale or 0.0,
                 out.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(self._index))
         if prefix_pages is None:
             check(self._lib.bq4_cache_attention(self._ref, ctypes.byref(seqs), longest, *tail))
@@ -193,7 +206,7 @@ class KVCache:
         return out
 
     def _plan(self, key):
-        """Bound of the lengths, workspace bytes and contiguous strides of an attention call of these sizes."""
+        """Bound of the lengths and workspace bytes of an attention call of these sizes."""
         (B, S, Hq, D), table_width, width, max_length = key
         held = table_width * self.page_size
         longest = held if max_length is None else max_length
@@ -204,5 +217,5 @@ class KVCache:
                                                            width * self.page_size, ctypes.byref(n)))
         if len(self._plans) >= 1024:
             self._plans.clear()
-        plan = self._plans[key] = (longest, n.value, _Strides(S * Hq * D, Hq * D, D))
+        plan = self._plans[key] = (longest, n.value)
         return plan
