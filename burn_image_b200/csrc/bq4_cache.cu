@@ -4,11 +4,11 @@
 //
 // Both kernels move each byte once and compute next to nothing, so HBM (and,
 // for a decode step's few rows, the launch) bounds them: 8 x 4352 rows of 8 kv
-// heads, 8 bits to f16, are read in 45 us (211 MB, 4.7 TB/s, 0.71 of the copy
+// heads, 8 bits to f16, are read in 43.5 us (211 MB, 4.9 TB/s, 0.74 of the copy
 // rate); 4352 f32 rows are written in 4 bits in 14.1 us (41 MB; some 110
 // instructions a row for two roundings and the packing); a decode step of 32
-// sequences takes 3.0 us to write and 2.8 to read back, an empty launch 1.4.
-// A warp takes 4 to 16 neighbouring positions of one page, for one head's k or
+// sequences takes 3.0 us to write and 2.3 to read back, an empty launch 1.4.
+// A warp takes 2 to 16 neighbouring positions of one page, for one head's k or
 // v, as many as it loads before it uses the first: page, row and sequence are
 // worked out once for them.  A row of HP values is taken by HP / W lanes, W
 // consecutive values each: 8 when they are written (what a block's maximum and
@@ -115,16 +115,21 @@ __device__ __forceinline__ void load_words(const uint8_t* src, uint32_t* w) {
 
 // How a warp of the append and of the read kernel (kF16: of f16 rows) takes
 // rows: kW values a lane, kLanes lanes a row, kPer rows at a time, kTake in all.
-template <int kHP>
+template <int kHP, bool kMany>
 struct TakeAppend {
-  static constexpr int kW = 8, kLanes = kHP / kW, kPer = 32 / kLanes, kRounds = kPer < 4 ? 4 : 2;
+  static constexpr int kW = 8, kLanes = kHP / kW, kPer = 32 / kLanes, kRounds = !kMany ? 1 : kPer < 4 ? 4 : 2;
   static constexpr int kTake = kPer * kRounds;
 };
-template <bool kF16, int kHP>
+template <bool kF16, int kHP, bool kMany>
 struct TakeRead {
-  static constexpr int kW = kF16 ? 8 : 4, kLanes = kHP / kW, kPer = 32 / kLanes, kRounds = 4;
+  static constexpr int kW = kF16 ? 8 : 4, kLanes = kHP / kW, kPer = 32 / kLanes;
+  static constexpr int kRounds = !kMany ? 2 : kPer < 4 ? 8 : 4;
   static constexpr int kTake = kPer * kRounds;
 };
+// Calls of more rows than this (k and v, of all heads) take kMany: 8 rounds a warp
+// read 557056 rows of 8 bits in 43.5 us (4: 45.2, 2: 51.9), 2 rounds the 512 of a
+// decode step in 2.3 (4: 2.8, 8: 3.2); 1 round a warp writes 2590 in 3.0 us (4: 4.3).
+constexpr int64_t kManyRows = 4096;
 
 struct AppendArgs {
   CacheView c;
@@ -146,9 +151,9 @@ __device__ __forceinline__ int page_of(const CacheView& c, const SeqView& s, int
   return -1;
 }
 
-template <int kFmt, bool kF16, int kHP>
+template <int kFmt, bool kF16, int kHP, bool kMany>
 __global__ void __launch_bounds__(kCThreads) cache_append_kernel(const __grid_constant__ AppendArgs a) {
-  using T = TakeAppend<kHP>;
+  using T = TakeAppend<kHP, kMany>;
   constexpr int kW = T::kW, kLanes = T::kLanes, kPer = T::kPer, kAhead = T::kRounds, kTake = T::kTake;
   constexpr int kRow = kFmt == BQ4_CACHE_F16 ? 2 * kHP : kFmt == BQ4_CACHE_Q8 ? kHP : kHP / 2;
   constexpr int kNb = kFmt == BQ4_CACHE_Q8 ? 1 : kHP / kCacheBlock;
@@ -281,9 +286,9 @@ struct ReadArgs {
   int* err;
 };
 
-template <int kFmt, bool kF16, int kHP>
+template <int kFmt, bool kF16, int kHP, bool kMany>
 __global__ void __launch_bounds__(kCThreads) cache_read_kernel(const __grid_constant__ ReadArgs a) {
-  using T = TakeRead<kF16, kHP>;
+  using T = TakeRead<kF16, kHP, kMany>;
   constexpr int kW = T::kW, kLanes = T::kLanes, kPer = T::kPer, kAhead = T::kRounds, kTake = T::kTake;
   constexpr int kRow = kFmt == BQ4_CACHE_F16 ? 2 * kHP : kFmt == BQ4_CACHE_Q8 ? kHP : kHP / 2;
   constexpr int kNb = kFmt == BQ4_CACHE_Q8 ? 1 : kHP / kCacheBlock;
@@ -500,34 +505,51 @@ bool strides_vec(const void* base, const int64_t* st, int esize) {
   return al(base, 16) && st[0] % n == 0 && st[1] % n == 0 && st[2] % n == 0;
 }
 
+// Launches; false: too many warps for one.
+template <int kFmt, bool kF16, int kHP, bool kMany>
+bool launch_append(AppendArgs& a, int64_t batch, cudaStream_t s) {
+  constexpr int kTake = TakeAppend<kHP, kMany>::kTake;
+  a.steps = (int)(((int64_t)a.tokens + 2 * kTake - 2) / kTake);
+  int64_t items = 0;
+  if (!row_count(2 * batch, a.steps, a.c.kv_heads, &items)) return false;
+  a.items = (unsigned)items;
+  const unsigned grid = (unsigned)((items + kCThreads / 32 - 1) / (kCThreads / 32));
+  cache_append_kernel<kFmt, kF16, kHP, kMany><<<grid, kCThreads, 0, s>>>(a);
+  return true;
+}
+template <int kFmt, bool kF16, int kHP>
+bool launch_append(AppendArgs& a, int64_t batch, cudaStream_t s) {
+  return 2 * batch * a.tokens * a.c.kv_heads > kManyRows ? launch_append<kFmt, kF16, kHP, true>(a, batch, s)
+                                                         : launch_append<kFmt, kF16, kHP, false>(a, batch, s);
+}
 template <int kFmt>
-void launch_append(const AppendArgs& a, bool f16, unsigned grid, cudaStream_t s) {
-  if (a.c.hp == 64) {
-    if (f16)
-      cache_append_kernel<kFmt, true, 64><<<grid, kCThreads, 0, s>>>(a);
-    else
-      cache_append_kernel<kFmt, false, 64><<<grid, kCThreads, 0, s>>>(a);
-  } else {
-    if (f16)
-      cache_append_kernel<kFmt, true, 128><<<grid, kCThreads, 0, s>>>(a);
-    else
-      cache_append_kernel<kFmt, false, 128><<<grid, kCThreads, 0, s>>>(a);
-  }
+bool launch_append(AppendArgs& a, bool f16, int64_t batch, cudaStream_t s) {
+  if (a.c.hp == 64)
+    return f16 ? launch_append<kFmt, true, 64>(a, batch, s) : launch_append<kFmt, false, 64>(a, batch, s);
+  return f16 ? launch_append<kFmt, true, 128>(a, batch, s) : launch_append<kFmt, false, 128>(a, batch, s);
 }
 
+template <int kFmt, bool kF16, int kHP, bool kMany>
+bool launch_read(ReadArgs& a, int64_t batch, int64_t count, cudaStream_t s) {
+  constexpr int kTake = TakeRead<kF16, kHP, kMany>::kTake;
+  a.steps = (int)((count + 2 * kTake - 2) / kTake);
+  int64_t items = 0;
+  if (!row_count(2 * batch, a.steps, a.c.kv_heads, &items)) return false;
+  a.items = (unsigned)items;
+  const unsigned grid = (unsigned)((items + kCThreads / 32 - 1) / (kCThreads / 32));
+  cache_read_kernel<kFmt, kF16, kHP, kMany><<<grid, kCThreads, 0, s>>>(a);
+  return true;
+}
+template <int kFmt, bool kF16, int kHP>
+bool launch_read(ReadArgs& a, int64_t batch, int64_t count, cudaStream_t s) {
+  return 2 * batch * count * a.c.kv_heads > kManyRows ? launch_read<kFmt, kF16, kHP, true>(a, batch, count, s)
+                                                      : launch_read<kFmt, kF16, kHP, false>(a, batch, count, s);
+}
 template <int kFmt>
-void launch_read(const ReadArgs& a, bool f16, unsigned grid, cudaStream_t s) {
-  if (a.c.hp == 64) {
-    if (f16)
-      cache_read_kernel<kFmt, true, 64><<<grid, kCThreads, 0, s>>>(a);
-    else
-      cache_read_kernel<kFmt, false, 64><<<grid, kCThreads, 0, s>>>(a);
-  } else {
-    if (f16)
-      cache_read_kernel<kFmt, true, 128><<<grid, kCThreads, 0, s>>>(a);
-    else
-      cache_read_kernel<kFmt, false, 128><<<grid, kCThreads, 0, s>>>(a);
-  }
+bool launch_read(ReadArgs& a, bool f16, int64_t batch, int64_t count, cudaStream_t s) {
+  if (a.c.hp == 64)
+    return f16 ? launch_read<kFmt, true, 64>(a, batch, count, s) : launch_read<kFmt, false, 64>(a, batch, count, s);
+  return f16 ? launch_read<kFmt, true, 128>(a, batch, count, s) : launch_read<kFmt, false, 128>(a, batch, count, s);
 }
 
 // The sizes that both the workspace query and the calls check and plan with.
@@ -649,21 +671,13 @@ bq4_status bq4_cache_append(const bq4_cache* cache, const bq4_cache_sequences* s
   }
   a.vec = strides_vec(k, k_strides, es) && strides_vec(v, v_strides, es);
   a.tokens = (int)tokens;
-  const int take = a.c.hp == 64 ? TakeAppend<64>::kTake : TakeAppend<128>::kTake;
-  a.steps = (int)((tokens + 2 * take - 2) / take);
-  if (!row_count(2 * seqs->batch, a.steps, cache->kv_heads, &rows))
-    return set_error(BQ4_EINVAL_SHAPE, "batch * tokens * kv_heads too large for one launch");
-  a.items = (unsigned)rows;
   a.err = device_error_word();
   if (!a.err) return set_error(BQ4_ECUDA, "device error word unavailable");
-  const unsigned grid = (unsigned)((rows + kCThreads / 32 - 1) / (kCThreads / 32));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (cache->format == BQ4_CACHE_F16)
-    launch_append<BQ4_CACHE_F16>(a, es == 2, grid, s);
-  else if (cache->format == BQ4_CACHE_Q8)
-    launch_append<BQ4_CACHE_Q8>(a, es == 2, grid, s);
-  else
-    launch_append<BQ4_CACHE_Q4>(a, es == 2, grid, s);
+  const bool ok = cache->format == BQ4_CACHE_F16  ? launch_append<BQ4_CACHE_F16>(a, es == 2, seqs->batch, s)
+                  : cache->format == BQ4_CACHE_Q8 ? launch_append<BQ4_CACHE_Q8>(a, es == 2, seqs->batch, s)
+                                                  : launch_append<BQ4_CACHE_Q4>(a, es == 2, seqs->batch, s);
+  if (!ok) return set_error(BQ4_EINVAL_SHAPE, "batch * tokens * kv_heads too large for one launch");
   note_launch();
   return check_cuda(cudaGetLastError(), "cache append launch");
 }
@@ -697,22 +711,13 @@ bq4_status bq4_cache_read(const bq4_cache* cache, const bq4_cache_sequences* seq
   for (int i = 0; i < 3; ++i) a.stride[i] = strides[i];
   a.vec = strides_vec(k_out, strides, es) && strides_vec(v_out, strides, es);
   a.count = (int)count;
-  const int take = es == 2 ? a.c.hp == 64 ? TakeRead<true, 64>::kTake : TakeRead<true, 128>::kTake
-                   : a.c.hp == 64 ? TakeRead<false, 64>::kTake : TakeRead<false, 128>::kTake;
-  a.steps = (int)((count + 2 * take - 2) / take);
-  if (!row_count(2 * seqs->batch, a.steps, cache->kv_heads, &rows))
-    return set_error(BQ4_EINVAL_SHAPE, "batch * count * kv_heads too large for one launch");
-  a.items = (unsigned)rows;
   a.err = device_error_word();
   if (!a.err) return set_error(BQ4_ECUDA, "device error word unavailable");
-  const unsigned grid = (unsigned)((rows + kCThreads / 32 - 1) / (kCThreads / 32));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (cache->format == BQ4_CACHE_F16)
-    launch_read<BQ4_CACHE_F16>(a, es == 2, grid, s);
-  else if (cache->format == BQ4_CACHE_Q8)
-    launch_read<BQ4_CACHE_Q8>(a, es == 2, grid, s);
-  else
-    launch_read<BQ4_CACHE_Q4>(a, es == 2, grid, s);
+  const bool ok = cache->format == BQ4_CACHE_F16  ? launch_read<BQ4_CACHE_F16>(a, es == 2, seqs->batch, count, s)
+                  : cache->format == BQ4_CACHE_Q8 ? launch_read<BQ4_CACHE_Q8>(a, es == 2, seqs->batch, count, s)
+                                                  : launch_read<BQ4_CACHE_Q4>(a, es == 2, seqs->batch, count, s);
+  if (!ok) return set_error(BQ4_EINVAL_SHAPE, "batch * count * kv_heads too large for one launch");
   note_launch();
   return check_cuda(cudaGetLastError(), "cache read launch");
 }
