@@ -32,9 +32,9 @@
 // Every wait is bounded (BQ4_ETIMEOUT), as in bq4_attn_fused.cu.
 //
 // What bounds it: the softmax threads' chain from S to P.  A 512-token chunk of 32
-// / 8 heads on 8704 rows of 8 bits takes 115 us (widening 13, products 96, join
-// 8 with its start hidden): 71 GFLOP, 0.37 of the bf16 peak; the products alone
-// run a record of 256 rows in 2.7 us, 1.5 at the peak.  Tried: two threads a row
+// / 8 heads on 8704 rows of 8 bits takes 113 us (widening 13, products 92, join
+// 8 with its start hidden): 71 GFLOP, 0.37 of the bf16 peak; a record of 256 rows
+// takes 2.6 us, 1.5 at the peak.  Tried: two threads a row
 // (their exchange and the registers that it costs: 152 us), a row's 128 scores
 // in registers (spilled), equal shares of all records for every CTA instead of
 // halves of a range on 128 of 148 SMs (113 to 118 us; 103 against 99 us behind
