@@ -64,6 +64,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 #include <type_traits>
 
@@ -1023,10 +1024,6 @@ cudaError_t launch_head(const SplitArgs& s, int nt, unsigned grid, cudaStream_t 
   return s.a.c.hp == 64 ? launch_rows<kFmt, 64>(s, nt, grid, stream) : launch_rows<kFmt, 128>(s, nt, grid, stream);
 }
 
-}  // namespace
-
-namespace {
-
 // Which kernels take the prefix's and the sequences' own keys, and their workspaces.
 struct CachePlan {
   bool tile_p, tile_s;
@@ -1041,16 +1038,19 @@ struct CachePlan {
 // us, fitted to calls of 16 to 256 rows on 300 to 4000 keys (`keys` over all
 // sets and kv heads, as both take them):
 //   split  9 + 2.6e-6 rows (keys + 256 a set and head)
-//   tile  14 + (230e-6 + 35e-6 ceil(rows / 128)) keys
+//   tile  14 + (230e-6 + 35e-6 ceil(rows / 128)) keys, and 7 for every wave of
+//         256-row tiles after the first
 // Measured, 8 kv heads of 8 bits, split against tile: one sequence of 1000 keys,
 // 256 rows 18.0 / 21.4; of 4000 keys 96 rows 20.5 / 21.0, 256 rows 32.6 / 30.5; 16
 // sequences of 1000 keys 64 rows 40.5 / 46.8, 96 rows 51.7 / 47.2; of 4000 keys
-// 96 rows 132 / 152, 128 rows 191 / 152.  BQ4_CACHE_TILE=0 or 1 chooses for
+// 96 rows 132 / 152, 128 rows 191 / 152; 72 sequences of 8 keys behind 8
+// shared ones, 20 rows, 37 / 69 in all.  BQ4_CACHE_TILE=0 or 1 chooses for
 // every call whose workspace stays within 1 GB (tests).
 bool use_tile(const CacheAttnCall& a, bool prefix, int64_t rows, int64_t keys, int sms, CacheTilePlan* p) {
   const double heads = (double)a.c.kv_heads * (prefix ? 1 : a.s.batch), all = heads * (double)keys;
   const double split = 9.0 + 2.6e-6 * (double)rows * (all + 256.0 * heads);
-  const double tile = 14.0 + (230e-6 + 35e-6 * (double)((rows + 127) / 128)) * all;
+  const double waves = std::ceil(heads * (double)((rows + 255) / 256) / sms);
+  const double tile = 14.0 + (230e-6 + 35e-6 * (double)((rows + 127) / 128)) * all + 7.0 * (waves - 1.0);
   bool take = tile < split;
   if (const char* f = getenv("BQ4_CACHE_TILE")) take = f[0] != '0';
   return take && rows > 0 && keys > 0 && plan_cache_tile(a, prefix, sms, p) &&
