@@ -87,13 +87,13 @@ struct CacheAttnCall {
 // Where a row's partial results (m, l and O of some of its keys) lie: the
 // join kernel's input, one of the prefix's and one of the sequence's own keys.
 // Row r of a range (kv head, tile of tile_rows rows) is at slot * tile_rows + r:
-// pieces: slots first CTA + range .. last CTA + range of the split kernel's line;
-// else slots range * chunks .., one for each `span` keys that the tile sees.
+// pieces: slots first CTA + range .. last CTA + range of the split kernel's line, of
+// `grid` CTAs; else slots range * chunks .., one for each `span` keys that the tile sees.
 struct CacheJoinSource {
   const float* part;
   const float2* ml;
   const int2* pieces;
-  int tile_rows, tiles, span, chunks, first_range;
+  int grid, tile_rows, tiles, span, chunks, first_range;
 };
 
 // Launch plan of the many-row kernels (bq4_cache_tile.cu) for the prefix or the

@@ -69,6 +69,7 @@
 #include <type_traits>
 
 #include "bq4_cache.h"
+#include "cache_bounds.h"
 #include "sm100_ptx.cuh"
 
 namespace bq4 {
@@ -853,7 +854,8 @@ __device__ __forceinline__ int2 slots_of(const JoinArgs& g, const CacheJoinSourc
     const int range = s.first_range + (set * g.a.c.kv_heads + kvh) * s.tiles + tile;
     if (keys <= 0) return make_int2(0, 0);
     const int2 cta = s.pieces[range];
-    return make_int2(cta.x + range, cta.y - cta.x + 1);
+    const CacheSlots c = cache_slots(cta.x, cta.y, range, s.grid);
+    return make_int2(c.first, c.count);
   }
   const int last_i = (min((tile + 1) * s.tile_rows, rows) - 1) / g.group;
   const int end = max(0, causal ? keys - g.a.tokens + last_i + 1 : keys);
@@ -1101,6 +1103,7 @@ bq4_status run_split(const CacheAttnCall& a, const SplitPlan& p, bool finish, vo
   own->part = prefix->part = s.part;
   own->ml = prefix->ml = s.ml;
   own->pieces = prefix->pieces = s.pieces;
+  own->grid = prefix->grid = p.grid;
   own->tile_rows = prefix->tile_rows = 8 * p.nt;
   prefix->tiles = p.p_tiles;
   prefix->first_range = 0;
