@@ -756,13 +756,13 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
     // ---- join the four warps through shared memory, in warp order
     __syncthreads();
     if (abort_flag) {
-      // wait once more for the copies under way, then leave
+      // wait once more for the copies under way (put == get may mean none or a full ring), then leave
       __shared__ int never;
       if (threadIdx.x == 0) never = 0;
       __syncthreads();
-      for (; get != put; get = get + 1 == Y::kStages ? 0 : get + 1) {
+      for (int left = cache_pending(j, mine, Y::kStages); left > 0; --left) {
         ptx::mbar_wait(&full[get], parity, &never);
-        if (get + 1 == Y::kStages) parity ^= 1;
+        if (++get == Y::kStages) get = 0, parity ^= 1;
       }
       return;
     }

@@ -25,4 +25,10 @@ BQ4_BOTH CacheSlots cache_slots(int from, int to, int range, int grid) {
   return s;
 }
 
+// Copies of a warp's ring that are under way when it gives up on step j of `mine`: step j has
+// asked for step j + stages - 1, and nothing from step j on has been waited for.
+BQ4_BOTH int cache_pending(int j, int mine, int stages) {
+  return j >= mine ? 0 : mine - j < stages ? mine - j : stages;
+}
+
 }  // namespace bq4

@@ -14,6 +14,7 @@ extern "C" void slots(int from, int to, int range, int grid, int* out) {
   const bq4::CacheSlots s = bq4::cache_slots(from, to, range, grid);
   out[0] = s.first, out[1] = s.count;
 }
+extern "C" int pending(int j, int mine, int stages) { return bq4::cache_pending(j, mine, stages); }
 """
 
 
@@ -49,3 +50,19 @@ def test_whatever_the_workspace_holds_the_slots_exist(bounds):
                 for z in some:
                     first, count = slots(bounds, a, z, range_, grid)
                     assert range_ <= first and 1 <= count and first + count <= range_ + grid
+
+
+def test_every_copy_under_way_is_waited_for(bounds):
+    # the ring as the kernel drives it: stages - 1 fetches ahead, one more at the start of each step
+    for stages in range(2, 9):
+        for mine in range(20):
+            for fails in range(mine + 1):
+                issued = min(mine, stages - 1)
+                waited = 0
+                for j in range(mine):
+                    if j + stages - 1 < mine:
+                        issued += 1
+                    if j == fails:
+                        break
+                    waited += 1
+                assert bounds.pending(fails, mine, stages) == issued - waited
