@@ -167,8 +167,9 @@ __global__ void __launch_bounds__(kCThreads) cache_append_kernel(const __grid_co
   item /= (unsigned)a.c.kv_heads;
   const int b = (int)(item / (unsigned)a.steps), step = (int)(item - (unsigned)b * a.steps);
   const int end = seq_length(a.s, a.c.page_size, b, a.err), from = end - a.tokens, first = max(from, 0);
-  const int base = (first & ~(kTake - 1)) + kTake * step;
-  if (base >= end) return;
+  const int64_t from_here = (first & ~(kTake - 1)) + (int64_t)kTake * step;  // the last steps may pass 2^31
+  if (from_here >= end) return;
+  const int base = (int)from_here;
   int place0;
   const int page = page_of(a.c, a.s, b, base, &place0, a.err);
   if (page < 0) return;
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(kCThreads) cache_read_kernel(const __grid_cons
   item >>= 1;
   const int b = (int)(item / (unsigned)a.c.kv_heads), head = (int)(item - (unsigned)b * a.c.kv_heads);
   const int64_t start = a.starts ? (int64_t)a.starts[b] : 0;
-  const int64_t base = (start & ~(int64_t)(kTake - 1)) + kTake * step, to = start + a.count;
+  const int64_t base = (start & ~(int64_t)(kTake - 1)) + (int64_t)kTake * step, to = start + a.count;
   if (base >= to) return;
   const int end = seq_length(a.s, a.c.page_size, b, a.err);
   int place0 = 0, page = -1;

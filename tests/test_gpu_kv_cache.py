@@ -642,3 +642,19 @@ def test_same_bits_every_time():
     for _ in range(5):
         assert torch.equal(one, book.cache.attention(q, book.table, book.lengths))
         assert torch.equal(two, book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths))
+
+
+def test_more_tokens_than_a_cache_holds():
+    # 2^31 - 8 rows given (one row, expanded), of which the cache keeps the last 5
+    c = KVCache(2, 16, 1, 8, "f16", DEV)
+    c.data.fill_(0x5A)
+    before = c.data.clone()
+    x = torch.randn((1, 1, 1, 8), generator=torch.Generator(device=DEV).manual_seed(5), device=DEV)
+    many = x.expand(1, 2 ** 31 - 8, 1, 8)
+    table = torch.tensor([[1]], dtype=torch.int32, device=DEV)
+    c.append(many, -many, table, torch.tensor([5], dtype=torch.int32, device=DEV))
+    q4.poll_device_error()
+    for got, want in zip(c.read(table, torch.tensor([5], dtype=torch.int32, device=DEV), 5), (x, -x)):
+        assert torch.equal(got, want.half().expand(1, 1, 5, 8))
+    half = c.data.numel() // 2
+    assert torch.equal(c.data[:half], before[:half])  # page 0 stayed as it was
