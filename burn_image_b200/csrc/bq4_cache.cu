@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kCThreads) cache_append_kernel(const __grid_co
   constexpr int kRow = kFmt == BQ4_CACHE_F16 ? 2 * kHP : kFmt == BQ4_CACHE_Q8 ? kHP : kHP / 2;
   constexpr int kNb = kFmt == BQ4_CACHE_Q8 ? 1 : kHP / kCacheBlock;
   const int lane = threadIdx.x & 31, L = lane % kLanes, sub = lane / kLanes, d0 = kW * L;
-  unsigned item = (blockIdx.x * kCThreads + threadIdx.x) >> 5;
+  unsigned item = blockIdx.x * (kCThreads / 32) + (threadIdx.x >> 5);
   if (item >= a.items) return;
   // kv, then head, fastest: neighbouring warps read neighbouring rows
   const int kv = item & 1;
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kCThreads) cache_read_kernel(const __grid_cons
   constexpr int kHeld = kFmt == BQ4_CACHE_F16 ? 2 * kW : kFmt == BQ4_CACHE_Q8 ? kW : kW / 2;  // bytes of kW values
   constexpr int kWords = kHeld < 4 ? 1 : kHeld / 4;
   const int lane = threadIdx.x & 31, L = lane % kLanes, sub = lane / kLanes, d0 = kW * L;
-  unsigned item = (blockIdx.x * kCThreads + threadIdx.x) >> 5;
+  unsigned item = blockIdx.x * (kCThreads / 32) + (threadIdx.x >> 5);
   if (item >= a.items) return;
   const int step = (int)(item % (unsigned)a.steps);
   item /= (unsigned)a.steps;

@@ -658,3 +658,21 @@ def test_more_tokens_than_a_cache_holds():
         assert torch.equal(got, want.half().expand(1, 1, 5, 8))
     half = c.data.numel() // 2
     assert torch.equal(c.data[:half], before[:half])  # page 0 stayed as it was
+
+
+def test_more_warps_than_32_bits_of_threads():
+    # one row of each of 2^26 + 8 sequences, k and v: 2^27 + 16 warps.  All but the last sequence are empty.
+    B = 2 ** 26 + 8
+    c = KVCache(2, 16, 1, 8, "f16", DEV)
+    x = torch.randn((1, 1, 1, 8), generator=torch.Generator(device=DEV).manual_seed(6), device=DEV).half()
+    table = torch.ones((1, 1), dtype=torch.int32, device=DEV).expand(B, 1)
+    lengths = torch.zeros(B, dtype=torch.int32, device=DEV)
+    lengths[-1] = 1
+    c.append(x.expand(B, 1, 1, 8), -x.expand(B, 1, 1, 8), table, lengths)
+    k, v = c.read(table[:1], lengths[-1:], 1)
+    assert torch.equal(k[0, 0, 0], x[0, 0, 0]) and torch.equal(v[0, 0, 0], -x[0, 0, 0])
+    outs = c.read(table, lengths, 1)
+    q4.poll_device_error()
+    for got, want in zip(outs, (x, -x)):
+        assert torch.equal(got[-1, 0, 0], want[0, 0, 0])
+        assert not got[:-1].any()
