@@ -581,8 +581,8 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
 
       // ---- z = x - base, x in log2 units; a masked key's is -inf
       const float c0 = kFmt == BQ4_CACHE_Q8 ? sk[0][0] * c : c, c1 = kFmt == BQ4_CACHE_Q8 ? sk[1][0] * c : c;
-      // log2 of the keys' largest v scales; not below -100, so that p stays in f32's range beside
-      // a v of 0
+      // log2 of the keys' largest v scales; not below -64, so that beside a v of 0 the sum of 2^30
+      // p of at most 2^(14 + 64) stays in f32 (scales below that are 0 in an f16 result)
       float lg[2] = {0.0f, 0.0f};
       if constexpr (Y::kQ) {
 #pragma unroll
@@ -590,7 +590,7 @@ __global__ void __launch_bounds__(kSThreads, Layout<kFmt, kHP>::per_sm(kNT))
           float top = sv[r][0];
 #pragma unroll
           for (int e = 1; e < Y::kNb; ++e) top = fmaxf(top, sv[r][e]);
-          lg[r] = fmaxf(lg2(top), -100.0f);
+          lg[r] = fmaxf(lg2(top), -64.0f);
         }
       }
       float z[kNT][4];

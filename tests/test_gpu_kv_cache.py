@@ -676,3 +676,17 @@ def test_more_warps_than_32_bits_of_threads():
     for got, want in zip(outs, (x, -x)):
         assert torch.equal(got[-1, 0, 0], want[0, 0, 0])
         assert not got[:-1].any()
+
+
+def test_many_keys_with_values_of_zero():
+    # 40 million keys of k = v = 0 (rows that nothing wrote) and one with a value: the sum of their
+    # probabilities, as large as a v scale of 0 lets them be, stays in f32
+    n, page = 40_000_000, 65536
+    c = KVCache(-(-n // page), page, 1, 8, "q8", DEV)
+    table = torch.arange(c.pages, dtype=torch.int32, device=DEV)[None]
+    length = torch.tensor([n], dtype=torch.int32, device=DEV)
+    v = torch.linspace(-6e4, 6e4, 8, device=DEV)[None, None, None]
+    c.append(torch.zeros_like(v), v, table, length)
+    q = torch.ones((1, 1, 2, 8), device=DEV).half()
+    exact = (held(v, "q8") / n).expand(1, 1, 2, 8)
+    check(c.attention(q, table, length), exact, exact.abs(), 0.0)
