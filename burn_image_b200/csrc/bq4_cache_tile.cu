@@ -12,12 +12,14 @@
 //           (8 bits), q s_b / s (4 bits: s the power of two above the row's
 //           scales, the product has 11 bits and is exact), or the rows (f16);
 //   v tile  [2][hp][64 keys] f16 (transposed), 128-byte swizzle: q s_v 2^-e,
-//           rounded once (2^-11 of it; exact for 4 bits and f16);
+//           rounded once (2^-11 of it; exact for 4 bits and f16), with the key's own
+//           e, 0 unless its v pass 2^15 (one of a whole record would take the others'
+//           bits, of rows that do not see that key too);
 //   consts  per key the factor ck that turns its raw score into log2 units (s_k,
-//           s or 1, times scale log2(e)) and lv = 0, or -inf for a row that does
-//           not exist; the record's e, 0 unless its v pass 2^15, and whether
-//           some lv is -inf.  (k rounded to f16 instead, without a factor a
-//           score, gained 7 %: not worth its error.)
+//           s or 1, times scale log2(e)), lv = e, or -inf for a row that does
+//           not exist, and w = 2^-e; whether some lv is not 0 and some e is not.
+//           (k rounded to f16 instead, without a factor a score, gained 7 %: not
+//           worth its error.)
 // A visible v row with a value that is not finite would carry 0 * NaN into the
 // rows that do not see it: it is stored as 0 and its key gets ck = NaN, so that
 // every output of a row that sees it is NaN.
@@ -26,8 +28,8 @@
 //   warp 0        bulk copies of the records (2 stages), q tiles once
 //   warp 1        S_t = q_t k^T and O_t += P_t v for the two 128-row tiles in
 //                 turn, so that one tile's softmax runs beside the other's products
-//   warps 4..11   a thread a row: y = S ck (+ lv), p = 2^(y + e - m) as f16 into
-//                 TMEM, l += p 2^-e; O is rescaled only when some p would
+//   warps 4..11   a thread a row: y = S ck (+ lv), p = 2^(y - m) as f16 into
+//                 TMEM, l += p (w); O is rescaled only when some p would
 //                 pass 2^14
 // Every wait is bounded (BQ4_ETIMEOUT), as in bq4_attn_fused.cu.
 //
@@ -55,7 +57,7 @@ namespace {
 constexpr int kKeys = 128;                   // keys of a record
 constexpr int kTThreads = 384;
 constexpr int kRing = 2;                     // stages of k and of v
-constexpr uint32_t kConsts = kKeys * 8 + 16;  // bytes of a record's consts
+constexpr uint32_t kConsts = kKeys * 12 + 16;  // bytes of a record's consts
 constexpr float kTNone = -1e30f;             // the maximum of no score
 // log2 units: m is set 2^6 below the maximum and moves when p would pass 2^14, so
 // that f16 holds p to its 2^-11 down to 2^-20 of the row's largest (a small p
@@ -63,10 +65,9 @@ constexpr float kTNone = -1e30f;             // the maximum of no score
 constexpr float kTHead = 6.0f, kTJump = 14.0f;
 
 struct Consts {
-  float ck[kKeys], lv[kKeys];
-  float e;
-  int partial;
-  int pad[2];
+  float ck[kKeys], lv[kKeys], w[kKeys];
+  int flags;  // 1: some lv is not 0; 2: some e is not
+  int pad[3];
 };
 static_assert(sizeof(Consts) == kConsts, "a record's consts are copied in 16-byte units");
 
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
   __shared__ int64_t at[kKeys];                // byte of the key's step in the cache, -1: no such row
   __shared__ int place[kKeys];
   __shared__ float sk[kKeys][kNb], sv[kKeys][kNb], ck[kKeys];
-  __shared__ float top[4];
+  __shared__ int flags[4];
   __shared__ uint16_t vt[kKeys * kPitch];
   const int64_t rec = blockIdx.x;
   const int j = (int)(rec % s.blocks);
@@ -160,7 +161,8 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
   if (tid < kKeys) {
     const int pos = j * kKeys + tid;
     int64_t where = -1;
-    float most = 0.0f, f = s.c;
+    float f = s.c;
+    int e_v = 0;
     if (pos < n) {
       const unsigned u = (unsigned)pos / kCachePageUnit;
       const int pi = (int)((u * s.page_magic) >> 38);
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
         where = step - c.data;
         if constexpr (kFmt != BQ4_CACHE_F16) {
           const uint16_t* sc = reinterpret_cast<const uint16_t*>(step + 32 * kRow) + (place[tid] & 15) * 2 * kNb;
-          float ktop = 0.0f;
+          float ktop = 0.0f, most = 0.0f;
           bool odd = false;
 #pragma unroll
           for (int e = 0; e < kNb; ++e) {
@@ -194,6 +196,11 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
             for (int e = 0; e < kNb; ++e) sk[tid][e] = odd ? 0.0f : sk[tid][e] * (1.0f / up);
           }
           if (odd) f = __int_as_float(0x7fc00000);
+          // |v| < 2^15 after the factor 2^-e
+          most *= kFmt == BQ4_CACHE_Q8 ? 127.0f : 7.0f;
+          if (most >= 0x1p15f) e_v = min((int)(__float_as_uint(most) >> 23) - 127 + 1 - 15, 120);
+#pragma unroll
+          for (int e = 0; e < kNb; ++e) sv[tid][e] *= __uint_as_float((uint32_t)(127 - e_v) << 23);
         }
       } else {
         atomicCAS(s.a.err, 0, (int)BQ4_EINVAL_ARG);
@@ -201,24 +208,13 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
     }
     at[tid] = where;
     ck[tid] = where < 0 ? 0.0f : f;
-    s.consts[rec].lv[tid] = where < 0 ? -INFINITY : 0.0f;
-#pragma unroll
-    for (int w = 16; w; w >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
-    if ((tid & 31) == 0) top[tid >> 5] = most;
+    s.consts[rec].lv[tid] = where < 0 ? -INFINITY : (float)e_v;
+    s.consts[rec].w[tid] = __uint_as_float((uint32_t)(127 - e_v) << 23);
+    const bool weighted = __any_sync(0xffffffffu, e_v > 0), partial = __any_sync(0xffffffffu, where < 0);
+    if ((tid & 31) == 0) flags[tid >> 5] = weighted ? 3 : partial ? 1 : 0;
   }
-  const int gone = __syncthreads_or(tid < kKeys && at[tid] < 0);
-  // v of this block: |v| < 2^15 after the factor 2^-e
-  float unit = 1.0f;
-  if constexpr (kFmt != BQ4_CACHE_F16) {
-    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * (kFmt == BQ4_CACHE_Q8 ? 127.0f : 7.0f);
-    int e = 0;
-    if (most >= 0x1p15f) e = min((int)(__float_as_uint(most) >> 23) - 127 + 1 - 15, 120);
-    unit = __uint_as_float((uint32_t)(127 - e) << 23);
-    if (tid == 0) s.consts[rec].e = (float)e;
-  } else {
-    if (tid == 0) s.consts[rec].e = 0.0f;
-  }
-  if (tid == 0) s.consts[rec].partial = gone;
+  __syncthreads();
+  if (tid == 0) s.consts[rec].flags = flags[0] | flags[1] | flags[2] | flags[3];
 
   uint8_t* kd = s.k + rec * kTile;
 #pragma unroll 4
@@ -247,7 +243,7 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
         if constexpr (kFmt == BQ4_CACHE_Q8) {
           const uint2 a = *reinterpret_cast<const uint2*>(kr + cache_swizzle(0, kRow, pl, 8 * ch));
           const uint2 b = *reinterpret_cast<const uint2*>(vr + cache_swizzle(1, kRow, pl, 8 * ch));
-          const float w = sv[key][0] * unit;
+          const float w = sv[key][0];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             kx[e] = (float)((int)((e < 4 ? a.x : a.y) >> 8 * (e & 3) & 255) - 128);
@@ -257,7 +253,7 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
           const int blk = ch >> 2;
           const uint32_t a =
               *reinterpret_cast<const uint32_t*>(kr + cache_swizzle(0, kRow, pl, 4 * ((ch & 3) * kNb + blk)));
-          const float wk = sk[key][blk], wv = sv[key][blk] * unit;
+          const float wk = sk[key][blk], wv = sv[key][blk];
           uint32_t b = 0;
 #pragma unroll
           for (int h = 0; h < 2; ++h)
@@ -346,8 +342,10 @@ __device__ __forceinline__ float scores64(uint32_t (&r)[64], const Consts* k, in
   return fmaxf(mp[0], mp[1]);
 }
 
-// p = 2^(y + shift) of 64 keys as f16 pairs into 32 TMEM columns; returns their sum.
-__device__ __forceinline__ float probs64(const uint32_t (&r)[64], float shift, uint32_t t_p) {
+// p = 2^(y + shift) of 64 keys as f16 pairs into 32 TMEM columns; returns their sum, of
+// kWeighted each times its key's w.
+template <bool kWeighted>
+__device__ __forceinline__ float probs64(const uint32_t (&r)[64], float shift, uint32_t t_p, const float* w) {
   const uint64_t s2 = attn_pack2(shift, shift);
   uint64_t acc[2] = {0, 0};
 #pragma unroll
@@ -359,7 +357,11 @@ __device__ __forceinline__ float probs64(const uint32_t (&r)[64], float shift, u
       attn_unpack2(attn_add2(attn_pack2(__uint_as_float(r[16 * cc + i]), __uint_as_float(r[16 * cc + i + 1])), s2),
                    x0, x1);
       const float p0 = attn_ex2(x0), p1 = attn_ex2(x1);
-      acc[(i >> 1) & 1] = attn_add2(acc[(i >> 1) & 1], attn_pack2(p0, p1));
+      if constexpr (kWeighted)
+        acc[(i >> 1) & 1] = attn_fma2(attn_pack2(p0, p1), *reinterpret_cast<const uint64_t*>(w + 16 * cc + i),
+                                      acc[(i >> 1) & 1]);
+      else
+        acc[(i >> 1) & 1] = attn_add2(acc[(i >> 1) & 1], attn_pack2(p0, p1));
       const __half2 hp = __floats2half2_rn(p0, p1);
       pk[i >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
     }
@@ -572,15 +574,16 @@ __global__ void __launch_bounds__(kTThreads, 1) cache_tile_kernel(const __grid_c
       ptx::tc_fence_after();
       const Consts* k = &consts[st];
       const int valid = see - (j0 + j) * kKeys;
-      const float e = k->e;
-      const bool plain = !k->partial && __all_sync(0xffffffffu, valid >= kKeys);
+      const int flags = k->flags;
+      const bool weighted = flags & 2;
+      const bool plain = !flags && __all_sync(0xffffffffu, valid >= kKeys);
       attn_ld64(t_s, r);
       float top = plain ? scores64<true>(r, k, 0, valid) : scores64<false>(r, k, 0, valid);
 #pragma unroll
       for (int i = 0; i < 64; i += 16)  // y of keys 0..63 goes back over S until the P pass
         ptx::tmem_st_32x32b_x16(t_s + i, *reinterpret_cast<uint32_t(*)[16]>(r + i));
       attn_ld64(t_s + 64, r);  // kept for the P pass
-      top = fmaxf(top, plain ? scores64<true>(r, k, 64, valid) : scores64<false>(r, k, 64, valid)) + e;
+      top = fmaxf(top, plain ? scores64<true>(r, k, 64, valid) : scores64<false>(r, k, 64, valid));
       const bool jump = top > m + kTJump;
       const float m_use = jump ? top - kTHead : m;
       const float alpha = jump ? attn_ex2(m - m_use) : 1.0f;
@@ -597,15 +600,16 @@ __global__ void __launch_bounds__(kTThreads, 1) cache_tile_kernel(const __grid_c
         }
       }
       // keys 64..127 -> P columns 96..127 (S columns already read): their half of P v may start
-      float sum = probs64(r, e - m_use, t_s + 96);
+      float sum = weighted ? probs64<true>(r, -m_use, t_s + 96, k->w + 64)
+                           : probs64<false>(r, -m_use, t_s + 96, nullptr);
       ptx::tmem_st_wait();  // P (and a rescaled O) in TMEM before the MMA reads them
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&p_half[t]);
       // keys 0..63 (y stored above, and the wait for P's stores since) -> P columns 64..95
       attn_ld64(t_s, r);
-      sum += probs64(r, e - m_use, t_s + 64);
-      l = l * alpha + sum * attn_ex2(-e);
+      sum += weighted ? probs64<true>(r, -m_use, t_s + 64, k->w) : probs64<false>(r, -m_use, t_s + 64, nullptr);
+      l = l * alpha + sum;
       m = m_use;
       ptx::tmem_st_wait();
       ptx::tc_fence_before();

@@ -690,3 +690,36 @@ def test_many_keys_with_values_of_zero():
     q = torch.ones((1, 1, 2, 8), device=DEV).half()
     exact = (held(v, "q8") / n).expand(1, 1, 2, 8)
     check(c.attention(q, table, length), exact, exact.abs(), 0.0)
+
+
+@pytest.mark.parametrize("fmt", ["q8", "q4"])
+def test_large_values_that_a_query_does_not_see(fmt, path):
+    # f32 rows: the v of one of the newest tokens is far beyond f16, the others' are not.  Queries before it
+    # do not see it; to the others it is there with the weight that its score gives it.
+    n, S, late = 400, 64, 10
+    book = Book(fmt, [n, n], 1, 128, 32, seed=51)
+    for size in (1e12, 3e30):
+        v = book.v[0].clone()
+        x = torch.randn((1, 1, 1, 128), generator=book.g, device=DEV)
+        big = x * size
+        book.cache.append(x, big, book.table[:1], book.lengths[:1] - late + 1)
+        k = book.k[0].clone()
+        k[n - late], v[n - late] = held(x[0, 0], fmt), held(big[0, 0], fmt)
+        q = book.query(S, 4)
+        got = book.cache.attention(q, book.table, book.lengths)
+        q4.poll_device_error()
+        exact, mag, top = attend(q.double(), [k, book.k[1]], [v, book.v[1]], True)
+        check(got[:, :S - late], exact[:, :S - late], mag[:, :S - late], top, staged=True)
+        check(got[1:], exact[1:], mag[1:], top, staged=True)
+        assert not got[0, S - late:].isfinite().all()
+    # seen, with a weight of 2^-43: 2^40 in its place adds 2^-3 to every output
+    k = torch.zeros((1, 1, 1, 128), device=DEV)
+    k[..., 0] = -30 * 128 ** 0.5
+    v = torch.full((1, 1, 1, 128), 2.0 ** 40, device=DEV)
+    book.cache.append(k, v, book.table[:1], book.lengths[:1] - late + 1)
+    k0, v0 = book.k[0].clone(), book.v[0].clone()
+    k0[n - late], v0[n - late] = held(k[0, 0], fmt), held(v[0, 0], fmt)
+    q = torch.zeros_like(book.query(S, 4))
+    q[..., 0] = 1.0
+    got = book.cache.attention(q, book.table, book.lengths)
+    check(got, *attend(q.double(), [k0, book.k[1]], [v0, book.v[1]], True), staged=True)
