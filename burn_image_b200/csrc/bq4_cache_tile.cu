@@ -474,11 +474,13 @@ __global__ void __launch_bounds__(kTThreads, 1) cache_tile_kernel(const __grid_c
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // the records and q tiles of the kernel before: every role waits for it here, since the bounded
+  // waits below would count its time (and that of a kernel it was launched beside) as theirs
+  ptx::griddep_wait();
 
   if (warp == 0) {
     if (lane == 0) {
       // ------------------------------------------------ copies
-      ptx::griddep_wait();  // the records and q tiles of the kernel before
       ptx::mbar_arrive_expect_tx(q_full, nt * kTile);
       for (int t = 0; t < nt; ++t)
         ptx::bulk_load(qs + t * kTile, s.q + (head * 2 * s.tiles + 2 * rt + t) * kTile, kTile, q_full);
