@@ -603,7 +603,7 @@ bq4_status attention(const bq4_cache* cache, const int32_t* prefix_pages, int64_
   if (seqs->batch == 0 || tokens == 0) return BQ4_OK;
   if (!q || !q_strides || !out) return set_error(BQ4_EINVAL_ARG, "q/q_strides/out is NULL");
   if (!al(q, 2) || !al(out, 16)) return set_error(BQ4_EALIGN, "q misaligned or out not 16-byte aligned");
-  if (!(scale == scale)) return set_error(BQ4_EINVAL_ARG, "scale is NaN");
+  if (!(scale <= 3.402823466e38f)) return set_error(BQ4_EINVAL_ARG, "scale is NaN or infinite");
   st = device_ready(cache->device);
   if (st) return st;
   Guard guard(cache->device);

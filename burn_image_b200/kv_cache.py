@@ -18,6 +18,7 @@ fallback.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -161,7 +162,7 @@ class KVCache:
         h // (q_heads // kv_heads).  causal: query i of sequence b sees
         positions below lengths[b] - S + i + 1, else every row.  A query that
         sees nothing gives 0.  Returns float16 [B, S, q_heads, head_dim].
-        scale None: 1 / sqrt(head_dim).  max_length: a bound of the lengths
+        scale: positive; None: 1 / sqrt(head_dim).  max_length: a bound of the lengths
         known to the host, by which the keys are split (None: the page
         table's width)."""
         return self._attention(query, None, None, page_table, lengths, causal, scale, max_length, out)
@@ -184,6 +185,9 @@ class KVCache:
         q = self._rows(query, "query", None)
         if q.dtype is not torch.float16:
             raise Bq4Error(L.EINVAL_ARG, "query must be float16")
+        # (the library takes a scale of 0 or less for the default)
+        if scale is not None and not 0.0 < ctypes.c_float(scale).value < math.inf:
+            raise Bq4Error(L.EINVAL_ARG, f"scale={scale} is not a positive float32 (None: 1 / sqrt(head_dim))")
         shape = q.shape
         seqs = self._sequences(page_table, lengths, shape[0])
         if out is None:

@@ -723,3 +723,14 @@ def test_large_values_that_a_query_does_not_see(fmt, path):
     q[..., 0] = 1.0
     got = book.cache.attention(q, book.table, book.lengths)
     check(got, *attend(q.double(), [k0, book.k[1]], [v0, book.v[1]], True), staged=True)
+
+
+def test_scales_that_are_refused():
+    book = Book("q8", [20], 2, 128, 16)
+    q = book.query(1, 4)
+    for scale in (0.0, -0.0, -1.0, math.inf, -math.inf, math.nan, 1e39, 1e-60):
+        with pytest.raises(Bq4Error, match="scale"):
+            book.cache.attention(q, book.table, book.lengths, scale=scale)
+        with pytest.raises(Bq4Error, match="scale"):
+            book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths, scale=scale)
+    run_attention(book, 1, 4, scale=1)

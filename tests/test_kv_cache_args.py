@@ -141,3 +141,9 @@ def test_python_refuses_what_it_cannot_take():
         KVCache(4, 20, 2, 128)
     with pytest.raises(Bq4Error, match="CUDA device"):
         KVCache(4, 16, 2, 128, device="cpu")
+
+
+def test_an_infinite_scale_is_refused():
+    for scale in (float("inf"), 1e39):
+        assert attention(scale=scale) == L.EINVAL_ARG
+        assert b"scale" in L.lib().bq4_last_error_string()
