@@ -48,6 +48,9 @@ class KVCache:
                  device: Optional[torch.device] = None):
         if format not in FORMATS:
             raise Bq4Error(L.EINVAL_ARG, f"format {format!r} is not one of {', '.join(FORMATS)}")
+        for what, size in (("pages", pages), ("page_size", page_size), ("kv_heads", kv_heads), ("head_dim", head_dim)):
+            if not 0 < size < 2 ** 31:  # a ctypes field would keep its low bits
+                raise Bq4Error(L.EINVAL_SHAPE, f"{what}={size} must be in [1, 2^31)")
         c = L.Cache(None, pages, page_size, kv_heads, head_dim, FORMATS[format], 0)
         n = ctypes.c_size_t()
         check(L.lib().bq4_cache_size(ctypes.byref(c), ctypes.byref(n)))
@@ -213,11 +216,11 @@ class KVCache:
         """Bound of the lengths and workspace bytes of an attention call of these sizes."""
         (B, S, Hq, D), table_width, width, max_length = key
         held = table_width * self.page_size
-        longest = held if max_length is None else max_length
+        longest = held if max_length is None else min(max_length, held)
         if longest < 0:
             raise Bq4Error(L.EINVAL_SHAPE, f"max_length={max_length}")
         n = ctypes.c_size_t()
-        check(self._lib.bq4_cache_attention_workspace_size(self._ref, B, S, Hq, min(longest, held) or held,
+        check(self._lib.bq4_cache_attention_workspace_size(self._ref, B, S, Hq, longest or held,
                                                            width * self.page_size, ctypes.byref(n)))
         if len(self._plans) >= 1024:
             self._plans.clear()

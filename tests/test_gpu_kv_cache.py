@@ -734,3 +734,12 @@ def test_scales_that_are_refused():
         with pytest.raises(Bq4Error, match="scale"):
             book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths, scale=scale)
     run_attention(book, 1, 4, scale=1)
+
+
+def test_a_bound_past_64_bits_is_the_page_tables():
+    book = Book("q8", [40, 20], 2, 128, 16)
+    q = book.query(1, 4)
+    want = book.cache.attention(q, book.table, book.lengths)
+    for bound in (2 ** 64 + 5, 2 ** 63, 2 ** 31):
+        assert torch.equal(book.cache.attention(q, book.table, book.lengths, max_length=bound), want)
+    q4.poll_device_error()

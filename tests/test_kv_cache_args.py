@@ -147,3 +147,12 @@ def test_an_infinite_scale_is_refused():
     for scale in (float("inf"), 1e39):
         assert attention(scale=scale) == L.EINVAL_ARG
         assert b"scale" in L.lib().bq4_last_error_string()
+
+
+@pytest.mark.parametrize("what", ["pages", "page_size", "kv_heads", "head_dim"])
+def test_sizes_past_their_c_fields_are_refused(what):
+    for size in (2 ** 64 + 16, 2 ** 32 + 16, 2 ** 31, 0, -16):
+        sizes = dict(pages=4, page_size=16, kv_heads=2, head_dim=128)
+        sizes[what] = size
+        with pytest.raises(Bq4Error, match=what):
+            KVCache(**sizes)
