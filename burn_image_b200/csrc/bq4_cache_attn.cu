@@ -957,12 +957,18 @@ struct SplitPlan {
 };
 
 // Rows of a warp, in eights: a step costs about as much for its widening as for
-// 16 rows, so the tiles are those that cost least together (24 rows as one tile
-// 25.5 us, as two of 16 27.1).
-int row_tile(int64_t rows) {
+// 16 rows, so the tiles are those that cost least together, over the keys of the
+// prefix and of the sequences (24 rows as one tile 25.5 us, as two of 16 27.1; 128
+// single tokens on 2000 rows in 4 bits behind 16 shared ones, where the prefix's 512
+// rows alone would take three, 204 -> 95).
+int row_tile(int64_t own, int64_t own_keys, int64_t all, int64_t prefix_keys) {
   int best = 1;
-  for (int nt = 2; nt <= 3; ++nt)
-    if ((rows + 8 * nt - 1) / (8 * nt) * (2 + nt) < (rows + 8 * best - 1) / (8 * best) * (2 + best)) best = nt;
+  double least = 0.0;
+  for (int nt = 1; nt <= 3; ++nt) {
+    const double cost = (2.0 + nt) * ((double)((own + 8 * nt - 1) / (8 * nt)) * (double)own_keys +
+                                      (double)((all + 8 * nt - 1) / (8 * nt)) * (double)prefix_keys);
+    if (nt == 1 || cost < least) best = nt, least = cost;
+  }
   return best;
 }
 
@@ -972,7 +978,8 @@ bool plan_split(const CacheAttnCall& a, int sms, SplitPlan* p) {
   const int group = a.q_heads / a.c.kv_heads;
   const int64_t own = (int64_t)a.tokens * group, all = own * a.s.batch;
   const int64_t prefix = (int64_t)a.prefix_width * a.c.page_size;
-  p->nt = row_tile(prefix > 0 ? all : own);
+  constexpr int64_t kStart = kLead * kUnit;  // keys that a range's start and end count for
+  p->nt = row_tile(own, a.max_length ? a.s.batch * (a.max_length + kStart) : 0, all, prefix ? prefix + kStart : 0);
   const int tile = 8 * p->nt;
   p->s_tiles = (int)((own + tile - 1) / tile);
   p->p_tiles = prefix > 0 ? (int)((all + tile - 1) / tile) : 0;

@@ -22,12 +22,14 @@ The kernels for many rows a kv head also round the widened v of an 8-bit cache t
 f16 (at most half a step, 2^-11 of each value): where `staged` is given, another
 2^-11 a.  BQ4_CACHE_TILE=1 takes them for every call, 0 for none.
 """
+import ctypes
 import math
 
 import pytest
 import torch
 
 from burn_image_b200 import KVCache, q4
+from burn_image_b200 import _lib as L
 from burn_image_b200 import f16 as F
 from burn_image_b200.q4 import Bq4Error
 
@@ -743,3 +745,16 @@ def test_a_bound_past_64_bits_is_the_page_tables():
     for bound in (2 ** 64 + 5, 2 ** 63, 2 ** 31):
         assert torch.equal(book.cache.attention(q, book.table, book.lengths, max_length=bound), want)
     q4.poll_device_error()
+
+
+def test_a_short_prefix_keeps_the_row_tile():
+    # 128 single tokens: the 512 rows that share 16 keys do not make the sequences' own 4 rows run in
+    # tiles of 24, whose partial results the workspace would have to hold
+    c = KVCache(4, 16, 8, 128, "q4", DEV)
+    n = ctypes.c_size_t()
+
+    def size(prefix):
+        L.check(L.lib().bq4_cache_attention_workspace_size(ctypes.byref(c._c), 128, 1, 32, 2000, prefix, ctypes.byref(n)))
+        return n.value
+
+    assert size(16) < 1.5 * size(0)
