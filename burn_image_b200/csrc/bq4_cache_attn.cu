@@ -16,7 +16,7 @@
 // covers are finished at once; cache_join_kernel joins the others: O = sum_c
 // 2^(m_c - M) O_c, l likewise, pieces in their order, so that a call gives the
 // same bits every time.  Calls with many rows a kv head run the kernels of
-// bq4_cache_tile.cu instead (use_tile).
+// bq4_cache_tile.cu instead (plan_cache).
 //
 // cache_split_kernel: four warps, each its own 16-key steps.
 //   * Keys are the M side of the tensor core's m16n8k16 (f16 in, f32 out) and
@@ -1052,27 +1052,53 @@ struct CachePlan {
 // Measured, 8 kv heads of 8 bits, split against tile: one sequence of 1000 keys,
 // 256 rows 18.0 / 21.4; of 4000 keys 96 rows 20.5 / 21.0, 256 rows 32.6 / 30.5; 16
 // sequences of 1000 keys 64 rows 40.5 / 46.8, 96 rows 51.7 / 47.2; of 4000 keys
-// 96 rows 132 / 152, 128 rows 191 / 152; 72 sequences of 8 keys behind 8
-// shared ones, 20 rows, 37 / 69 in all.  BQ4_CACHE_TILE=0 or 1 chooses for
-// every call whose workspace stays within 1 GB (tests).
-bool use_tile(const CacheAttnCall& a, bool prefix, int64_t rows, int64_t keys, int sms, CacheTilePlan* p) {
+// 96 rows 132 / 152, 128 rows 191 / 152.
+struct CacheCost {
+  double split, tile;  // without the 9 and 14 of the launches
+};
+constexpr double kSplitStart = 9.0, kTileStart = 14.0;
+CacheCost cost_of(const CacheAttnCall& a, bool prefix, int64_t rows, int64_t keys, int sms) {
   const double heads = (double)a.c.kv_heads * (prefix ? 1 : a.s.batch), all = heads * (double)keys;
-  const double split = 9.0 + 2.6e-6 * (double)rows * (all + 256.0 * heads);
   const double waves = std::ceil(heads * (double)((rows + 255) / 256) / sms);
-  const double tile = 14.0 + (230e-6 + 35e-6 * (double)((rows + 127) / 128)) * all + 7.0 * (waves - 1.0);
-  bool take = tile < split;
-  if (const char* f = getenv("BQ4_CACHE_TILE")) take = f[0] != '0';
-  return take && rows > 0 && keys > 0 && plan_cache_tile(a, prefix, sms, p) &&
-         p->workspace_bytes <= (size_t)1 << 30;
+  CacheCost c;
+  c.split = 2.6e-6 * (double)rows * (all + 256.0 * heads);
+  c.tile = (230e-6 + 35e-6 * (double)((rows + 127) / 128)) * all + 7.0 * (waves - 1.0);
+  return c;
 }
 
+// With a prefix a call is one of: the split kernel for every key; the tile kernels for the prefix and
+// the split kernel, beside their widening, for the sequences' own keys; the tile kernels for both.
+// The one of the least time as a whole is taken, each launch's start counted once: neither does a
+// short prefix keep long own keys from the tile kernels, nor do those take a prefix that does not
+// gain the launches that they add.  Measured over 432 calls (32 / 8 heads; 1 to 128 sequences of 1
+// to 200 tokens, 8 to 8192 own rows, 16 to 16384 shared ones) the rule's choice takes 1.013 times
+// the best one's time, at most 1.33 times (a rule for each part by itself: 1.039, 1.59).  The three
+// in us, 8 bits: 200 tokens on 8192 rows behind 16 shared ones 148 / 154 / 96; 72 x 5 on 8 behind 16
+// 38 / 46 / 70; 8 x 20 on 200 behind 300 30 / 45 / 46; 32 x 8 on 200 behind 4096 116 / 70 / 88; 128 x 1
+// on 8 behind 1000, where the rule is furthest off among the small ones, 38 / 31 / 100.
 bq4_status plan_cache(const CacheAttnCall& a, int sms, CachePlan* p) {
   const int group = a.q_heads / a.c.kv_heads;
   const int64_t own = (int64_t)a.tokens * group, all = own * a.s.batch;
   const int64_t prefix = (int64_t)a.prefix_width * a.c.page_size;
-  p->tile_s = use_tile(a, false, own, a.max_length, sms, &p->s);
-  p->tile_p = prefix > 0 && use_tile(a, true, all, prefix, sms, &p->p);
-  if (prefix > 0 && !p->tile_p) p->tile_s = false;  // the split kernel takes both or the sequences' own
+  const CacheCost cs = cost_of(a, false, own, a.max_length, sms), cp = cost_of(a, true, all, prefix, sms);
+  const bool has_p = prefix > 0;
+  double by_split = kSplitStart + cs.split + (has_p ? cp.split : 0.0);
+  double by_both = kSplitStart + kTileStart + cs.split + cp.tile;
+  double by_tile = kTileStart + cs.tile + (has_p ? kTileStart + cp.tile : 0.0);
+  // BQ4_CACHE_TILE (tests): 0 none, p for the prefix alone, else wherever a workspace stays within 1 GB
+  if (const char* f = getenv("BQ4_CACHE_TILE")) {
+    by_split = f[0] == '0' ? 0.0 : 3.0;
+    by_both = f[0] == '0' ? 3.0 : f[0] == 'p' ? 0.0 : 2.0;
+    by_tile = f[0] == '0' || f[0] == 'p' ? 3.0 : 1.0;
+  }
+  p->tile_p = p->tile_s = false;
+  auto fits = [&](bool pre, CacheTilePlan* t) {
+    return (pre ? prefix : a.max_length) > 0 && plan_cache_tile(a, pre, sms, t) &&
+           t->workspace_bytes <= (size_t)1 << 30;
+  };
+  if (has_p && (by_both < by_split || by_tile < by_split)) p->tile_p = fits(true, &p->p);
+  if ((!has_p || p->tile_p) && by_tile < (p->tile_p ? by_both : by_split)) p->tile_s = fits(false, &p->s);
+  if (p->tile_p && !p->tile_s && by_both >= by_split) p->tile_p = false;
   p->call = a;
   if (p->tile_p) p->call.prefix_width = 0, p->call.prefix_table = nullptr, p->call.prefix_length = nullptr;
   p->split_bytes = 0;

@@ -758,3 +758,44 @@ def test_a_short_prefix_keeps_the_row_tile():
         return n.value
 
     assert size(16) < 1.5 * size(0)
+
+
+def launches(call):
+    before = L.lib().bq4_launch_count()
+    out = call()
+    return out, L.lib().bq4_launch_count() - before
+
+
+def test_a_short_prefix_leaves_long_own_keys_to_the_many_row_kernels():
+    book = Book("q8", [3000], 8, 128, 16, prefix=16, seed=61)
+    q = book.query(200, 32)
+    got, alone = launches(lambda: book.cache.attention(q, book.table, book.lengths))
+    assert alone >= 2  # widening and products (the split kernel's call: itself and the join)
+    check(got, *attend(q.double(), book.k, book.v, True), staged=True)
+    got, n = launches(lambda: book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths))
+    assert n == 5  # both for the prefix, both for the own keys, the join
+    check(got, *attend(q.double(), book.k, book.v, True, book.pk, book.pv), staged=True)
+
+
+def test_a_prefix_takes_no_launches_that_it_does_not_gain():
+    book = Book("q8", [8] * 72, 8, 128, 16, prefix=16, seed=62)
+    q = book.query(5, 32)
+    got, n = launches(lambda: book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths))
+    assert n == 2  # the split kernel and the join
+    check(got, *attend(q.double(), book.k, book.v, True, book.pk, book.pv))
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8", "q4"])
+@pytest.mark.parametrize("S,page", [(1, 16), (7, 48), (40, 64)])
+def test_prefix_by_the_many_row_kernels_and_own_keys_by_the_split_kernel(fmt, S, page, monkeypatch):
+    # the two run beside each other; the join takes both
+    monkeypatch.setenv("BQ4_CACHE_TILE", "p")
+    book = Book(fmt, [0, 1, 500, S, 77, 263], 2, 128, page, prefix=700, seed=S, poison=True)
+    q = book.query(S, 8)
+    for causal in (True, False):
+        got, n = launches(lambda: book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths,
+                                                              causal=causal))
+        assert n == 4
+        check(got, *attend(q.double(), book.k, book.v, causal, book.pk, book.pv), staged=True)
+        assert torch.equal(got, book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths,
+                                                            causal=causal))
