@@ -844,6 +844,7 @@ struct JoinArgs {
   CacheAttnCall a;
   CacheJoinSource p, s;  // of the prefix and of the sequences' own keys
   int group, have_p, finish;
+  int first;  // sequences before a's in the batch whose rows the prefix's partial results are
 };
 
 // Slots of row r (of `rows`) of kv head kvh that sees `see` keys: first and number.
@@ -879,7 +880,7 @@ __global__ void __launch_bounds__(kSThreads) cache_join_kernel(const __grid_cons
   const int bi = (int)(row / (unsigned)a.q_heads), h = (int)row - bi * a.q_heads;
   const int b = bi / a.tokens, kvh = h / g.group, per = a.tokens * g.group;
   const int own = (bi - b * a.tokens) * g.group + h - kvh * g.group;  // row among the sequence's
-  const int all = b * per + own;                                     // among the prefix's
+  const int all = (g.first + b) * per + own;                         // among the prefix's
   int2 sp = make_int2(0, 0);
   if (g.have_p) sp = slots_of(g, g.p, 0, kvh, all, a.s.batch * per, prefix_rows(a), false);
   const int2 ss = slots_of(g, g.s, b, kvh, own, per, own_length(a, b), a.causal);
@@ -960,7 +961,7 @@ struct SplitPlan {
 // 16 rows, so the tiles are those that cost least together, over the keys of the
 // prefix and of the sequences (24 rows as one tile 25.5 us, as two of 16 27.1; 128
 // single tokens on 2000 rows in 4 bits behind 16 shared ones, where the prefix's 512
-// rows alone would take three, 204 -> 95).
+// rows alone would take three, 205 -> 91).
 int row_tile(int64_t own, int64_t own_keys, int64_t all, int64_t prefix_keys) {
   int best = 1;
   double least = 0.0;
@@ -1036,7 +1037,8 @@ cudaError_t launch_head(const SplitArgs& s, int nt, unsigned grid, cudaStream_t 
 // Which kernels take the prefix's and the sequences' own keys, and their workspaces.
 struct CachePlan {
   bool tile_p, tile_s;
-  CacheTilePlan p, s;
+  CacheTilePlan p, s;  // s: of `slice` sequences, one slice after the other
+  int slice;
   SplitPlan split;
   CacheAttnCall call;  // of the split kernel: without a prefix that the tile kernel takes
   size_t split_bytes, bytes;
@@ -1066,16 +1068,35 @@ CacheCost cost_of(const CacheAttnCall& a, bool prefix, int64_t rows, int64_t key
   return c;
 }
 
+// What the tile kernels may widen at a time.  A batch whose own keys take more runs in slices of its
+// sequences, one after the other in one workspace: 24 sequences of 512 tokens on 8192 rows, 32 / 8
+// heads of 8 bits, take 2.3 ms so, 7.3 on the split kernel; 64 sequences 5.6 and 20.4.
+constexpr size_t kTileWorkspace = (size_t)1 << 30;
+
+// The plan of the largest equal slices of the batch that fit; false: not even one sequence does.
+bool plan_slices(const CacheAttnCall& a, int sms, CacheTilePlan* t, int* slice) {
+  const int64_t batch = a.s.batch;
+  CacheAttnCall part = a;
+  for (int64_t n = 1;;) {
+    *slice = part.s.batch = (int)((batch + n - 1) / n);
+    const bool ok = plan_cache_tile(part, false, sms, t);
+    if (ok && t->workspace_bytes <= kTileWorkspace) return true;
+    if (part.s.batch == 1) return false;
+    const int64_t more = ok ? n * (int64_t)((t->workspace_bytes + kTileWorkspace - 1) / kTileWorkspace) : 2 * n;
+    n = std::min(batch, std::max(n + 1, more));
+  }
+}
+
 // With a prefix a call is one of: the split kernel for every key; the tile kernels for the prefix and
 // the split kernel, beside their widening, for the sequences' own keys; the tile kernels for both.
 // The one of the least time as a whole is taken, each launch's start counted once: neither does a
 // short prefix keep long own keys from the tile kernels, nor do those take a prefix that does not
 // gain the launches that they add.  Measured over 432 calls (32 / 8 heads; 1 to 128 sequences of 1
-// to 200 tokens, 8 to 8192 own rows, 16 to 16384 shared ones) the rule's choice takes 1.013 times
-// the best one's time, at most 1.33 times (a rule for each part by itself: 1.039, 1.59).  The three
-// in us, 8 bits: 200 tokens on 8192 rows behind 16 shared ones 148 / 154 / 96; 72 x 5 on 8 behind 16
-// 38 / 46 / 70; 8 x 20 on 200 behind 300 30 / 45 / 46; 32 x 8 on 200 behind 4096 116 / 70 / 88; 128 x 1
-// on 8 behind 1000, where the rule is furthest off among the small ones, 38 / 31 / 100.
+// to 200 tokens, 8 to 8192 own rows, 16 to 16384 shared ones) the rule's choice takes 1.015 times
+// the best one's time, at most 1.36 times (a rule for each part by itself: 1.046, 1.68).  The three
+// in us, 8 bits: 200 tokens on 8192 rows behind 16 shared ones 147 / 144 / 87; 72 x 5 on 8 behind 16
+// 38 / 46 / 70; 8 x 20 on 200 behind 300 28 / 44 / 44; 32 x 8 on 200 behind 4096 107 / 65 / 82; 128 x 1
+// on 8 behind 1000, one of those that the rule misses, 35 / 31 / 99.
 bq4_status plan_cache(const CacheAttnCall& a, int sms, CachePlan* p) {
   const int group = a.q_heads / a.c.kv_heads;
   const int64_t own = (int64_t)a.tokens * group, all = own * a.s.batch;
@@ -1085,19 +1106,18 @@ bq4_status plan_cache(const CacheAttnCall& a, int sms, CachePlan* p) {
   double by_split = kSplitStart + cs.split + (has_p ? cp.split : 0.0);
   double by_both = kSplitStart + kTileStart + cs.split + cp.tile;
   double by_tile = kTileStart + cs.tile + (has_p ? kTileStart + cp.tile : 0.0);
-  // BQ4_CACHE_TILE (tests): 0 none, p for the prefix alone, else wherever a workspace stays within 1 GB
+  // BQ4_CACHE_TILE (tests): 0 none, p for the prefix alone, else wherever a workspace fits
   if (const char* f = getenv("BQ4_CACHE_TILE")) {
     by_split = f[0] == '0' ? 0.0 : 3.0;
     by_both = f[0] == '0' ? 3.0 : f[0] == 'p' ? 0.0 : 2.0;
     by_tile = f[0] == '0' || f[0] == 'p' ? 3.0 : 1.0;
   }
   p->tile_p = p->tile_s = false;
-  auto fits = [&](bool pre, CacheTilePlan* t) {
-    return (pre ? prefix : a.max_length) > 0 && plan_cache_tile(a, pre, sms, t) &&
-           t->workspace_bytes <= (size_t)1 << 30;
-  };
-  if (has_p && (by_both < by_split || by_tile < by_split)) p->tile_p = fits(true, &p->p);
-  if ((!has_p || p->tile_p) && by_tile < (p->tile_p ? by_both : by_split)) p->tile_s = fits(false, &p->s);
+  p->slice = 0;
+  if (has_p && (by_both < by_split || by_tile < by_split))
+    p->tile_p = plan_cache_tile(a, true, sms, &p->p) && p->p.workspace_bytes <= kTileWorkspace;
+  if ((!has_p || p->tile_p) && by_tile < (p->tile_p ? by_both : by_split) && a.max_length > 0)
+    p->tile_s = plan_slices(a, sms, &p->s, &p->slice);
   if (p->tile_p && !p->tile_s && by_both >= by_split) p->tile_p = false;
   p->call = a;
   if (p->tile_p) p->call.prefix_width = 0, p->call.prefix_table = nullptr, p->call.prefix_length = nullptr;
@@ -1145,6 +1165,24 @@ bq4_status run_split(const CacheAttnCall& a, const SplitPlan& p, bool finish, vo
   return check_cuda(e, "cache attention launch");
 }
 
+bq4_status run_join(const JoinArgs& g, cudaStream_t stream) {
+  // launched ahead: it waits on the device for the partial results
+  cudaLaunchConfig_t cfg = {};
+  const unsigned rows = (unsigned)((int64_t)g.a.s.batch * g.a.tokens * g.a.q_heads);
+  const bool few = rows <= 1024;
+  cfg.gridDim = dim3(few ? rows : (rows + kSWarps - 1) / kSWarps);
+  cfg.blockDim = dim3(kSThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, few ? cache_join_kernel<kSWarps> : cache_join_kernel<1>, g, rows);
+  note_launch();
+  return check_cuda(e, "cache attention join launch");
+}
+
 }  // namespace
 
 bq4_status cache_attn_workspace(const CacheAttnCall& a, int sms, size_t* bytes) {
@@ -1180,26 +1218,22 @@ bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, cuda
     if (st) return st;
     ws += p.p.workspace_bytes;
   }
-  if (p.tile_s) {
-    const bool finish = alone && p.s.chunks == 1;
-    st = run_cache_tile(a, p.s, finish, false, ws, &g.s, stream);
-    if (st || finish) return st;
+  if (!p.tile_s) return run_join(g, stream);
+  const bool finish = alone && p.s.chunks == 1;
+  for (; g.first < a.s.batch; g.first += p.slice) {
+    CacheTilePlan t = p.s;
+    g.a.s.batch = t.sets = std::min(p.slice, a.s.batch - g.first);
+    t.records = (int64_t)t.sets * a.c.kv_heads * t.blocks;
+    t.q_tiles = (int64_t)t.sets * a.c.kv_heads * 2 * t.tiles;
+    g.a.s.table = a.s.table + g.first * a.s.table_stride;
+    g.a.s.lengths = a.s.lengths + g.first;
+    g.a.q = a.q + g.first * a.q_stride[0];
+    g.a.out = a.out + (int64_t)g.first * a.tokens * a.q_heads * a.c.head_dim;
+    st = run_cache_tile(g.a, t, finish, false, ws, &g.s, stream);
+    if (!st && !finish) st = run_join(g, stream);
+    if (st) return st;
   }
-  // the join is launched ahead and waits on the device for the partial results
-  cudaLaunchConfig_t cfg = {};
-  const unsigned rows = (unsigned)((int64_t)a.s.batch * a.tokens * a.q_heads);
-  const bool few = rows <= 1024;
-  cfg.gridDim = dim3(few ? rows : (rows + kSWarps - 1) / kSWarps);
-  cfg.blockDim = dim3(kSThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, few ? cache_join_kernel<kSWarps> : cache_join_kernel<1>, g, rows);
-  note_launch();
-  return check_cuda(e, "cache attention join launch");
+  return BQ4_OK;
 }
 
 }  // namespace bq4

@@ -799,3 +799,29 @@ def test_prefix_by_the_many_row_kernels_and_own_keys_by_the_split_kernel(fmt, S,
         check(got, *attend(q.double(), book.k, book.v, causal, book.pk, book.pv), staged=True)
         assert torch.equal(got, book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths,
                                                             causal=causal))
+
+
+@pytest.mark.parametrize("prefix", [0, 200])
+def test_a_batch_of_prompts_in_slices(prefix, monkeypatch):
+    # 37 sequences of 40 tokens on up to 8192 rows (the same pages, other lengths): their widened keys pass
+    # the workspace that one run may have, so that the batch runs in slices, the last of another size
+    monkeypatch.setenv("BQ4_CACHE_TILE", "1")
+    B, S, H, n = 37, 40, 8, 8192
+    book = Book("q8", [n], H, 128, 64, prefix=prefix, seed=71)
+    lengths = [n - 211 * i for i in range(B - 2)] + [0, 17]
+    table, t = book.table.expand(B, -1), torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    q = torch.randn((B, S, 2 * H, 128), generator=book.g, device=DEV).half()
+    q = q.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)  # not contiguous
+
+    def call():
+        if prefix:
+            return book.cache.prefix_attention(q, book.ptable, book.plen, table, t)
+        return book.cache.attention(q, table, t)
+
+    got, count = launches(call)
+    slices = (count - (2 if prefix else 0)) // 3
+    assert slices > 1 and B % slices and count == 3 * slices + (2 if prefix else 0)
+    assert torch.equal(got, call())
+    at = sorted({i for s in range(1, slices) for i in (s * -(-B // slices) - 1, s * -(-B // slices))} | {0, B - 2, B - 1})
+    ks, vs = ([x[0][:lengths[i]] for i in at] for x in (book.k, book.v))
+    check(got[at], *attend(q[at].double(), ks, vs, True, book.pk, book.pv), staged=True)
