@@ -608,12 +608,6 @@ bq4_status attention(const bq4_cache* cache, const int32_t* prefix_pages, int64_
   if (st) return st;
   Guard guard(cache->device);
   const int sms = device_sm_count(cache->device);
-  size_t need = 0;
-  st = cache_attn_workspace(call, sms, &need);
-  if (st) return st;
-  if (need > workspace_bytes || (need && !workspace))
-    return set_error(BQ4_EWORKSPACE, "workspace of %zu bytes; cache attention needs %zu", workspace_bytes, need);
-  if (need && !al(workspace, 256)) return set_error(BQ4_EALIGN, "workspace not 256-byte aligned");
   call.s = sv;
   call.prefix_table = prefix ? prefix_pages : nullptr;
   call.prefix_length = prefix ? prefix_length : nullptr;
@@ -624,7 +618,7 @@ bq4_status attention(const bq4_cache* cache, const int32_t* prefix_pages, int64_
   call.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)cache->head_dim);
   call.err = device_error_word();
   if (!call.err) return set_error(BQ4_ECUDA, "device error word unavailable");
-  return run_cache_attn(call, sms, workspace, stream);
+  return run_cache_attn(call, sms, workspace, workspace_bytes, stream);
 }
 
 }  // namespace

@@ -104,13 +104,15 @@ struct CacheTilePlan {
   int64_t records, q_tiles, slots;
   size_t tile_bytes, consts_bytes, q_bytes, part_bytes, ml_bytes, workspace_bytes;
 };
-bool plan_cache_tile(const CacheAttnCall& a, bool prefix, int sms, CacheTilePlan* p);
+// The best plan that `room` bytes hold; false: none does (workspace_bytes is what one needs at
+// least then), or the sizes are past the kernels' (workspace_bytes is 0).
+bool plan_cache_tile(const CacheAttnCall& a, bool prefix, int sms, size_t room, CacheTilePlan* p);
 // finish: there is one chunk and no other source, and the rows are finished.
 // beside: the kernel before on the stream is independent, and may run at the same time.
 bq4_status run_cache_tile(const CacheAttnCall& a, const CacheTilePlan& p, bool finish, bool beside, void* workspace,
                           CacheJoinSource* source, cudaStream_t stream);
 
 bq4_status cache_attn_workspace(const CacheAttnCall& c, int sms, size_t* bytes);
-bq4_status run_cache_attn(const CacheAttnCall& c, int sms, void* workspace, cudaStream_t s);
+bq4_status run_cache_attn(const CacheAttnCall& c, int sms, void* workspace, size_t workspace_bytes, cudaStream_t s);
 
 }  // namespace bq4

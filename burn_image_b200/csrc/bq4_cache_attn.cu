@@ -954,33 +954,16 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 struct SplitPlan {
   int nt, p_tiles, s_tiles, grid;
-  size_t part_bytes, ml_bytes, pieces_bytes;
+  size_t part_bytes, ml_bytes, pieces_bytes, bytes;
 };
 
-// Rows of a warp, in eights: a step costs about as much for its widening as for
-// 16 rows, so the tiles are those that cost least together, over the keys of the
-// prefix and of the sequences (24 rows as one tile 25.5 us, as two of 16 27.1; 128
-// single tokens on 2000 rows in 4 bits behind 16 shared ones, where the prefix's 512
-// rows alone would take three, 205 -> 91).
-int row_tile(int64_t own, int64_t own_keys, int64_t all, int64_t prefix_keys) {
-  int best = 1;
-  double least = 0.0;
-  for (int nt = 1; nt <= 3; ++nt) {
-    const double cost = (2.0 + nt) * ((double)((own + 8 * nt - 1) / (8 * nt)) * (double)own_keys +
-                                      (double)((all + 8 * nt - 1) / (8 * nt)) * (double)prefix_keys);
-    if (nt == 1 || cost < least) best = nt, least = cost;
-  }
-  return best;
-}
-
-// CTAs: what the GPU holds at a time, or fewer where the lengths' bounds give
-// fewer units.
-bool plan_split(const CacheAttnCall& a, int sms, SplitPlan* p) {
+// The plan with nt eights of rows a warp: CTAs are what the GPU holds at a time, or fewer
+// where the lengths' bounds give fewer units.
+bool plan_rows(const CacheAttnCall& a, int nt, int sms, SplitPlan* p) {
   const int group = a.q_heads / a.c.kv_heads;
   const int64_t own = (int64_t)a.tokens * group, all = own * a.s.batch;
   const int64_t prefix = (int64_t)a.prefix_width * a.c.page_size;
-  constexpr int64_t kStart = kLead * kUnit;  // keys that a range's start and end count for
-  p->nt = row_tile(own, a.max_length ? a.s.batch * (a.max_length + kStart) : 0, all, prefix ? prefix + kStart : 0);
+  p->nt = nt;
   const int tile = 8 * p->nt;
   p->s_tiles = (int)((own + tile - 1) / tile);
   p->p_tiles = prefix > 0 ? (int)((all + tile - 1) / tile) : 0;
@@ -999,7 +982,29 @@ bool plan_split(const CacheAttnCall& a, int sms, SplitPlan* p) {
   p->part_bytes = up256((size_t)slots * a.c.hp * 4);
   p->ml_bytes = up256((size_t)slots * 8);
   p->pieces_bytes = up256((size_t)ranges * 8);
+  p->bytes = p->part_bytes + p->ml_bytes + p->pieces_bytes;
   return true;
+}
+
+// Rows of a warp, in eights: a step costs about as much for its widening as for
+// 16 rows, so the tiles are those that cost least together, over the keys of the
+// prefix and of the sequences (24 rows as one tile 25.5 us, as two of 16 27.1; 128
+// single tokens on 2000 rows in 4 bits behind 16 shared ones, where the prefix's 512
+// rows alone would take three, 205 -> 91), among those that `room` bytes hold.
+bool plan_split(const CacheAttnCall& a, int sms, size_t room, SplitPlan* p) {
+  constexpr double kStart = kLead * kUnit;  // keys that a range's start and end count for
+  const double own_keys = a.max_length ? a.s.batch * (a.max_length + kStart) : 0.0;
+  const double prefix_keys = a.prefix_width ? (double)a.prefix_width * a.c.page_size + kStart : 0.0;
+  bool found = false;
+  double least = 0.0;
+  for (int nt = 1; nt <= 3; ++nt) {
+    SplitPlan t;
+    if (!plan_rows(a, nt, sms, &t) || t.bytes > room) continue;
+    const int64_t all = ((int64_t)a.tokens * (a.q_heads / a.c.kv_heads) * a.s.batch + 8 * nt - 1) / (8 * nt);
+    const double cost = (2.0 + nt) * ((double)t.s_tiles * own_keys + (double)all * prefix_keys);
+    if (!found || cost < least) found = true, least = cost, *p = t;
+  }
+  return found;
 }
 
 template <int kFmt, int kHP, int kNT>
@@ -1041,7 +1046,7 @@ struct CachePlan {
   int slice;
   SplitPlan split;
   CacheAttnCall call;  // of the split kernel: without a prefix that the tile kernel takes
-  size_t split_bytes, bytes;
+  size_t bytes;
 };
 
 // The tile kernels widen a key set once for all its rows and then take 256 rows
@@ -1074,15 +1079,14 @@ CacheCost cost_of(const CacheAttnCall& a, bool prefix, int64_t rows, int64_t key
 constexpr size_t kTileWorkspace = (size_t)1 << 30;
 
 // The plan of the largest equal slices of the batch that fit; false: not even one sequence does.
-bool plan_slices(const CacheAttnCall& a, int sms, CacheTilePlan* t, int* slice) {
+bool plan_slices(const CacheAttnCall& a, int sms, size_t room, CacheTilePlan* t, int* slice) {
   const int64_t batch = a.s.batch;
   CacheAttnCall part = a;
   for (int64_t n = 1;;) {
     *slice = part.s.batch = (int)((batch + n - 1) / n);
-    const bool ok = plan_cache_tile(part, false, sms, t);
-    if (ok && t->workspace_bytes <= kTileWorkspace) return true;
+    if (plan_cache_tile(part, false, sms, room, t)) return true;
     if (part.s.batch == 1) return false;
-    const int64_t more = ok ? n * (int64_t)((t->workspace_bytes + kTileWorkspace - 1) / kTileWorkspace) : 2 * n;
+    const int64_t more = t->workspace_bytes && room ? n * (int64_t)std::min<size_t>((t->workspace_bytes + room - 1) / room, batch) : 2 * n;
     n = std::min(batch, std::max(n + 1, more));
   }
 }
@@ -1097,38 +1101,58 @@ bool plan_slices(const CacheAttnCall& a, int sms, CacheTilePlan* t, int* slice) 
 // in us, 8 bits: 200 tokens on 8192 rows behind 16 shared ones 147 / 144 / 87; 72 x 5 on 8 behind 16
 // 38 / 46 / 70; 8 x 20 on 200 behind 300 28 / 44 / 44; 32 x 8 on 200 behind 4096 107 / 65 / 82; 128 x 1
 // on 8 behind 1000, one of those that the rule misses, 35 / 31 / 99.
-bq4_status plan_cache(const CacheAttnCall& a, int sms, CachePlan* p) {
+//
+// The plan is the best one that a workspace of `room` bytes holds.  That of the best plan for a
+// bound of the lengths holds one for every smaller bound too: with the same kernels, row tile,
+// chunks and slices each part takes no more.
+bq4_status plan_cache(const CacheAttnCall& a, int sms, size_t room, CachePlan* p) {
   const int group = a.q_heads / a.c.kv_heads;
   const int64_t own = (int64_t)a.tokens * group, all = own * a.s.batch;
   const int64_t prefix = (int64_t)a.prefix_width * a.c.page_size;
   const CacheCost cs = cost_of(a, false, own, a.max_length, sms), cp = cost_of(a, true, all, prefix, sms);
   const bool has_p = prefix > 0;
-  double by_split = kSplitStart + cs.split + (has_p ? cp.split : 0.0);
-  double by_both = kSplitStart + kTileStart + cs.split + cp.tile;
-  double by_tile = kTileStart + cs.tile + (has_p ? kTileStart + cp.tile : 0.0);
-  // BQ4_CACHE_TILE (tests): 0 none, p for the prefix alone, else wherever a workspace fits
-  if (const char* f = getenv("BQ4_CACHE_TILE")) {
-    by_split = f[0] == '0' ? 0.0 : 3.0;
-    by_both = f[0] == '0' ? 3.0 : f[0] == 'p' ? 0.0 : 2.0;
-    by_tile = f[0] == '0' || f[0] == 'p' ? 3.0 : 1.0;
+  struct Option {
+    double cost;
+    bool tile_p, tile_s;
+  } options[3];
+  int count = 0;
+  auto option = [&](double cost, bool tile_p, bool tile_s) {
+    int at = count++;
+    for (; at > 0 && cost < options[at - 1].cost; --at) options[at] = options[at - 1];
+    options[at] = {cost, tile_p, tile_s};
+  };
+  // BQ4_CACHE_TILE (tests): 0 none, p for the prefix alone, else wherever they can
+  const char* f = getenv("BQ4_CACHE_TILE");
+  auto cost = [&](double fitted, double forced) { return f ? forced : fitted; };
+  const bool none = f && f[0] == '0', half = f && f[0] == 'p';
+  option(cost(kSplitStart + cs.split + (has_p ? cp.split : 0.0), none ? 0.0 : 3.0), false, false);
+  if (has_p) option(cost(kSplitStart + kTileStart + cs.split + cp.tile, none ? 3.0 : half ? 0.0 : 2.0), true, false);
+  if (a.max_length > 0)
+    option(cost(kTileStart + cs.tile + (has_p ? kTileStart + cp.tile : 0.0), none || half ? 3.0 : 1.0), has_p, true);
+  for (int i = 0; i < count; ++i) {
+    size_t left = room;
+    p->tile_p = options[i].tile_p;
+    p->tile_s = options[i].tile_s;
+    p->call = a;
+    p->bytes = 0;
+    if (p->tile_p) {
+      if (!plan_cache_tile(a, true, sms, std::min(left, kTileWorkspace), &p->p)) continue;
+      p->bytes = p->p.workspace_bytes;
+      left -= p->bytes;
+      p->call.prefix_width = 0, p->call.prefix_table = nullptr, p->call.prefix_length = nullptr;
+    }
+    if (p->tile_s) {
+      if (!plan_slices(a, sms, std::min(left, kTileWorkspace), &p->s, &p->slice)) continue;
+      p->bytes += p->s.workspace_bytes;
+    } else {
+      if (!plan_split(p->call, sms, left, &p->split)) continue;
+      p->bytes += p->split.bytes;
+    }
+    return BQ4_OK;
   }
-  p->tile_p = p->tile_s = false;
-  p->slice = 0;
-  if (has_p && (by_both < by_split || by_tile < by_split))
-    p->tile_p = plan_cache_tile(a, true, sms, &p->p) && p->p.workspace_bytes <= kTileWorkspace;
-  if ((!has_p || p->tile_p) && by_tile < (p->tile_p ? by_both : by_split) && a.max_length > 0)
-    p->tile_s = plan_slices(a, sms, &p->s, &p->slice);
-  if (p->tile_p && !p->tile_s && by_both >= by_split) p->tile_p = false;
-  p->call = a;
-  if (p->tile_p) p->call.prefix_width = 0, p->call.prefix_table = nullptr, p->call.prefix_length = nullptr;
-  p->split_bytes = 0;
-  if (!p->tile_s) {
-    if (!plan_split(p->call, sms, &p->split))
-      return set_error(BQ4_EINVAL_SHAPE, "cache attention: too many rows for one launch");
-    p->split_bytes = p->split.part_bytes + p->split.ml_bytes + p->split.pieces_bytes;
-  }
-  p->bytes = p->split_bytes + (p->tile_s ? p->s.workspace_bytes : 0) + (p->tile_p ? p->p.workspace_bytes : 0);
-  return BQ4_OK;
+  if (room == SIZE_MAX) return set_error(BQ4_EINVAL_SHAPE, "cache attention: too many rows for one launch");
+  bq4_status st = plan_cache(a, sms, SIZE_MAX, p);
+  return st ? st : set_error(BQ4_EWORKSPACE, "workspace of %zu bytes; cache attention needs %zu", room, p->bytes);
 }
 
 bq4_status run_split(const CacheAttnCall& a, const SplitPlan& p, bool finish, void* workspace, CacheJoinSource* prefix,
@@ -1187,16 +1211,18 @@ bq4_status run_join(const JoinArgs& g, cudaStream_t stream) {
 
 bq4_status cache_attn_workspace(const CacheAttnCall& a, int sms, size_t* bytes) {
   CachePlan p;
-  bq4_status st = plan_cache(a, sms, &p);
+  bq4_status st = plan_cache(a, sms, SIZE_MAX, &p);
   if (st) return st;
   *bytes = p.bytes;
   return BQ4_OK;
 }
 
-bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, cudaStream_t stream) {
+bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, size_t workspace_bytes,
+                          cudaStream_t stream) {
   CachePlan p;
-  bq4_status st = plan_cache(a, sms, &p);
+  bq4_status st = plan_cache(a, sms, workspace ? workspace_bytes : 0, &p);
   if (st) return st;
+  if (reinterpret_cast<uintptr_t>(workspace) % 256) return set_error(BQ4_EALIGN, "workspace not 256-byte aligned");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   JoinArgs g = {};
   g.a = a;
@@ -1209,7 +1235,7 @@ bq4_status run_cache_attn(const CacheAttnCall& a, int sms, void* workspace, cuda
     st = run_split(p.call, p.split, alone, ws, &gp, &g.s, stream);
     if (st) return st;
     if (alone) g.p = gp;
-    ws += p.split_bytes;
+    ws += p.split.bytes;
   }
   if (p.tile_p) {
     // the prefix's keys are widened while the sequences' own CTAs end: 128 sequences behind 16384

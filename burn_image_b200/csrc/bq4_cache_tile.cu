@@ -702,7 +702,8 @@ cudaError_t launch_widen(const TileArgs& s, unsigned grid, bool beside, cudaStre
 
 }  // namespace
 
-bool plan_cache_tile(const CacheAttnCall& a, bool prefix, int sms, CacheTilePlan* p) {
+bool plan_cache_tile(const CacheAttnCall& a, bool prefix, int sms, size_t room, CacheTilePlan* p) {
+  p->workspace_bytes = 0;
   const int group = a.q_heads / a.c.kv_heads;
   const int64_t rows = (int64_t)a.tokens * group * (prefix ? a.s.batch : 1);
   const int64_t keys = prefix ? (int64_t)a.prefix_width * a.c.page_size : a.max_length;
@@ -714,27 +715,33 @@ bool plan_cache_tile(const CacheAttnCall& a, bool prefix, int sms, CacheTilePlan
   p->sets = (int)sets;
   p->tiles = (int)tiles;
   p->blocks = (int)blocks;
+  p->records = heads * blocks;
+  p->q_tiles = heads * 2 * tiles;
+  if (p->records + p->q_tiles > 0x7fffffff) return false;
+  const size_t tile = (size_t)kKeys * a.c.hp * 2;
+  p->tile_bytes = up256((size_t)p->records * tile);
+  p->consts_bytes = up256((size_t)p->records * kConsts);
+  p->q_bytes = up256((size_t)p->q_tiles * 128 * a.c.hp * 2);
+  auto bytes = [&](int64_t chunks) {  // with so many chunks of a tile
+    p->slots = heads * tiles * chunks * 256;
+    p->part_bytes = up256((size_t)p->slots * a.c.hp * 4);
+    p->ml_bytes = up256((size_t)p->slots * 8);
+    return 2 * p->tile_bytes + p->consts_bytes + p->q_bytes + p->part_bytes + p->ml_bytes;
+  };
   // chunks of a tile: as many as make waves of the GPU's SMs fullest, a chunk's start and end
   // costing about as much as three records
   double best = 0.0;
   p->span = (int)blocks;
   for (int64_t ch = 1; ch <= std::min<int64_t>(blocks, 64); ++ch) {
-    const int64_t span = (blocks + ch - 1) / ch, waves = (heads * tiles * ((blocks + span - 1) / span) + sms - 1) / sms;
+    const int64_t span = (blocks + ch - 1) / ch, chunks = (blocks + span - 1) / span;
+    const int64_t waves = (heads * tiles * chunks + sms - 1) / sms;
     const double cost = (double)waves * (span + 3) + (ch > 1 ? 2.0 : 0.0);
-    if (ch == 1 || cost < best) best = cost, p->span = (int)span;
+    if (ch == 1 || (cost < best && heads * tiles * chunks <= 0x7fffffff && bytes(chunks) <= room))
+      best = cost, p->span = (int)span;
   }
   p->chunks = (int)((blocks + p->span - 1) / p->span);
-  p->records = heads * blocks;
-  p->q_tiles = heads * 2 * tiles;
-  p->slots = heads * tiles * p->chunks * 256;
-  const size_t tile = (size_t)kKeys * a.c.hp * 2;
-  p->tile_bytes = up256((size_t)p->records * tile);
-  p->consts_bytes = up256((size_t)p->records * kConsts);
-  p->q_bytes = up256((size_t)p->q_tiles * 128 * a.c.hp * 2);
-  p->part_bytes = up256((size_t)p->slots * a.c.hp * 4);
-  p->ml_bytes = up256((size_t)p->slots * 8);
-  p->workspace_bytes = 2 * p->tile_bytes + p->consts_bytes + p->q_bytes + p->part_bytes + p->ml_bytes;
-  return heads * tiles * p->chunks <= 0x7fffffff && p->records + p->q_tiles <= 0x7fffffff;
+  p->workspace_bytes = bytes(p->chunks);
+  return p->workspace_bytes <= room;
 }
 
 bq4_status run_cache_tile(const CacheAttnCall& a, const CacheTilePlan& p, bool finish, bool beside, void* workspace,

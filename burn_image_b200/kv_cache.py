@@ -166,8 +166,9 @@ class KVCache:
         positions below lengths[b] - S + i + 1, else every row.  A query that
         sees nothing gives 0.  Returns float16 [B, S, q_heads, head_dim].
         scale: positive; None: 1 / sqrt(head_dim).  max_length: a bound of the lengths
-        known to the host, by which the keys are split (None: the page
-        table's width)."""
+        known to the host, by which the work is planned (None: the page
+        table's width, which costs time where it is far above the
+        lengths)."""
         return self._attention(query, None, None, page_table, lengths, causal, scale, max_length, out)
 
     def prefix_attention(self, query: torch.Tensor, prefix_pages: torch.Tensor, prefix_length: torch.Tensor,

@@ -642,10 +642,16 @@ BQ4_API bq4_status bq4_cache_read(const bq4_cache* cache, const bq4_cache_sequen
  * nothing gives 0.  q is f16, strided (batch, token, head) like k above; out f16
  * [batch][tokens][q_heads][head_dim], contiguous.  scale <= 0 means
  * 1/sqrt(head_dim).  max_length bounds the lengths on the host (the split of
- * the keys is planned by it; 0 means table_width * page_size).  Calls with many
- * query rows a kv head widen the cache rows once into the workspace and run on
- * tcgen05 (BQ4_CACHE_TILE=0 or 1 in the environment forbids or forces it); there
- * a visible v row that is not finite makes the whole output row NaN. */
+ * the keys is planned by it; 0, or more than that, means table_width *
+ * page_size).  Calls with many query rows a kv head widen the cache rows once
+ * into the workspace, at most 1 GiB at a time, and run on tcgen05; there a
+ * visible v row that is not finite makes the whole output row NaN.  Each call
+ * reads BQ4_CACHE_TILE in the environment (tests): 0 keeps it from them, 1 takes
+ * them wherever they can run, p for a prefix alone.
+ * The size query takes the call's own batch, tokens, q_heads and max_prefix, and
+ * as max_length the bound that the call gives, or table_width * page_size.  A call
+ * with a smaller bound or table makes do with that workspace (its plan is the
+ * best one that fits). */
 BQ4_API bq4_status bq4_cache_attention_workspace_size(const bq4_cache* cache, int64_t batch, int64_t tokens,
                                                       int64_t q_heads, int64_t max_length, int64_t max_prefix,
                                                       size_t* bytes);

@@ -825,3 +825,50 @@ def test_a_batch_of_prompts_in_slices(prefix, monkeypatch):
     at = sorted({i for s in range(1, slices) for i in (s * -(-B // slices) - 1, s * -(-B // slices))} | {0, B - 2, B - 1})
     ks, vs = ([x[0][:lengths[i]] for i in at] for x in (book.k, book.v))
     check(got[at], *attend(q[at].double(), ks, vs, True, book.pk, book.pv), staged=True)
+
+
+@pytest.mark.parametrize("S,B,Hkv,longest,prefix", [(128, 1, 8, 8192, 0), (64, 1, 8, 2432, 0), (1, 20, 2, 4000, 0),
+                                                    (40, 3, 8, 3000, 0), (1, 60, 8, 2000, 16), (9, 12, 2, 1500, 700),
+                                                    (200, 1, 8, 3000, 16)])
+def test_a_workspace_serves_every_smaller_bound(S, B, Hkv, longest, prefix):
+    # one workspace, sized for the largest bound, and calls with bounds below it (the lengths follow)
+    book = Book("q8", [longest], Hkv, 128, 16, prefix=prefix, seed=S + B)
+    c, lib, group = book.cache, L.lib(), 4
+    q = torch.randn((B, S, group * Hkv, 128), generator=book.g, device=DEV).half()
+    out = torch.empty_like(q)
+    n = ctypes.c_size_t()
+    L.check(lib.bq4_cache_attention_workspace_size(c._ref, B, S, group * Hkv, longest, prefix, ctypes.byref(n)))
+    ws = torch.empty(n.value, dtype=torch.uint8, device=DEV)
+    strides = (ctypes.c_int64 * 3)(*q.stride()[:3])
+    stream = torch.cuda.current_stream().cuda_stream
+    bounds = sorted({max(1, longest * i // 97) for i in range(98)} | {longest - 128, longest - 1, 1, 127, 128, 129})
+    for bound in bounds:
+        lengths = torch.full((B,), bound, dtype=torch.int32, device=DEV)
+        # the bound given, or all that a table of so many rows holds
+        for width, given in ((book.table.shape[1], bound), (-(-bound // 16), 0)):
+            if given == 0 and width * 16 > longest:
+                continue
+            seqs = L.CacheSequences(book.table.data_ptr(), 0, width, lengths.data_ptr(), B)
+            tail = (q.data_ptr(), strides, S, group * Hkv, 1, 0.0, out.data_ptr(), ws.data_ptr(), n.value, stream)
+            out.zero_()
+            if prefix:
+                L.check(lib.bq4_cache_prefix_attention(c._ref, book.ptable.data_ptr(), -(-prefix // 16),
+                                                       book.plen.data_ptr(), ctypes.byref(seqs), given, *tail))
+            else:
+                L.check(lib.bq4_cache_attention(c._ref, ctypes.byref(seqs), given, *tail))
+            if bound in (1, bounds[len(bounds) // 2], bounds[-1]):
+                ks, vs = [book.k[0][:bound]] * B, [book.v[0][:bound]] * B
+                check(out, *attend(q.double(), ks, vs, True, book.pk, book.pv), staged=True)
+    q4.poll_device_error()
+    with pytest.raises(Bq4Error, match="workspace"):  # a workspace that holds no plan is refused
+        L.check(lib.bq4_cache_attention(c._ref, ctypes.byref(seqs), 0, *tail[:-2], 256, stream))
+
+
+def test_the_environment_may_change_between_calls(monkeypatch):
+    book = Book("q8", [700, 300], 2, 128, 16, prefix=100, seed=81)
+    q = book.query(24, 8)
+    for setting in ("0", "1", "p", "1", "0"):
+        monkeypatch.setenv("BQ4_CACHE_TILE", setting)
+        check(book.cache.attention(q, book.table, book.lengths), *attend(q.double(), book.k, book.v, True), staged=True)
+        got = book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths)
+        check(got, *attend(q.double(), book.k, book.v, True, book.pk, book.pv), staged=True)
