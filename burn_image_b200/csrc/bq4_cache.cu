@@ -609,6 +609,7 @@ bq4_status attention(const bq4_cache* cache, const int32_t* prefix_pages, int64_
   Guard guard(cache->device);
   const int sms = device_sm_count(cache->device);
   call.s = sv;
+  call.bounded = max_length > 0;
   call.prefix_table = prefix ? prefix_pages : nullptr;
   call.prefix_length = prefix ? prefix_length : nullptr;
   call.q = static_cast<const uint16_t*>(q);
@@ -724,8 +725,11 @@ bq4_status bq4_cache_attention_workspace_size(const bq4_cache* cache, int64_t ba
   if (!bytes) return set_error(BQ4_EINVAL_ARG, "bytes is NULL");
   *bytes = 0;
   CacheAttnCall call = {};
-  st = attention_shape(cache, batch, tokens, q_heads, max_length, max_prefix, &call);
+  const bool bounded = max_length >= 0;
+  if (max_length < -((int64_t)1 << 30)) return set_error(BQ4_EINVAL_SHAPE, "max_length=%lld", (long long)max_length);
+  st = attention_shape(cache, batch, tokens, q_heads, bounded ? max_length : -max_length, max_prefix, &call);
   if (st) return st;
+  call.bounded = bounded;
   if (batch == 0 || tokens == 0) return BQ4_OK;
   st = device_ready(cache->device);
   if (st) return st;

@@ -80,6 +80,7 @@ struct CacheAttnCall {
   uint16_t* out;                 // f16 [batch][tokens][q_heads][head_dim]
   int32_t tokens, q_heads, causal;
   int32_t max_length;            // lengths are at most this
+  bool bounded;                  // the caller said so: else it is what the page table holds
   float scale;                   // of the scores
   int* err;
 };

@@ -1127,8 +1127,16 @@ bq4_status plan_cache(const CacheAttnCall& a, int sms, size_t room, CachePlan* p
   const bool none = f && f[0] == '0', half = f && f[0] == 'p';
   option(cost(kSplitStart + cs.split + (has_p ? cp.split : 0.0), none ? 0.0 : 3.0), false, false);
   if (has_p) option(cost(kSplitStart + kTileStart + cs.split + cp.tile, none ? 3.0 : half ? 0.0 : 2.0), true, false);
+  // Slices are cut by the bound of the lengths.  Where that is only the page table's width and the
+  // lengths are far below it, each still costs a slice's 40 us with most SMs idle, and the split kernel
+  // follows the lengths: 16 sequences of 128 tokens in tables 65536 rows wide take 335 us so and 146
+  // there with 500 rows each, 1396 and 1159 with 8000; of 256 tokens 387 and 274, 1472 and 2243.  So
+  // without a bound slices have to gain four times by the fit.
+  const int64_t records = (int64_t)a.s.batch * a.c.kv_heads * ((a.max_length + 127) / 128);
+  const bool slices = records * (128 * 4 * a.c.hp) > (int64_t)kTileWorkspace;
   if (a.max_length > 0)
-    option(cost(kTileStart + cs.tile + (has_p ? kTileStart + cp.tile : 0.0), none || half ? 3.0 : 1.0), has_p, true);
+    option(cost(kTileStart + cs.tile * (slices && !a.bounded ? 4.0 : 1.0) + (has_p ? kTileStart + cp.tile : 0.0),
+                none || half ? 3.0 : 1.0), has_p, true);
   for (int i = 0; i < count; ++i) {
     size_t left = room;
     p->tile_p = options[i].tile_p;

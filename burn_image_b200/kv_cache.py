@@ -201,16 +201,16 @@ class KVCache:
         width = prefix_pages.shape[0] if prefix_pages is not None else 0
         key = (shape, seqs.table_width, width, max_length)
         plan = self._plans.get(key) or self._plan(key)
-        longest, nbytes = plan
+        bound, nbytes = plan
         # a workspace of the call's own: calls on several streams, and graphs captured side by side, never share one
         ws = q.new_empty(nbytes // 2)
         tail = (q.data_ptr(), self._strides(q), shape[1], shape[2], causal, scale or 0.0,
                 out.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(self._index))
         if prefix_pages is None:
-            check(self._lib.bq4_cache_attention(self._ref, ctypes.byref(seqs), longest, *tail))
+            check(self._lib.bq4_cache_attention(self._ref, ctypes.byref(seqs), bound, *tail))
         else:
             check(self._lib.bq4_cache_prefix_attention(self._ref, prefix_pages.data_ptr(), width,
-                                                       prefix_length.data_ptr(), ctypes.byref(seqs), longest, *tail))
+                                                       prefix_length.data_ptr(), ctypes.byref(seqs), bound, *tail))
         return out
 
     def _plan(self, key):
@@ -220,10 +220,11 @@ class KVCache:
         longest = held if max_length is None else min(max_length, held)
         if longest < 0:
             raise Bq4Error(L.EINVAL_SHAPE, f"max_length={max_length}")
+        bound = 0 if max_length is None else longest  # 0: none is known
         n = ctypes.c_size_t()
-        check(self._lib.bq4_cache_attention_workspace_size(self._ref, B, S, Hq, longest or held,
+        check(self._lib.bq4_cache_attention_workspace_size(self._ref, B, S, Hq, bound or -held,
                                                            width * self.page_size, ctypes.byref(n)))
         if len(self._plans) >= 1024:
             self._plans.clear()
-        plan = self._plans[key] = (longest, n.value)
+        plan = self._plans[key] = (bound, n.value)
         return plan

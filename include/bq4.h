@@ -649,9 +649,9 @@ BQ4_API bq4_status bq4_cache_read(const bq4_cache* cache, const bq4_cache_sequen
  * reads BQ4_CACHE_TILE in the environment (tests): 0 keeps it from them, 1 takes
  * them wherever they can run, p for a prefix alone.
  * The size query takes the call's own batch, tokens, q_heads and max_prefix, and
- * as max_length the bound that the call gives, or table_width * page_size.  A call
- * with a smaller bound or table makes do with that workspace (its plan is the
- * best one that fits). */
+ * as max_length the bound that the call gives, or, where it gives none, minus
+ * table_width * page_size.  A call with a smaller bound or table makes do with
+ * that workspace (its plan is the best one that fits). */
 BQ4_API bq4_status bq4_cache_attention_workspace_size(const bq4_cache* cache, int64_t batch, int64_t tokens,
                                                       int64_t q_heads, int64_t max_length, int64_t max_prefix,
                                                       size_t* bytes);

@@ -872,3 +872,17 @@ def test_the_environment_may_change_between_calls(monkeypatch):
         check(book.cache.attention(q, book.table, book.lengths), *attend(q.double(), book.k, book.v, True), staged=True)
         got = book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths)
         check(got, *attend(q.double(), book.k, book.v, True, book.pk, book.pv), staged=True)
+
+
+def test_a_wide_table_without_a_bound():
+    # 16 sequences of up to 40 rows in tables of 65536: neither the kernels for many rows of keys that
+    # are not there, nor their workspace
+    book = Book("q8", [40, 9, 31, 40] * 4, 8, 128, 16, seed=91)
+    table = torch.zeros((16, 4096), dtype=torch.int32, device=DEV)
+    table[:, :book.table.shape[1]] = book.table
+    q = book.query(32, 32)
+    torch.cuda.reset_peak_memory_stats()
+    held_before = torch.cuda.memory_allocated()
+    got, n = launches(lambda: book.cache.attention(q, table, book.lengths))
+    assert n == 2 and torch.cuda.max_memory_allocated() - held_before < 2 ** 28
+    check(got, *attend(q.double(), book.k, book.v, True))

@@ -156,3 +156,17 @@ def test_sizes_past_their_c_fields_are_refused(what):
         sizes[what] = size
         with pytest.raises(Bq4Error, match=what):
             KVCache(**sizes)
+
+
+def test_workspace_size_arguments():
+    n, c = ctypes.c_size_t(), cache()
+
+    def size(batch=1, tokens=1, q_heads=4, max_length=64, max_prefix=0):
+        return L.lib().bq4_cache_attention_workspace_size(ctypes.byref(c), batch, tokens, q_heads, max_length,
+                                                          max_prefix, ctypes.byref(n))
+
+    for bad in (dict(max_length=-2 ** 30 - 1), dict(max_length=-2 ** 63), dict(max_length=2 ** 30 + 1),
+                dict(max_prefix=-1), dict(max_prefix=2 ** 30 + 1), dict(batch=-1), dict(tokens=-1), dict(q_heads=3),
+                dict(tokens=2 ** 31)):
+        assert size(**bad) == L.EINVAL_SHAPE, bad
+    assert size(batch=0) == size(batch=0, max_length=-64) == size(tokens=0) == L.OK and n.value == 0
