@@ -25,13 +25,16 @@ f16 (at most half a step, 2^-11 of each value): where `staged` is given, another
 import ctypes
 import math
 
+import numpy as np
 import pytest
 import torch
 
+import oracle as O
 from burn_image_b200 import KVCache, q4
 from burn_image_b200 import _lib as L
 from burn_image_b200 import f16 as F
 from burn_image_b200.q4 import Bq4Error
+from conftest import gen_q4
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -886,3 +889,102 @@ def test_a_wide_table_without_a_bound():
     got, n = launches(lambda: book.cache.attention(q, table, book.lengths))
     assert n == 2 and torch.cuda.max_memory_allocated() - held_before < 2 ** 28
     check(got, *attend(q.double(), book.k, book.v, True))
+
+
+# --------------------------------------------------------------------- calls of many rows, the whole chain
+
+@pytest.mark.parametrize("fmt", ["f16", "q8", "q4"])
+@pytest.mark.parametrize("D", [128, 120, 72, 64, 40])
+@pytest.mark.parametrize("src", [torch.float32, torch.float16])
+def test_many_rows_written_and_read_back(fmt, D, src):
+    # above the 4096 rows from which warps take several at a time; positions that begin inside their groups
+    B, S, H, page = 3, 331, 7, 48
+    g = torch.Generator(device=DEV).manual_seed(D)
+    lengths = torch.tensor([S + 13, S, 100], dtype=torch.int32, device=DEV)  # the third: 231 rows fall below 0
+    W = -(-(S + 13) // page)
+    table = torch.randperm(3 * W + 2, generator=torch.Generator().manual_seed(1)).int().to(DEV)[:3 * W].reshape(3, W)
+    c = KVCache(3 * W + 2, page, H, D, fmt, DEV)
+    c.data.fill_(0x5A)
+    k = (torch.randn((B, S, H, D), generator=g, device=DEV) * 3).to(src)
+    v = torch.randn((B, H, S, D), generator=g, device=DEV).to(src).transpose(1, 2)
+    c.append(k, v, table, lengths)
+    odd = [torch.empty(B * S * H * D + 1, dtype=src, device=DEV)[1:].view(B, S, H, D).copy_(x) for x in (k, v)]
+    d = KVCache(3 * W + 2, page, H, D, fmt, DEV)
+    d.data.fill_(0x5A)
+    d.append(*odd, table, lengths)  # rows on no 16-byte boundary
+    assert torch.equal(c.data, d.data)
+    for dtype in (torch.float32, torch.float16):
+        for extra in (0, 5):  # starts of whole and of broken groups, some below 0
+            got = c.read(table, lengths, S + 2 * extra, starts=lengths - S - extra, dtype=dtype)
+            for x, y in zip((k, v), got):
+                want = torch.zeros((B, H, S + 2 * extra, D), dtype=torch.float64, device=DEV)
+                want[:, :, extra:extra + S] = held(x, fmt).transpose(1, 2)
+                want[2, :, :S - 100 + extra] = 0.0  # positions below 0
+                if extra:  # rows before the first written one hold anything
+                    y[0, :, :extra] = 0.0
+                assert torch.equal(y, want.float().to(dtype))
+    got = c.read(table, lengths, S + 13, dtype=torch.float16)
+    assert torch.equal(got[0][1, :, :S], held(k[1], fmt).transpose(0, 1).float().half())
+    assert not got[1][1:, :, S:].any() and not got[1][2, :, 100:].any()
+    q4.poll_device_error()
+
+
+@pytest.mark.parametrize("fmt,D", [("q8", 128), ("q4", 128), ("f16", 120)])
+def test_projection_cache_attention_and_next_linear(fmt, D, rng):
+    # as a decoder layer runs them: projection with QK-norm and RoPE, k and v into the cache, attention of
+    # the newest tokens, the next linear; a prompt, then tokens one by one, the last of them from a graph.
+    # Each step is held to its own inputs in 64 bits: attention as above, linears to the library's 5e-3.
+    B, Hq, Hkv, K = 2, 8, 2, 256
+    N = (Hq + 2 * Hkv) * D
+    w, s = gen_q4(K, N, 128, O.LAYOUT_ROW, rng)
+    w2, s2 = gen_q4(1024, K, 128, O.LAYOUT_ROW, rng)
+    dev = lambda a: torch.from_numpy(a.view(np.int32) if a.dtype == np.uint32 else a).to(DEV)  # noqa: E731
+    qkv_w = q4.PreparedQ4Weight(dev(w), dev(s), K, N, 128, O.LAYOUT_ROW, DEV)
+    out_w = q4.PreparedQ4Weight(dev(w2), dev(s2), 1024, K, 128, O.LAYOUT_ROW, DEV)
+    wide = O.unpack(w2, s2, 1024, K, 128, O.LAYOUT_ROW)
+    gamma = torch.rand(D, device=DEV) + 0.5
+    angle = torch.arange(128, device=DEV)[:, None] * (100.0 ** (-torch.arange(0, D, 2, device=DEV) / D))[None]
+    cos, sin = (f(angle).repeat_interleave(2, 1).contiguous() for f in (torch.cos, torch.sin))
+    c = KVCache(2 * 8, 16, Hkv, D, fmt, DEV)
+    table = torch.randperm(16, generator=torch.Generator().manual_seed(2)).int().to(DEV).reshape(2, 8)
+    lengths = torch.zeros(B, dtype=torch.int32, device=DEV)
+    ks, vs = [torch.zeros((0, Hkv, D), dtype=torch.float64, device=DEV)] * B, [torch.zeros((0, Hkv, D),
+                                                                                      dtype=torch.float64, device=DEV)] * B
+
+    def layer(x, cos, sin, S):
+        y = qkv_w.linear_qk_norm_rope(x, Hq, Hkv, D, gamma_q=gamma, gamma_k=gamma, cos=cos, sin=sin,
+                                      out_dtype=torch.float16)
+        q, k, v = y.view(B, S, Hq + 2 * Hkv, D).split([Hq, Hkv, Hkv], 2)
+        c.append(k, v, table, lengths)
+        a = c.attention(q, table, lengths)
+        padded = torch.nn.functional.pad(a.view(B * S, Hq * D), (0, 1024 - Hq * D))
+        return q, k, v, a, out_w.linear_ex(padded, out_dtype=torch.float32)
+
+    def verify(q, k, v, a, z):
+        for b in range(B):
+            ks[b], vs[b] = torch.cat([ks[b], held(k[b], fmt)]), torch.cat([vs[b], held(v[b], fmt)])
+        check(a, *attend(q.double(), ks, vs, True), staged=True)
+        flat = torch.nn.functional.pad(a.reshape(-1, Hq * D), (0, 1024 - Hq * D)).double().cpu().numpy()
+        assert O.rel_frobenius(z.cpu().numpy(), flat @ wide) <= 5e-3
+
+    at = 0
+    for S in (37, 1, 5, 1):
+        lengths += S
+        x = torch.randn((B * S, K), device=DEV)
+        verify(*layer(x, cos[at:at + S].repeat(B, 1), sin[at:at + S].repeat(B, 1), S))
+        at += S
+    x, ct, st = torch.randn((B, K), device=DEV), cos[:B].clone(), sin[:B].clone()
+    lengths += 1
+    layer(x, ct, st, 1)  # warm-up at the next position; the replays below write it again
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = layer(x, ct, st, 1)
+    for step in range(3):
+        lengths.fill_(at + step + 1)
+        x.copy_(torch.randn((B, K), device=DEV))
+        ct.copy_(cos[at + step].expand(B, -1)), st.copy_(sin[at + step].expand(B, -1))
+        graph.replay()
+        torch.cuda.synchronize()
+        verify(*got)
+    q4.poll_device_error()
