@@ -20,9 +20,10 @@
 //           not exist, and w = 2^-e; whether some lv is not 0 and some e is not.
 //           (k rounded to f16 instead, without a factor a score, gained 7 %: not
 //           worth its error.)
-// A visible v row with a value that is not finite would carry 0 * NaN into the
-// rows that do not see it: it is stored as 0 and its key gets ck = NaN, so that
-// every output of a row that sees it is NaN.
+// A v value that is not finite would carry 0 * NaN into the rows that do not see
+// it.  It is stored as 0 and its key marked: the rows that see the key take it from
+// the cache at their end.  (A row of 8 bits has one scale: its key gets ck = NaN,
+// as one of a k that is not finite does.)
 //
 // cache_tile_kernel, one CTA for 256 rows and a range of records:
 //   warp 0        bulk copies of the records (2 stages), q tiles once
@@ -57,7 +58,7 @@ namespace {
 constexpr int kKeys = 128;                   // keys of a record
 constexpr int kTThreads = 384;
 constexpr int kRing = 2;                     // stages of k and of v
-constexpr uint32_t kConsts = kKeys * 12 + 16;  // bytes of a record's consts
+constexpr uint32_t kConsts = kKeys * 12 + 32;  // bytes of a record's consts
 constexpr float kTNone = -1e30f;             // the maximum of no score
 // log2 units: m is set 2^6 below the maximum and moves when p would pass 2^14, so
 // that f16 holds p to its 2^-11 down to 2^-20 of the row's largest (a small p
@@ -66,7 +67,8 @@ constexpr float kTHead = 6.0f, kTJump = 14.0f;
 
 struct Consts {
   float ck[kKeys], lv[kKeys], w[kKeys];
-  int flags;  // 1: some lv is not 0; 2: some e is not
+  unsigned odd[4];  // a bit for each key with a v value that is not finite
+  int flags;        // 1: some lv is not 0; 2: some e is not; 4: some bit of odd is set
   int pad[3];
 };
 static_assert(sizeof(Consts) == kConsts, "a record's consts are copied in 16-byte units");
@@ -150,7 +152,7 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
   __shared__ int64_t at[kKeys];                // byte of the key's step in the cache, -1: no such row
   __shared__ int place[kKeys];
   __shared__ float sk[kKeys][kNb], sv[kKeys][kNb], ck[kKeys];
-  __shared__ int flags[4];
+  __shared__ unsigned flags[4], odd_v[4];
   __shared__ uint16_t vt[kKeys * kPitch];
   const int64_t rec = blockIdx.x;
   const int j = (int)(rec % s.blocks);
@@ -163,6 +165,7 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
     int64_t where = -1;
     float f = s.c;
     int e_v = 0;
+    bool some_v = false;  // some v of the row is not finite
     if (pos < n) {
       const unsigned u = (unsigned)pos / kCachePageUnit;
       const int pi = (int)((u * s.page_magic) >> 38);
@@ -174,13 +177,16 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
         if constexpr (kFmt != BQ4_CACHE_F16) {
           const uint16_t* sc = reinterpret_cast<const uint16_t*>(step + 32 * kRow) + (place[tid] & 15) * 2 * kNb;
           float ktop = 0.0f, most = 0.0f;
-          bool odd = false;
+          bool odd = false;  // the row's scores are NaN
 #pragma unroll
           for (int e = 0; e < kNb; ++e) {
             sk[tid][e] = __uint_as_float((uint32_t)sc[e] << 16);
             float w = __uint_as_float((uint32_t)sc[kNb + e] << 16);
-            odd |= !(w <= 3.402823466e38f) || !(sk[tid][e] <= 3.402823466e38f);
-            if (!(w <= 3.402823466e38f)) w = 0.0f;
+            odd |= !(sk[tid][e] <= 3.402823466e38f);
+            if (!(w <= 3.402823466e38f)) {
+              w = 0.0f;
+              (kFmt == BQ4_CACHE_Q8 ? odd : some_v) = true;
+            }
             sv[tid][e] = w;
             ktop = fmaxf(ktop, sk[tid][e]);
             most = fmaxf(most, w);
@@ -211,10 +217,13 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
     s.consts[rec].lv[tid] = where < 0 ? -INFINITY : (float)e_v;
     s.consts[rec].w[tid] = __uint_as_float((uint32_t)(127 - e_v) << 23);
     const bool weighted = __any_sync(0xffffffffu, e_v > 0), partial = __any_sync(0xffffffffu, where < 0);
-    if ((tid & 31) == 0) flags[tid >> 5] = weighted ? 3 : partial ? 1 : 0;
+    const unsigned marked = __ballot_sync(0xffffffffu, some_v);
+    if ((tid & 31) == 0) {
+      flags[tid >> 5] = weighted ? 3 : partial ? 1 : 0;
+      odd_v[tid >> 5] = marked;
+    }
   }
   __syncthreads();
-  if (tid == 0) s.consts[rec].flags = flags[0] | flags[1] | flags[2] | flags[3];
 
   uint8_t* kd = s.k + rec * kTile;
 #pragma unroll 4
@@ -237,7 +246,7 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
           if ((vw[e] & 0x7c00u) == 0x7c00u) odd = true, vw[e] &= 0xffff0000u;
           if ((vw[e] & 0x7c000000u) == 0x7c000000u) odd = true, vw[e] &= 0xffffu;
         }
-        if (odd) ck[key] = __int_as_float(0x7fc00000);
+        if (odd) atomicOr(&odd_v[key >> 5], 1u << (key & 31));
       } else {
         float kx[8], vx[8];
         if constexpr (kFmt == BQ4_CACHE_Q8) {
@@ -283,6 +292,10 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const __grid_constant_
   }
   __syncthreads();
   if (tid < kKeys) s.consts[rec].ck[tid] = ck[tid];
+  if (tid < 4) s.consts[rec].odd[tid] = odd_v[tid];
+  if (tid == 0)
+    s.consts[rec].flags = flags[0] | flags[1] | flags[2] | flags[3] |
+                          ((odd_v[0] | odd_v[1] | odd_v[2] | odd_v[3]) ? 4 : 0);
 
   // ---- v transposed: 8 lanes write the 8 pieces (8 keys each) of one value's 64 keys
   uint8_t* vd = s.v + rec * kTile;
@@ -381,6 +394,40 @@ struct TileSmem {
   static constexpr uint32_t kOffBars = kOffConsts + kRing * kConsts;
   static constexpr uint32_t kBytes = kOffBars + 256;
 };
+
+// Adds the v values that are not finite of the keys that a row sees, among nblk records, to its
+// results: out_row of the output or (finish not set) slot of the partial ones.
+__device__ __noinline__ void add_not_finite(const TileArgs& s, int set, int kvh, int j0, int nblk, int see,
+                                            int64_t out_row, int64_t slot) {
+  const CacheView& c = s.a.c;
+  const int32_t* table = s.prefix ? s.a.prefix_table : s.a.s.table + set * s.a.s.table_stride;
+  const Consts* k = s.consts + ((int64_t)set * c.kv_heads + kvh) * s.blocks + j0;
+  for (int j = 0; j < nblk; ++j, ++k) {
+    if (!(k->flags & 4)) continue;
+    for (int i = 0; i < kKeys; ++i) {
+      const int pos = (j0 + j) * kKeys + i;
+      if (!(k->odd[i >> 5] >> (i & 31) & 1) || pos >= see) continue;
+      const int pi = pos / c.page_size, place = pos - pi * c.page_size;
+      const uint8_t* step = cache_step(c, table[pi], kvh, place);
+      for (int d = 0; d < c.head_dim; ++d) {
+        float x;
+        if (c.format == BQ4_CACHE_F16)
+          x = __half2float(*reinterpret_cast<const __half*>(step + 16 * c.row_bytes +
+                                                            cache_swizzle(1, c.row_bytes, place & 15, 2 * d)));
+        else
+          x = __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(
+                                  step + 32 * c.row_bytes)[((place & 15) * 2 + 1) * c.nb + d / kCacheBlock] << 16);
+        if (fabsf(x) <= 3.402823466e38f) continue;
+        if (s.finish) {
+          __half* o = reinterpret_cast<__half*>(s.a.out) + out_row * c.head_dim + d;
+          *o = __float2half_rn(__half2float(*o) + x);
+        } else {
+          s.part[slot * c.hp + d] += x;
+        }
+      }
+    }
+  }
+}
 
 template <int kHP>
 __global__ void __launch_bounds__(kTThreads, 1) cache_tile_kernel(const __grid_constant__ TileArgs s) {
@@ -567,6 +614,7 @@ __global__ void __launch_bounds__(kTThreads, 1) cache_tile_kernel(const __grid_c
     const uint32_t t_s = t_lane + (uint32_t)t * 128, t_o = t_lane + kColO + (uint32_t)t * 128;
     float m = kTNone, l = 0.0f;
     bool ok = true;
+    int seen_flags = 0;
     uint32_t r[64];
     for (int j = 0; j < nblk && ok; ++j) {
       const int st = j % kRing;
@@ -578,7 +626,8 @@ __global__ void __launch_bounds__(kTThreads, 1) cache_tile_kernel(const __grid_c
       const int valid = see - (j0 + j) * kKeys;
       const int flags = k->flags;
       const bool weighted = flags & 2;
-      const bool plain = !flags && __all_sync(0xffffffffu, valid >= kKeys);
+      seen_flags |= flags;
+      const bool plain = !(flags & 1) && __all_sync(0xffffffffu, valid >= kKeys);
       attn_ld64(t_s, r);
       float top = plain ? scores64<true>(r, k, 0, valid) : scores64<false>(r, k, 0, valid);
 #pragma unroll
@@ -650,6 +699,7 @@ __global__ void __launch_bounds__(kTThreads, 1) cache_tile_kernel(const __grid_c
         }
       }
       if (!s.finish && r0 < rows) s.ml[slot] = make_float2(m, l);
+      if ((seen_flags & 4) && r0 < rows) add_not_finite(s, set, kvh, j0, nblk, see, row, slot);
     }
   }
   ptx::tc_fence_before();

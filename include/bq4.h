@@ -643,11 +643,12 @@ BQ4_API bq4_status bq4_cache_read(const bq4_cache* cache, const bq4_cache_sequen
  * [batch][tokens][q_heads][head_dim], contiguous.  scale <= 0 means
  * 1/sqrt(head_dim).  max_length bounds the lengths on the host (the split of
  * the keys is planned by it; 0, or more than that, means table_width *
- * page_size).  Calls with many query rows a kv head widen the cache rows once
- * into the workspace, at most 1 GiB at a time, and run on tcgen05; there a
- * visible v row that is not finite makes the whole output row NaN.  Each call
- * reads BQ4_CACHE_TILE in the environment (tests): 0 keeps it from them, 1 takes
- * them wherever they can run, p for a prefix alone.
+ * page_size).  A k value that is not finite makes the scores with its row so; a v
+ * value makes the outputs so that it adds to (of 4 bits its block's, of 8 bits
+ * its row's), for the queries that see it.  Calls with many query rows a kv head
+ * widen the cache rows once into the workspace, at most 1 GiB at a time, and run
+ * on tcgen05.  Each call reads BQ4_CACHE_TILE in the environment (tests): 0 keeps
+ * it from those kernels, 1 takes them wherever they can run, p for a prefix alone.
  * The size query takes the call's own batch, tokens, q_heads and max_prefix, and
  * as max_length the bound that the call gives, or, where it gives none, minus
  * table_width * page_size.  A call with a smaller bound or table makes do with

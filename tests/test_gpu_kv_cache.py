@@ -988,3 +988,42 @@ def test_projection_cache_attention_and_next_linear(fmt, D, rng):
         torch.cuda.synchronize()
         verify(*got)
     q4.poll_device_error()
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q4", "q8"])
+def test_a_value_that_is_not_finite_stays_where_it_is(fmt, path):
+    # one v value of NaN or infinity: what holds it (the value, a 4-bit block, an 8-bit row) reaches the
+    # outputs of the queries that see it, there only, whichever kernels run; with keys on other CTAs,
+    # a shared prefix, and D short of the padded head
+    D, S, n, prefix = 120, 40, 900, 300
+    book = Book(fmt, [n, 50], 2, D, 16, prefix=prefix, seed=101, poison=True)
+    q = book.query(S, 8)
+    for bad, d, at in ((math.nan, 77, n - 9), (math.inf, 3, n - 30), (-math.inf, 119, 200), (math.nan, 64, -50)):
+        x, y = book.rows(1, 2, D)[None], book.rows(1, 2, D)[None].clone()
+        y[0, 0, 1, d] = bad  # kv head 1
+        if at < 0:           # a row of the prefix, which every query sees
+            book.cache.append(x, y, book.ptable[None], book.plen + at + 1)
+            at += prefix
+            book.pk[at], book.pv[at] = held(x[0, 0], fmt), held(y[0, 0], fmt)
+        else:
+            book.cache.append(x, y, book.table[:1], book.lengths[:1] - n + at + 1)
+            book.k[0][at], book.v[0][at] = held(x[0, 0], fmt), held(y[0, 0], fmt)
+        for pre in (False, True):
+            if pre:
+                got = book.cache.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths)
+            else:
+                got = book.cache.attention(q, book.table, book.lengths)
+            q4.poll_device_error()
+            exact, mag, top = attend(q.double(), book.k, book.v, True, *((book.pk, book.pv) if pre else ()))
+            # the formula's 0 * NaN of keys that a query does not see is not meant: recompute those
+            for i in range(S):
+                seen = [x[:len(x) - S + i + 1] for x in book.k], [x[:len(x) - S + i + 1] for x in book.v]
+                e, m, _ = attend(q.double()[:, i:i + 1], *seen, False, *((book.pk, book.pv) if pre else ()))
+                exact[:, i:i + 1], mag[:, i:i + 1] = e, m
+            fine = exact.isfinite()
+            assert torch.equal(got.isfinite(), fine)
+            if fmt == "f16":
+                assert torch.equal(got.isposinf(), exact.isposinf()) and torch.equal(got.isneginf(), exact.isneginf())
+            zero = torch.zeros((), dtype=torch.float64, device=DEV)
+            check(torch.where(fine, got.double(), zero), torch.where(fine, exact, zero), mag.nan_to_num(0, 0, 0), top,
+                  staged=True)
