@@ -129,7 +129,12 @@ struct TakeRead {
 // Calls of more rows than this (k and v, of all heads) take kMany: 8 rounds a warp
 // read 557056 rows of 8 bits in 43.5 us (4: 45.2, 2: 51.9), 2 rounds the 512 of a
 // decode step in 2.3 (4: 2.8, 8: 3.2); 1 round a warp writes 2590 in 3.0 us (4: 4.3).
-constexpr int64_t kManyRows = 4096;
+// Around the switch, few / many in us, f16 rows of 128: 8 bits written 4096 rows
+// 3.3 / 5.4, 8192 3.9 / 5.5, 16384 5.9 / 6.2, 32768 8.9 / 8.2, read 2.5 / 3.4, 2.7 / 3.5,
+// 3.6 / 3.5, 4.8 / 4.4; 4 bits written 3.2 / 5.7, 4.0 / 5.8, 6.0 / 6.4, 9.3 / 10.6, read
+// 2.8 / 4.9, 3.0 / 4.8, 3.9 / 5.0, 6.0 / 6.0; f16 written 2.4 / 3.2, 2.9 / 3.3, 3.8 / 3.7,
+// 5.9 / 4.6, read 2.4 / 3.2, 2.6 / 3.2, 3.1 / 3.3, 4.2 / 4.0.
+constexpr int64_t kManyRows = 16384;
 
 struct AppendArgs {
   CacheView c;

@@ -897,10 +897,10 @@ def test_a_wide_table_without_a_bound():
 @pytest.mark.parametrize("D", [128, 120, 72, 64, 40])
 @pytest.mark.parametrize("src", [torch.float32, torch.float16])
 def test_many_rows_written_and_read_back(fmt, D, src):
-    # above the 4096 rows from which warps take several at a time; positions that begin inside their groups
-    B, S, H, page = 3, 331, 7, 48
+    # above the 16384 rows from which warps take several at a time; positions that begin inside their groups
+    B, S, H, page = 3, 431, 7, 48
     g = torch.Generator(device=DEV).manual_seed(D)
-    lengths = torch.tensor([S + 13, S, 100], dtype=torch.int32, device=DEV)  # the third: 231 rows fall below 0
+    lengths = torch.tensor([S + 13, S, 100], dtype=torch.int32, device=DEV)  # the third: 331 rows fall below 0
     W = -(-(S + 13) // page)
     table = torch.randperm(3 * W + 2, generator=torch.Generator().manual_seed(1)).int().to(DEV)[:3 * W].reshape(3, W)
     c = KVCache(3 * W + 2, page, H, D, fmt, DEV)
