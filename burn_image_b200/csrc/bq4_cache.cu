@@ -172,9 +172,9 @@ __global__ void __launch_bounds__(kCThreads) cache_append_kernel(const __grid_co
   item /= (unsigned)a.c.kv_heads;
   const int b = (int)(item / (unsigned)a.steps), step = (int)(item - (unsigned)b * a.steps);
   const int end = seq_length(a.s, a.c.page_size, b, a.err), from = end - a.tokens, first = max(from, 0);
-  const int64_t from_here = (first & ~(kTake - 1)) + (int64_t)kTake * step;  // the last steps may pass 2^31
-  if (from_here >= end) return;
-  const int base = (int)from_here;
+  const int aligned = first & ~(kTake - 1);
+  if (step >= (end - aligned + kTake - 1) / kTake) return;  // (the last of 2^31 tokens' steps pass an int)
+  const int base = aligned + kTake * step;
   int place0;
   const int page = page_of(a.c, a.s, b, base, &place0, a.err);
   if (page < 0) return;
