@@ -49,11 +49,13 @@
 //     the common step).
 //   * Steps that every row sees whole run without any mask.
 //
-// What bounds it (148 SMs, 6.57 TB/s copied): HBM for f16 rows (16 sequences of
-// 3000 to 4352 rows of 64 values, 118 MB: 26 us, 0.68 of the copy rate); the
-// issue of instructions for 4 bits (64 sequences of 300 to 8192 rows, 314 MB:
-// 85 us, 0.56; some 350 instructions a warp and step of 2304 bytes, of which
-// 50 widen k, 70 v and 40 weigh p for the four v scales); latency for one short
+// What bounds it (148 SMs, 6.57 TB/s copied): for f16 rows HBM, and the start and
+// end of the one wave (16 sequences of 3000 to 4352 rows of 64 values, 118 MB:
+// 26.7 us, 0.67 of the copy rate); for 4 bits dependent instructions at low
+// occupancy (64 sequences of 300 to 8192 rows, 314 MB: 85 us, 0.56; some 350
+// instructions a warp and step of 2304 bytes, of which 50 widen k, 70 v and 40
+// weigh p for the four v scales, 0.54 of the issue slots with 2.8 warps a
+// scheduler, which mostly wait for an instruction before); latency for one short
 // sequence (1000 rows: 7.6 us, of which 3 are two launches' starts).
 // Taken on the way, device time: one warp a row 692 / 8502 us for one sequence
 // of 1000 rows / the 64 sequences; these tiles with 16-byte copies by each lane
@@ -136,10 +138,11 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 }
 
 // CTAs of the split kernel that an SM holds: 384 threads leave 168 registers
-// each, 512 leave 128.  16 rows a warp spill a few at 168 and still gain (a
-// draft of 24 rows, 8 bits, 32.0 -> 28.5 us against two CTAs of 255); 8 rows of
-// 4 bits keep their start values in registers at 168 (93.0 -> 91.3 us); f16's
-// ring allows three; 24 rows need 255.
+// each, 512 leave 128.  16 rows a warp of 128 values spill at 168 (28 bytes stored
+// for f16, 52 for 8 bits, 164 for 4) and still gain (a draft of 24 rows, 8 bits,
+// 32.0 -> 28.5 us against two CTAs of 255); 8 rows of 4 bits keep their start values
+// in registers at 168 (93.0 -> 91.3 us); f16's ring allows three; 24 rows take 255,
+// and spill 20 bytes for f16 and 208 for 4 bits.
 constexpr int split_per_sm(int format, int hp, int nt) {
   if (nt == 3) return 2;
   if (nt == 2) return 3;

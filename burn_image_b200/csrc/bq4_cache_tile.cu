@@ -37,7 +37,10 @@
 // What bounds it: the softmax threads' chain from S to P.  A 512-token chunk of 32
 // / 8 heads on 8704 rows of 8 bits takes 113 us (widening 13, products 92, join
 // 8 with its start hidden): 71 GFLOP, 0.37 of the bf16 peak; a record of 256 rows
-// takes 2.6 us, 1.5 at the peak.  Tried: two threads a row
+// takes 2.6 us, 1.5 at the peak.  Not tried: widening in this kernel, from raw rows
+// beside the operand stages (32,448 bytes are free; a record's 128 raw tokens take
+// 18,432 in 4 bits and 33,280 in 8, which the consts' addends and weights would have
+// to make room for).  Tried: two threads a row
 // (their exchange and the registers that it costs: 152 us), a row's 128 scores
 // in registers (spilled), equal shares of all records for every CTA instead of
 // halves of a range on 128 of 148 SMs (113 to 118 us; 103 against 99 us behind
