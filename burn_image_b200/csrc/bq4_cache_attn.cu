@@ -1161,7 +1161,7 @@ bq4_status plan_cache(const CacheAttnCall& a, int sms, size_t room, CachePlan* p
     }
     return BQ4_OK;
   }
-  if (room == SIZE_MAX) return set_error(BQ4_EINVAL_SHAPE, "cache attention: too many rows for one launch");
+  if (room == SIZE_MAX) return set_error(BQ4_EINVAL_SHAPE, "cache attention: too many rows and keys for one launch (max_length bounds the keys)");
   bq4_status st = plan_cache(a, sms, SIZE_MAX, p);
   return st ? st : set_error(BQ4_EWORKSPACE, "workspace of %zu bytes; cache attention needs %zu", room, p->bytes);
 }

@@ -1027,3 +1027,30 @@ def test_a_value_that_is_not_finite_stays_where_it_is(fmt, path):
             zero = torch.zeros((), dtype=torch.float64, device=DEV)
             check(torch.where(fine, got.double(), zero), torch.where(fine, exact, zero), mag.nan_to_num(0, 0, 0), top,
                   staged=True)
+
+
+def test_many_calls_at_once_on_several_streams(monkeypatch):
+    # every plan, on four streams: the results of calls one by one
+    book = Book("q8", [900, 300, 41], 2, 128, 16, prefix=500, seed=111)
+    c, big, one = book.cache, book.query(60, 8), book.query(1, 8)
+    calls = []
+    for setting in ("0", "1", "p"):
+        for q in (big, one):
+            calls.append((setting, lambda q=q: c.attention(q, book.table, book.lengths)))
+            calls.append((setting, lambda q=q: c.prefix_attention(q, book.ptable, book.plen, book.table, book.lengths)))
+    want = []
+    for setting, call in calls:
+        monkeypatch.setenv("BQ4_CACHE_TILE", setting)
+        want.append(call())
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(6):
+        for i, (setting, call) in enumerate(calls):
+            monkeypatch.setenv("BQ4_CACHE_TILE", setting)
+            with torch.cuda.stream(streams[(i + turn) % 4]):
+                got.append((i, call()))
+    torch.cuda.synchronize()
+    q4.poll_device_error()
+    for i, out in got:
+        assert torch.equal(out, want[i])
